@@ -8,3 +8,6 @@
 #include "router.cu"
 #include "pack.cu"
 #include "shared.cu"
+#include "latent_cache.cu"
+#include "latent_decode.cu"
+#include "latent_prefill.cu"

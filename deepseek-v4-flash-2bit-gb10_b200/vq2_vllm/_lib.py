@@ -37,6 +37,26 @@ class Vq2EpLayout(ctypes.Structure):
                                                "off_epoch", "off_count")]
 
 
+class Vq2LatentCache(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("pages", ctypes.c_longlong), ("page_size", ctypes.c_int),
+                ("latent_dim", ctypes.c_int), ("rope_dim", ctypes.c_int)]
+
+
+class Vq2LatentDecodeArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int) for n in ("B", "T", "heads", "latent_dim", "rope_dim", "page_size", "max_pages", "dtype")]
+                + [("pages", ctypes.c_longlong), ("scale", ctypes.c_float)]
+                + [(n, ctypes.c_void_p) for n in ("q", "cache", "block_table", "kv_len", "out")])
+
+
+class Vq2LatentPrefillArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int) for n in ("B", "heads", "nope_dim", "rope_dim", "v_dim", "max_q", "dtype", "total_q",
+                                             "total_k")]
+                + [("scale", ctypes.c_float)]
+                + [(n, ctypes.c_longlong) for n in ("q_stride_t", "q_stride_h", "k_stride_t", "k_stride_h", "v_stride_t",
+                                                    "v_stride_h", "r_stride_t")]
+                + [(n, ctypes.c_void_p) for n in ("q", "k_nope", "k_rope", "v", "cu_q", "cu_k", "out")])
+
+
 _SIGS = {
     "vq2_decode_workspace_size": (ctypes.c_size_t, [ctypes.c_int] * 4),
     "vq2_decode": (ctypes.c_int, [ctypes.POINTER(Vq2MoeArgs), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
@@ -93,6 +113,16 @@ _SIGS = {
     "vq2_decode_with_shared_workspace_size": (ctypes.c_size_t, [ctypes.c_int] * 5),
     "vq2_decode_with_shared": (ctypes.c_int, [ctypes.POINTER(Vq2MoeArgs), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
                                               ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "vq2_latent_row_bytes": (ctypes.c_size_t, [ctypes.c_int] * 2),
+    "vq2_latent_cache_write": (ctypes.c_int, [ctypes.POINTER(Vq2LatentCache), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
+                                              ctypes.c_longlong, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_int,
+                                              ctypes.c_int, ctypes.c_void_p]),
+    "vq2_latent_cache_read": (ctypes.c_int, [ctypes.POINTER(Vq2LatentCache), ctypes.c_void_p, ctypes.c_int, ctypes.c_int,
+                                             ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
+    "vq2_latent_decode_workspace_size": (ctypes.c_size_t, [ctypes.c_int] * 5),
+    "vq2_latent_decode": (ctypes.c_int, [ctypes.POINTER(Vq2LatentDecodeArgs), ctypes.c_void_p, ctypes.c_size_t,
+                                         ctypes.c_void_p]),
+    "vq2_latent_prefill": (ctypes.c_int, [ctypes.POINTER(Vq2LatentPrefillArgs), ctypes.c_void_p]),
     "vq2_device_status": (ctypes.c_int, [ctypes.c_int]),
     "vq2_strerror": (ctypes.c_char_p, [ctypes.c_int]),
     "vq2_version": (ctypes.c_int, []),

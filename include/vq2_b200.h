@@ -246,6 +246,77 @@ size_t vq2_decode_with_shared_workspace_size(int N, int topk, int H, int I, int 
 int vq2_decode_with_shared(const vq2_moe_args* a, const void* sw13, const void* sw2, int Is, int shared_sms,
                            void* ws, size_t ws_bytes, void* stream);
 
+/* ---- latent cache and latent attention (the attention half of a decoder layer whose keys and values
+   come from one shared latent vector a token). No counterpart in the reference plugin, whose
+   attention stays with vLLM.
+
+   One cached row per token, [pages][page_size][vq2_latent_row_bytes(L, R)] bytes, 16-byte aligned:
+   the latent c (L = latent_dim values, a multiple of 64, at most 512) in 4 bits and the rotary key
+   (R = rope_dim values, a multiple of 8, at most 64, or 0) in fp16. Per 64 values of c, with H the
+   normalised Sylvester Hadamard matrix: y = H c, s = clamp(bf16(max|y| * (1/7)), 2^-14, 2048),
+   n = clamp(rint(y / s), -7, 7); the row stands for H (n s). Bytes: L/2 of nibbles n + 8 (32-bit
+   little-endian words of 8 values, value j in bits 4 (j >> 1) + 16 (j & 1)), 2 R of fp16, 2 L/64 of
+   fp16 scales, zeros up to a multiple of 16. Values beyond 7 * 2048 (rotary part: 65504) saturate; a
+   NaN makes its group of 64 read as NaN. A slot is page * page_size + place in the page. */
+typedef struct vq2_latent_cache {
+  void* data;
+  long long pages;
+  int page_size, latent_dim, rope_dim;
+} vq2_latent_cache;
+
+size_t vq2_latent_row_bytes(int latent_dim, int rope_dim);   /* 0 for unsupported dimensions */
+/* Quantise rows c[i * c_stride ..] and k_rope[i * rope_stride ..] (VQ2_DT_*, strides in elements,
+   multiples of 8, 16-byte aligned bases) into slots[i] (VQ2_ID_*), i < n. A negative slot is skipped
+   (padding); one beyond the cache is skipped and vq2_device_status reports VQ2_ERR_SHAPE. Slots that
+   occur twice hold either row. */
+int vq2_latent_cache_write(const vq2_latent_cache* cache, const void* c, const void* k_rope, int dtype, long long c_stride,
+                           long long rope_stride, const void* slots, int slot_dtype, int n, void* stream);
+/* What slots[i] stand for: c [n][L] and k_rope [n][R] of VQ2_DT_* (zeros for a slot that write skips). */
+int vq2_latent_cache_read(const vq2_latent_cache* cache, const void* slots, int slot_dtype, int n, void* c, void* k_rope,
+                          int dtype, void* stream);
+
+/* Absorbed form: attention of T new tokens per sequence over the cache (the new tokens' own rows are in
+   it already). For query row (b, t, h): z_j = scale * (q_c . c_j + q_r . r_j) over j <= kv_len[b] - T + t,
+   out = sum_j softmax(z)_j c_j; a row that sees nothing gives zeros. Row j of sequence b is in page
+   block_table[b][j / page_size]; a page outside the cache is treated as masked and
+   vq2_device_status reports VQ2_ERR_SHAPE. kv_len is clamped to [0, max_pages * page_size]. */
+typedef struct vq2_latent_decode_args {
+  int B, T, heads, latent_dim, rope_dim;
+  int page_size, max_pages;      /* block_table is [B][max_pages] */
+  int dtype;                     /* VQ2_DT_BF16 or VQ2_DT_F16, of q and out */
+  long long pages;
+  float scale;
+  const void* q;                 /* [B][T][heads][latent_dim + rope_dim] */
+  const void* cache;
+  const int32_t* block_table;
+  const int32_t* kv_len;         /* [B] */
+  void* out;                     /* [B][T][heads][latent_dim] */
+} vq2_latent_decode_args;
+size_t vq2_latent_decode_workspace_size(int B, int T, int heads, int latent_dim, int rope_dim);
+int vq2_latent_decode(const vq2_latent_decode_args* a, void* workspace, size_t ws_bytes, void* stream);
+
+/* Expanded form: causal attention of a ragged batch of prompt chunks over per-head keys and values.
+   Sequence b: query rows cu_q[b] .. cu_q[b+1]-1, key rows cu_k[b] .. cu_k[b+1]-1 (a prefix first, then
+   the chunk's own): query i sees keys j <= i + keys - queries, so the last query sees all; a row that
+   sees nothing gives zeros. Key of head h: [k_nope[:, h], k_rope], the rotary part shared by the heads.
+   Strides in elements (multiples of 8; the last dimension is contiguous); max_q >= every
+   sequence's query rows. */
+typedef struct vq2_latent_prefill_args {
+  int B, heads, nope_dim, rope_dim, v_dim;   /* nope_dim, v_dim <= 128, rope_dim <= 64, multiples of 8 */
+  int max_q, dtype;                          /* VQ2_DT_BF16 or VQ2_DT_F16 */
+  int total_q, total_k;                      /* rows of q and of k_nope / k_rope / v */
+  float scale;
+  long long q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, r_stride_t;
+  const void* q;                             /* [total_q][heads][nope_dim + rope_dim] */
+  const void* k_nope;                        /* [total_k][heads][nope_dim] */
+  const void* k_rope;                        /* [total_k][rope_dim] */
+  const void* v;                             /* [total_k][heads][v_dim] */
+  const int32_t* cu_q;                       /* [B + 1] */
+  const int32_t* cu_k;                       /* [B + 1] */
+  void* out;                                 /* [total_q][heads][v_dim] */
+} vq2_latent_prefill_args;
+int vq2_latent_prefill(const vq2_latent_prefill_args* a, void* stream);
+
 /* Error word written by bounded device waits and device-side range checks (0 = none);
    reset = 1 clears it. Synchronises the device. */
 int vq2_device_status(int reset);
