@@ -99,7 +99,7 @@ extern "C" size_t vq2_latent_decode_workspace_size(int B, int T, int heads, int 
 extern "C" int vq2_latent_decode(const vq2_latent_decode_args* a, void* ws, size_t ws_bytes, void* stream) {
   if (!a || !a->q || !a->cache || !a->block_table || !a->kv_len || !a->out) return VQ2_ERR_NULL;
   if (a->B <= 0 || a->T <= 0 || a->heads <= 0 || a->page_size <= 0 || a->max_pages <= 0 || a->pages <= 0 ||
-      !latent_dims_ok(a->latent_dim, a->rope_dim) || (long long)a->B * a->T * a->heads > 0x7FFFFFFFLL)
+      !latent_dims_ok(a->latent_dim, a->rope_dim) || !(a->scale > 0.f) || (long long)a->B * a->T * a->heads > 0x7FFFFFFFLL)
     return VQ2_ERR_SHAPE;
   if (a->dtype != VQ2_DT_BF16 && a->dtype != VQ2_DT_F16) return VQ2_ERR_DTYPE;
   if (((uintptr_t)a->q | (uintptr_t)a->cache | (uintptr_t)a->out) & 15) return VQ2_ERR_ALIGN;

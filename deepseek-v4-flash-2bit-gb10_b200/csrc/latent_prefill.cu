@@ -4,50 +4,371 @@
 // rotary part shared by all heads:
 //   z_ij = scale * (q_i . k_j),  j <= i + keys - queries;   out_i = sum_j softmax(z_i)_j v_j
 //
-// One warp per (query row, head): the lanes hold the row's values, keys come one after another.
+// One CTA takes 256 queries of a head as two tiles of 128 and walks the keys 128 at a time, with a
+// running maximum and sum per row. Tensor memory holds, per tile, the scores S (128 columns; the
+// probabilities P overwrite them as packed 16-bit values) and the output O (128 columns): 512 in all.
+//   warp 0       TMA: 16 KB units of 128 rows x 64 values (128-byte swizzle), K then V of each key
+//                tile, through a ring; values past a dimension's end arrive as zeros
+//   warp 1       tcgen05.mma: S = Q K^T (both from shared memory), O += P V (P from tensor memory, V as it
+//                lies, rows = keys, so no transpose); the two tiles alternate, so one tile's products
+//                run under the other tile's softmax
+//   warps 4-11   softmax, one thread a query row (4 warps a tile): the row's 128 scores in registers
+// A row's maximum is refreshed only when it rose by more than 2^8 in the exponent: P then stays below
+// 256 (exact enough in 16 bits: the rounding is relative) and O is rarely rescaled.
 #include "vq2_common.cuh"
 
 namespace vq2 {
 
 constexpr int LP_MAX_D = 128;      // values a head: of the positionless key part, and of v
+constexpr int LP_TILE = 128;       // query rows a tile, key rows a step
+constexpr int LP_UNIT = LP_TILE * 128;         // bytes of a unit: 128 rows of 64 16-bit values
+constexpr int LP_RING = 8;         // units in flight: a step needs at most 3 (K) + 2 (V) at once
+constexpr int LP_THREADS = 384;
+constexpr float LP_RAISE = 8.f;    // log2 by which a row's maximum may grow before O is rescaled
+
+struct LpShared {
+  uint64_t full[LP_RING], empty[LP_RING];
+  uint64_t qfull[2], sfull[2], pfull[2], ofull[2], drain;
+  uint32_t tmem;
+  int abort;
+};
+constexpr size_t LP_SMEM = (size_t)(6 + LP_RING) * LP_UNIT + sizeof(LpShared) + 1024;
+static_assert(LP_SMEM <= 227 * 1024, "latent prefill shared memory");
+
+// Shared-memory descriptor of an operand whose rows run along the contraction (MN-major) in 128-byte
+// swizzled units of 64 columns: 8-row groups 1024 bytes apart, units of 64 columns `unit` bytes apart.
+__device__ __forceinline__ uint64_t umma_desc_mn(uint32_t saddr, uint32_t unit) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)((unit >> 4) & 0x3FFF) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
+  unsigned long long d, x, y, z;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(z) : "f"(c.x), "f"(c.y));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(x), "l"(y), "l"(z));
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
+  return r;
+}
+__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
+  unsigned long long d, x, y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
+  return r;
+}
+// 64 columns of this thread's lane; a tcgen05.wait::ld has to follow before the values are used.
+__device__ __forceinline__ void tmem_ld64(uint32_t t, float* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+               "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,"
+               "%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+                 "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+                 "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+                 "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]),
+                 "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]),
+                 "=f"(v[40]), "=f"(v[41]), "=f"(v[42]), "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]),
+                 "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]),
+                 "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
+               : "r"(t));
+}
+__device__ __forceinline__ void tmem_st64(uint32_t t, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x64.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
+               "%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,"
+               "%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,%64};"
+               ::"r"(t), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                 "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+                 "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+                 "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]),
+                 "r"(v[32]), "r"(v[33]), "r"(v[34]), "r"(v[35]), "r"(v[36]), "r"(v[37]), "r"(v[38]), "r"(v[39]),
+                 "r"(v[40]), "r"(v[41]), "r"(v[42]), "r"(v[43]), "r"(v[44]), "r"(v[45]), "r"(v[46]), "r"(v[47]),
+                 "r"(v[48]), "r"(v[49]), "r"(v[50]), "r"(v[51]), "r"(v[52]), "r"(v[53]), "r"(v[54]), "r"(v[55]),
+                 "r"(v[56]), "r"(v[57]), "r"(v[58]), "r"(v[59]), "r"(v[60]), "r"(v[61]), "r"(v[62]), "r"(v[63])
+               : "memory");
+}
+// keeps 64 registers allocated and unmodified up to this point (a store reads its sources late)
+__device__ __forceinline__ void keep_live64(const uint32_t* v) {
+#pragma unroll
+  for (int i = 0; i < 64; i += 16) keep_live16(v + i);
+}
+
+// A row's 128 scores as registers.
+__device__ __forceinline__ void tmem_ld128(uint32_t t, float* v) {
+  tmem_ld64(t, v);
+  tmem_ld64(t + 64, v + 64);
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 128; ++i) asm volatile("" : "+f"(v[i]));     // no use of a value moves before the wait
+}
 
 template <int DT>
-__global__ void __launch_bounds__(256) latent_prefill_rows_kernel(vq2_latent_prefill_args a) {
-  const int lane = threadIdx.x & 31, dn = a.nope_dim, R = a.rope_dim, dv = a.v_dim;
-  const int i = blockIdx.x * 8 + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z;
+__global__ void __launch_bounds__(LP_THREADS, 1)
+latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                      const __grid_constant__ CUtensorMap tr, const __grid_constant__ CUtensorMap tv) {
+  extern __shared__ __align__(1024) uint8_t lp_smem_raw[];
+  // block -> (sequence, head, query block): the last query block of every head and sequence first, as it has most keys
+  const int per = a.heads * a.B;
+  const int qb = nqb - 1 - (int)(blockIdx.x / per), h = (int)(blockIdx.x % per) % a.heads, b = (int)(blockIdx.x % per) / a.heads;
   // offsets are clamped to the tensors, so wrong ones give wrong rows and no access out of range
-  const int q0 = min(max(a.cu_q[b], 0), a.total_q), nq = min(max(a.cu_q[b + 1], q0), a.total_q) - q0;
+  const int q0 = min(max(a.cu_q[b], 0), a.total_q), nq = min(min(max(a.cu_q[b + 1], q0), a.total_q) - q0, a.max_q);
   const int k0 = min(max(a.cu_k[b], 0), a.total_k), nk = min(max(a.cu_k[b + 1], k0), a.total_k) - k0;
-  if (i >= min(nq, a.max_q)) return;
-  const long long qi = (long long)(q0 + i) * a.q_stride_t + (long long)h * a.q_stride_h;
-  float q[6] = {}, o[4] = {}, m = -INFINITY, l = 0.f;
-  for (int p = 0; p < 6; ++p)
-    if (lane + 32 * p < dn + R) q[p] = load_act(a.q, DT, qi + lane + 32 * p);
-  const int end = min(nk, i + 1 + nk - nq);
-  for (int j = 0; j < end; ++j) {
-    const long long kj = (long long)(k0 + j) * a.k_stride_t + (long long)h * a.k_stride_h;
-    const long long vj = (long long)(k0 + j) * a.v_stride_t + (long long)h * a.v_stride_h;
-    float z = 0.f;
-    for (int p = 0; p < 6; ++p) {
-      const int d = lane + 32 * p;
-      if (d < dn) z = fmaf(q[p], load_act(a.k_nope, DT, kj + d), z);
-      else if (d < dn + R) z = fmaf(q[p], load_act(a.k_rope, DT, (long long)(k0 + j) * a.r_stride_t + d - dn), z);
+  const int row0 = qb * 2 * LP_TILE;
+  if (row0 >= nq) return;
+  const int past = nk - nq;                       // key i + past is the newest that query i sees
+  const int ntile = nq - row0 > LP_TILE ? 2 : 1;
+  // key steps of each tile, by its last row
+  int steps[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+    steps[t] = t < ntile ? (max(0, min(nk, min(nq, row0 + (t + 1) * LP_TILE) + past)) + LP_TILE - 1) / LP_TILE : 0;
+  const int nsteps = max(steps[0], steps[1]);
+  const int kn = (a.nope_dim + 63) / 64, ku = kn + (a.rope_dim ? 1 : 0), vu = (a.v_dim + 63) / 64;   // units of a key row, of a value row
+
+  uint8_t* smem = (uint8_t*)(((uintptr_t)lp_smem_raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t qbase = smem_u32(smem), ring = qbase + 6 * LP_UNIT;
+  LpShared* sh = (LpShared*)(smem + (6 + LP_RING) * LP_UNIT);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < LP_RING; ++s) { mbar_init(&sh->full[s], 1); mbar_init(&sh->empty[s], 1); }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&sh->qfull[t], 1);
+      mbar_init(&sh->sfull[t], 1);
+      mbar_init(&sh->pfull[t], 4);
+      mbar_init(&sh->ofull[t], 1);
     }
-    z = warp_sum(z) * a.scale;
-    const float mn = fmaxf(m, z), f = expf(m - mn), e = expf(z - mn);
-    l = l * f + e;
-    for (int p = 0; p < 4; ++p)
-      if (lane + 32 * p < dv) o[p] = o[p] * f + e * load_act(a.v, DT, vj + lane + 32 * p);
-    m = mn;
+    mbar_init(&sh->drain, 1);
+    sh->abort = 0;
+    fence_mbar_init();
   }
-  for (int p = 0; p < 4; ++p) {
-    const int d = lane + 32 * p;
-    if (d >= dv) continue;
-    const long long at = ((long long)(q0 + i) * a.heads + h) * dv + d;
-    const float v = l > 0.f || l != l ? o[p] / l : 0.f;
-    if (DT == VQ2_DT_BF16) ((__nv_bfloat16*)a.out)[at] = __float2bfloat16_rn(v);
-    else ((__half*)a.out)[at] = __float2half_rn(v);
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh->tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem;
+  volatile int* abort = &sh->abort;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0 && lane == 0 && nsteps > 0) {
+      // ---------------- loader
+      for (int t = 0; t < ntile; ++t) {
+        mbar_arrive_expect_tx(&sh->qfull[t], ku * LP_UNIT);
+        for (int s = 0; s < ku; ++s)
+          tma_load_3d(qbase + (t * 3 + s) * LP_UNIT, &tq, s < kn ? s * 64 : a.nope_dim, h, q0 + row0 + t * LP_TILE, &sh->qfull[t]);
+      }
+      int g = 0;
+      for (int j = 0; j < nsteps && !*abort; ++j)
+        for (int s = 0; s < ku + vu; ++s, ++g) {
+          const int slot = g % LP_RING;
+          if (g >= LP_RING && !mbar_wait(&sh->empty[slot], ((g / LP_RING) - 1) & 1)) { *abort = 1; break; }
+          mbar_arrive_expect_tx(&sh->full[slot], LP_UNIT);
+          const CUtensorMap* m = s < kn ? &tk : s < ku ? &tr : &tv;
+          tma_load_3d(ring + slot * LP_UNIT, m, s < kn ? s * 64 : s < ku ? 0 : (s - ku) * 64, s < kn || s >= ku ? h : 0, k0 + j * LP_TILE,
+                      &sh->full[slot]);
+        }
+      // no copy is in flight when the block ends
+      for (int t = 0; t < ntile; ++t) mbar_wait(&sh->qfull[t], 0);
+      for (int q = max(0, g - LP_RING); q < g; ++q) mbar_wait(&sh->full[q % LP_RING], (q / LP_RING) & 1);
+    } else if (warp == 1 && nsteps > 0) {
+      // ---------------- products (the whole warp walks; lane 0 issues)
+      constexpr uint32_t fmt = DT == VQ2_DT_BF16 ? (1u << 7) | (1u << 10) : 0u;
+      const uint32_t id_s = (1u << 4) | fmt | ((LP_TILE >> 3) << 17) | ((LP_TILE >> 4) << 24);
+      auto id_o = [&](int n) { return (1u << 4) | fmt | (1u << 16) | ((uint32_t)((n + 15) / 16 * 2) << 17) | ((LP_TILE >> 4) << 24); };
+      const int gu = ku + vu;
+      // every lane waits and the warp agrees on the outcome, so no lane leaves a loop alone
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
+      bool ok = true;
+      int cleared = -1;
+      auto scores = [&](int t, int j) {             // S_t = Q_t K_j^T
+        for (int s = 0; s < ku; ++s) {
+          const int g = j * gu + s;
+          if (!wait(&sh->full[g % LP_RING], (g / LP_RING) & 1)) { ok = false; return; }
+          tc_fence_after();
+          const uint32_t qa = qbase + (t * 3 + s) * LP_UNIT, kb = ring + (g % LP_RING) * LP_UNIT;
+          const int cols = s < kn ? min(64, a.nope_dim - s * 64) : a.rope_dim;
+          if (lane == 0)
+            for (int ks = 0; ks * 16 < cols; ++ks)
+              umma_ss(tmem + t * 128, umma_desc_sw128(qa + ks * 32), umma_desc_sw128(kb + ks * 32), id_s, (s | ks) != 0);
+        }
+        if (lane == 0) umma_commit(&sh->sfull[t]);
+      };
+      auto release = [&](int g, int n) {            // units g .. g + n - 1 once the products issued so far are done
+        if (lane == 0)
+          for (int s = 0; s < n; ++s) umma_commit(&sh->empty[(g + s) % LP_RING]);
+      };
+      for (int t = 0; t < ntile && ok; ++t)
+        if (steps[t] > 0) {
+          if (!wait(&sh->qfull[t], 0)) { ok = false; break; }
+          scores(t, 0);
+        }
+      release(0, ku);
+      for (int j = 0; j < nsteps && ok; ++j) {
+        const int gv = j * gu + ku;
+        for (int t = 0; t < ntile && ok; ++t) {
+          if (j >= steps[t]) continue;
+          for (int s = 0; s < vu; ++s)
+            if (!wait(&sh->full[(gv + s) % LP_RING], ((gv + s) / LP_RING) & 1)) { ok = false; break; }
+          const int live = nk - j * LP_TILE;
+          if (live < LP_TILE && ok && cleared != j) {
+            cleared = j;
+            // rows past the last key belong to another sequence: their probabilities are 0, but 0 times
+            // a NaN there would reach this one's output, so they are cleared (only ever at the last step)
+            for (int s = 0; s < vu; ++s)
+              for (int i = live * 8 + lane; i < LP_TILE * 8; i += 32)
+                sts128_v(ring + ((gv + s) % LP_RING) * LP_UNIT + i * 16, make_uint4(0, 0, 0, 0));
+            fence_async_smem();
+            __syncwarp();
+          }
+          if (!ok || !wait(&sh->pfull[t], j & 1)) { ok = false; break; }
+          tc_fence_after();
+          // O_t += P_t V_j: one product over both value units where they lie side by side in the ring
+          const uint32_t v0 = ring + (gv % LP_RING) * LP_UNIT, v1 = ring + ((gv + 1) % LP_RING) * LP_UNIT;
+          const bool whole = vu == 1 || v1 == v0 + LP_UNIT;
+          if (lane == 0)
+            for (int ks = 0; ks < LP_TILE / 16; ++ks) {
+              const uint32_t p = tmem + t * 128 + ks * 8;
+              umma_ts(tmem + 256 + t * 128, p, umma_desc_mn(v0 + ks * 2048, LP_UNIT), id_o(whole ? a.v_dim : 64), (j | ks) != 0);
+              if (!whole) umma_ts(tmem + 320 + t * 128, p, umma_desc_mn(v1 + ks * 2048, LP_UNIT), id_o(a.v_dim - 64), (j | ks) != 0);
+            }
+          if (j + 1 < steps[t]) scores(t, j + 1);
+          else if (lane == 0) umma_commit(&sh->ofull[t]);
+        }
+        release(gv, vu);
+        if (j + 1 < nsteps) release(gv + vu, ku);
+      }
+      if (!ok) *abort = 1;
+      if (lane == 0) umma_commit(&sh->drain);
+      mbar_wait(&sh->drain, 0);
+    }
+  } else {
+    // ---------------- softmax: thread = query row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    const int t = (warp - 4) >> 2, r = (warp & 3) * 32 + lane, i = row0 + t * LP_TILE + r;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * 128;
+    const float sl = a.scale * 1.4426950408889634f;
+    const int seen = max(0, min(nk, i + 1 + past));           // keys 0 .. seen - 1
+    const int n = steps[t];
+    float m = -INFINITY;                                      // the maximum that P and O are relative to
+    float2 l2 = make_float2(0.f, 0.f);
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&sh->sfull[t], j & 1))) { ok = false; break; }
+      tc_fence_after();
+      float s[128];
+      tmem_ld128(ts, s);
+      const int lim = seen - j * LP_TILE;
+      if (__any_sync(0xffffffffu, lim < LP_TILE)) {
+#pragma unroll
+        for (int c = 0; c < 128; ++c) s[c] = c < lim ? s[c] : -INFINITY;
+      }
+      float m4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int c = 4; c < 128; c += 8) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m4[k] = c + 4 + k < 128 ? fmaxf(m4[k], fmaxf(s[c + k], s[c + 4 + k])) : fmaxf(m4[k], s[c + k]);
+      }
+      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+      // the first step sets the maximum; later ones raise it when it grew by more than LP_RAISE
+      const bool raise = m == -INFINITY ? mx > m : (mx - m) * sl > LP_RAISE;
+      if (__any_sync(0xffffffffu, raise) ) {
+        const float mn = raise ? mx : m, f = raise ? ex2((m - mn) * sl) : 1.f;
+        m = mn;
+        l2.x *= f;
+        l2.y *= f;
+        if (j > 0) {              // every product into O issued before this step's scores is done
+#pragma unroll 1
+          for (int c = 0; c < a.v_dim; c += 16) {
+            float o[16];
+            tmem_ld16(to + c, o);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] *= f;
+            tmem_st16(to + c, (const uint32_t*)o);
+            tmem_st_wait();
+            keep_live16((const uint32_t*)o);
+          }
+        }
+      }
+      const float mb = m == -INFINITY ? 0.f : -m * sl;
+      const float2 s2 = make_float2(sl, sl), b2 = make_float2(mb, mb);
+      float2 sum = make_float2(0.f, 0.f), sumb = sum;
+      uint32_t p[64];
+#pragma unroll
+      for (int c = 0; c < 128; c += 2) {
+        float2 x = ffma2(make_float2(s[c], s[c + 1]), s2, b2);
+        x.x = ex2(x.x);
+        x.y = ex2(x.y);
+        if (c & 2) sumb = fadd2(sumb, x);
+        else sum = fadd2(sum, x);
+        p[c >> 1] = pack2<DT>(x.x, x.y);
+      }
+      tmem_st64(ts, p);
+      l2 = fadd2(l2, fadd2(sum, sumb));
+      tmem_st_wait();
+      keep_live64(p);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->pfull[t]);
+    }
+    if (ok && n > 0 && !__all_sync(0xffffffffu, mbar_wait(&sh->ofull[t], 0))) ok = false;
+    if (!ok) *abort = 1;
+    tc_fence_after();
+    if (t < ntile) {
+      const float l = l2.x + l2.y;
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+      const long long at = ((long long)(q0 + i) * a.heads + h) * a.v_dim;
+#pragma unroll 1
+      for (int c = 0; c < a.v_dim; c += 8) {
+        float o[8];
+        if (n > 0) tmem_ld8(to + c, o);
+        if (i < nq) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) o[k] = n > 0 && l != 0.f ? o[k] * inv : 0.f;
+          store8<DT>(a.out, at + c, o);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  __syncwarp();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+// Tensor map of [rows][heads][dim] 16-bit values with element strides: boxes of 64 values x 1 head x 128 rows.
+static int lp_encode(CUtensorMap* m, const void* base, int dim, int heads, int rows, long long stride_h, long long stride_t) {
+  if (const int rc = tensor_map_ready()) return rc;
+  const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)rows};
+  // a dimension of one entry is never stepped over: any legal stride serves
+  const cuuint64_t strides[2] = {(cuuint64_t)(heads > 1 ? stride_h : (dim + 7) / 8 * 8) * 2, (cuuint64_t)(rows > 1 ? stride_t : 64 * 1024) * 2};
+  const cuuint32_t box[3] = {64, 1, LP_TILE}, one[3] = {1, 1, 1};
+  const CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, one,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? VQ2_OK : VQ2_ERR_CUDA;
 }
 
 }  // namespace vq2
@@ -58,7 +379,7 @@ extern "C" int vq2_latent_prefill(const vq2_latent_prefill_args* a, void* stream
   if (!a) return VQ2_ERR_NULL;
   if (a->B <= 0 || a->heads <= 0 || a->max_q < 0 || a->total_q < 0 || a->total_k < 0 || a->nope_dim <= 0 || a->nope_dim > LP_MAX_D ||
       a->nope_dim % 8 || a->v_dim <= 0 || a->v_dim > LP_MAX_D || a->v_dim % 8 || a->rope_dim < 0 || a->rope_dim > 64 ||
-      a->rope_dim % 8 || a->B > 65535 || a->heads > 65535)
+      a->rope_dim % 8 || !(a->scale > 0.f))
     return VQ2_ERR_SHAPE;
   if ((a->q_stride_t | a->q_stride_h | a->k_stride_t | a->k_stride_h | a->v_stride_t | a->v_stride_h | a->r_stride_t) & 7)
     return VQ2_ERR_SHAPE;
@@ -67,7 +388,20 @@ extern "C" int vq2_latent_prefill(const vq2_latent_prefill_args* a, void* stream
   if (!a->q || !a->cu_q || !a->cu_k || !a->out) return VQ2_ERR_NULL;
   if (a->total_k && (!a->k_nope || !a->v || (a->rope_dim && !a->k_rope))) return VQ2_ERR_NULL;
   if (((uintptr_t)a->q | (uintptr_t)a->k_nope | (uintptr_t)a->v | (uintptr_t)a->k_rope | (uintptr_t)a->out) & 15) return VQ2_ERR_ALIGN;
-  auto kernel = a->dtype == VQ2_DT_BF16 ? latent_prefill_rows_kernel<VQ2_DT_BF16> : latent_prefill_rows_kernel<VQ2_DT_F16>;
-  kernel<<<dim3((a->max_q + 7) / 8, a->heads, a->B), 256, 0, (cudaStream_t)stream>>>(*a);
+  const int nqb = (a->max_q + 2 * LP_TILE - 1) / (2 * LP_TILE);
+  const long long blocks = (long long)nqb * a->heads * a->B;
+  if (blocks > 0x7FFFFFFFLL) return VQ2_ERR_SHAPE;
+  CUtensorMap tq, tk, tr, tv;
+  // without keys nothing is loaded; the maps then describe q, so that they are valid
+  const bool any = a->total_k > 0;
+  int rc = lp_encode(&tq, a->q, a->nope_dim + a->rope_dim, a->heads, a->total_q, a->q_stride_h, a->q_stride_t);
+  tk = tr = tv = tq;
+  if (!rc && any) rc = lp_encode(&tk, a->k_nope, a->nope_dim, a->heads, a->total_k, a->k_stride_h, a->k_stride_t);
+  if (!rc && any) rc = lp_encode(&tv, a->v, a->v_dim, a->heads, a->total_k, a->v_stride_h, a->v_stride_t);
+  if (!rc && any && a->rope_dim) rc = lp_encode(&tr, a->k_rope, a->rope_dim, 1, a->total_k, 0, a->r_stride_t);
+  if (rc) return rc;
+  auto kernel = a->dtype == VQ2_DT_BF16 ? latent_prefill_kernel<VQ2_DT_BF16> : latent_prefill_kernel<VQ2_DT_F16>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)LP_SMEM) != cudaSuccess) return VQ2_ERR_CUDA;
+  kernel<<<(unsigned)blocks, LP_THREADS, LP_SMEM, (cudaStream_t)stream>>>(*a, nqb, tq, tk, tr, tv);
   return cudaGetLastError() == cudaSuccess ? VQ2_OK : VQ2_ERR_CUDA;
 }

@@ -852,8 +852,8 @@ __global__ void __launch_bounds__(256) had_quant_rows_warp_kernel(const float* _
 // ------------------------------------------------------------------ host
 static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 
-static int encode_2d(CUtensorMap* m, const void* base, uint64_t inner_bytes, uint64_t rows, uint32_t box_x,
-                     uint32_t box_y, bool swizzle128) {
+// Looks up the tensor-map encoder once.
+static int tensor_map_ready() {
   if (!g_encode) {
     cudaDriverEntryPointQueryResult q;
     void* fn = nullptr;
@@ -862,6 +862,12 @@ static int encode_2d(CUtensorMap* m, const void* base, uint64_t inner_bytes, uin
       return VQ2_ERR_CUDA;
     g_encode = (PFN_cuTensorMapEncodeTiled_v12000)fn;
   }
+  return VQ2_OK;
+}
+
+static int encode_2d(CUtensorMap* m, const void* base, uint64_t inner_bytes, uint64_t rows, uint32_t box_x,
+                     uint32_t box_y, bool swizzle128) {
+  if (const int rc = tensor_map_ready()) return rc;
   const cuuint64_t dims[2] = {inner_bytes, rows};
   const cuuint64_t strides[1] = {inner_bytes};
   const cuuint32_t box[2] = {box_x, box_y};

@@ -35,6 +35,8 @@ def latent_attention_decode(q: torch.Tensor, cache: LatentCache, block_table: to
     A sequence of length 0 (or a row that sees nothing) gives zeros; rows of the cache past kv_len are never
     used, whatever they hold. Nothing waits for the host: safe to capture in a CUDA graph."""
     L, R = cache.latent_dim, cache.rope_dim
+    if not scale > 0:
+        raise ValueError("vq2 latent attention: scale must be positive")
     if q.dim() != 4 or q.dtype not in _DT or q.shape[3] != L + R:
         raise ValueError(f"vq2 latent attention: q must be bf16 or fp16 [B, T, heads, {L + R}]")
     B, T, heads, _ = q.shape
@@ -81,6 +83,8 @@ def latent_attention_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_rope: torc
     most 128, rope at most 64."""
     if q.dtype not in _DT:
         raise ValueError("vq2 latent attention: q must be bf16 or fp16")
+    if not scale > 0:
+        raise ValueError("vq2 latent attention: scale must be positive")
     if q.dim() != 3 or k_nope.dim() != 3 or v.dim() != 3:
         raise ValueError("vq2 latent attention: q, k_nope and v must be [tokens, heads, dim]")
     Tq, heads, dq = q.shape
