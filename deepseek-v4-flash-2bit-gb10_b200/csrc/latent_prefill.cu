@@ -22,36 +22,46 @@ namespace vq2 {
 constexpr int LP_MAX_D = 128;      // values a head: of the positionless key part, and of v
 constexpr int LP_TILE = 128;       // query rows a tile, key rows a step
 constexpr int LP_UNIT = LP_TILE * 128;         // bytes of a unit: 128 rows of 64 16-bit values
-constexpr int LP_RING = 8;         // units in flight: a step needs at most 3 (K) + 2 (V) at once
+// Units in flight: K in a ring of 6 (two steps of at most 3, so a step's keys load under the step before),
+// V in a ring of 2 (one step of at most 2, loaded between its last product and the next step's first).
+constexpr int LP_KRING = 6, LP_VRING = 2;
 constexpr int LP_THREADS = 384;
 constexpr float LP_RAISE = 8.f;    // log2 by which a row's maximum may grow before O is rescaled
 
 struct LpShared {
-  uint64_t full[LP_RING], empty[LP_RING];
-  uint64_t qfull[2], sfull[2], pfull[2], ofull[2], drain;
+  uint64_t kfull[LP_KRING], kempty[LP_KRING], vfull[LP_VRING], vempty[LP_VRING];
+  uint64_t qfull[2], sfull[2], pfull[2], ofull[2], vtail, cleared, drain;
   uint32_t tmem;
   int abort;
 };
-constexpr size_t LP_SMEM = (size_t)(6 + LP_RING) * LP_UNIT + sizeof(LpShared) + 1024;
+constexpr size_t LP_SMEM = (size_t)(6 + LP_KRING + LP_VRING) * LP_UNIT + sizeof(LpShared) + 1024;
 static_assert(LP_SMEM <= 227 * 1024, "latent prefill shared memory");
 
-// Shared-memory descriptor of an operand whose rows run along the contraction (MN-major) in 128-byte
-// swizzled units of 64 columns: 8-row groups 1024 bytes apart, units of 64 columns `unit` bytes apart.
-__device__ __forceinline__ uint64_t umma_desc_mn(uint32_t saddr, uint32_t unit) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)((unit >> 4) & 0x3FFF) << 16 | (uint64_t)(1024 >> 4) << 32 |
-         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+// Shared-memory descriptors as two words: the low one holds the address (in 16-byte units, so a step
+// along the contraction is one 32-bit add) and the leading offset, the high one is a constant: 8-row
+// groups 1024 bytes apart, 128-byte swizzle. K-major operands (rows of S's operands) have no leading
+// offset; in V, whose rows run along the contraction, it is the distance between units of 64 columns.
+constexpr uint32_t LP_DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %5, 0;\n mov.b64 x, {%1, %3};\n mov.b64 y, {%2, %3};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n}"
+               ::"r"(d), "r"(a), "r"(b), "r"(LP_DESC_HI), "r"(idesc), "r"(acc));
 }
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc));
-}
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc));
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n .reg .pred p;\n .reg .b64 y;\n setp.ne.b32 p, %5, 0;\n mov.b64 y, {%2, %3};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n}"
+               ::"r"(d), "r"(a), "r"(b), "r"(LP_DESC_HI), "r"(idesc), "r"(acc));
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
+}
+// One lane of a converged warp. The compiler knows that a branch on it has a single thread, so addresses
+// and descriptors stay in uniform registers there (a branch on a lane number moves them there one by one).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(e));
+  return e != 0;
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -137,25 +147,28 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
   const int past = nk - nq;                       // key i + past is the newest that query i sees
   const int ntile = nq - row0 > LP_TILE ? 2 : 1;
   // key steps of each tile, by its last row
-  int steps[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-    steps[t] = t < ntile ? (max(0, min(nk, min(nq, row0 + (t + 1) * LP_TILE) + past)) + LP_TILE - 1) / LP_TILE : 0;
-  const int nsteps = max(steps[0], steps[1]);
+  const int n0 = (max(0, min(nk, min(nq, row0 + LP_TILE) + past)) + LP_TILE - 1) / LP_TILE;
+  const int n1 = ntile > 1 ? (max(0, min(nk, min(nq, row0 + 2 * LP_TILE) + past)) + LP_TILE - 1) / LP_TILE : 0;
+  const int nsteps = max(n0, n1);
+  const bool tail = nsteps * LP_TILE > nk;        // the last step's values end inside their units
+  auto n_of = [&](int t) { return t ? n1 : n0; };
   const int kn = (a.nope_dim + 63) / 64, ku = kn + (a.rope_dim ? 1 : 0), vu = (a.v_dim + 63) / 64;   // units of a key row, of a value row
 
   uint8_t* smem = (uint8_t*)(((uintptr_t)lp_smem_raw + 1023) & ~(uintptr_t)1023);
-  const uint32_t qbase = smem_u32(smem), ring = qbase + 6 * LP_UNIT;
-  LpShared* sh = (LpShared*)(smem + (6 + LP_RING) * LP_UNIT);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t qbase = smem_u32(smem), kring = qbase + 6 * LP_UNIT, vring = kring + LP_KRING * LP_UNIT;
+  LpShared* sh = (LpShared*)(smem + (6 + LP_KRING + LP_VRING) * LP_UNIT);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < LP_RING; ++s) { mbar_init(&sh->full[s], 1); mbar_init(&sh->empty[s], 1); }
+    for (int s = 0; s < LP_KRING; ++s) { mbar_init(&sh->kfull[s], 1); mbar_init(&sh->kempty[s], 1); }
+    for (int s = 0; s < LP_VRING; ++s) { mbar_init(&sh->vfull[s], 1); mbar_init(&sh->vempty[s], 1); }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sh->qfull[t], 1);
       mbar_init(&sh->sfull[t], 1);
       mbar_init(&sh->pfull[t], 4);
       mbar_init(&sh->ofull[t], 1);
     }
+    mbar_init(&sh->vtail, 1);
+    mbar_init(&sh->cleared, 1);
     mbar_init(&sh->drain, 1);
     sh->abort = 0;
     fence_mbar_init();
@@ -167,7 +180,7 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sh->tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sh->tmem, 0);
   volatile int* abort = &sh->abort;
 
   if (warp < 4) {
@@ -179,89 +192,101 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
         for (int s = 0; s < ku; ++s)
           tma_load_3d(qbase + (t * 3 + s) * LP_UNIT, &tq, s < kn ? s * 64 : a.nope_dim, h, q0 + row0 + t * LP_TILE, &sh->qfull[t]);
       }
-      int g = 0;
-      for (int j = 0; j < nsteps && !*abort; ++j)
-        for (int s = 0; s < ku + vu; ++s, ++g) {
-          const int slot = g % LP_RING;
-          if (g >= LP_RING && !mbar_wait(&sh->empty[slot], ((g / LP_RING) - 1) & 1)) { *abort = 1; break; }
-          mbar_arrive_expect_tx(&sh->full[slot], LP_UNIT);
-          const CUtensorMap* m = s < kn ? &tk : s < ku ? &tr : &tv;
-          tma_load_3d(ring + slot * LP_UNIT, m, s < kn ? s * 64 : s < ku ? 0 : (s - ku) * 64, s < kn || s >= ku ? h : 0, k0 + j * LP_TILE,
-                      &sh->full[slot]);
-        }
-      // no copy is in flight when the block ends
-      for (int t = 0; t < ntile; ++t) mbar_wait(&sh->qfull[t], 0);
-      for (int q = max(0, g - LP_RING); q < g; ++q) mbar_wait(&sh->full[q % LP_RING], (q / LP_RING) & 1);
-    } else if (warp == 1 && nsteps > 0) {
-      // ---------------- products (the whole warp walks; lane 0 issues)
-      constexpr uint32_t fmt = DT == VQ2_DT_BF16 ? (1u << 7) | (1u << 10) : 0u;
-      const uint32_t id_s = (1u << 4) | fmt | ((LP_TILE >> 3) << 17) | ((LP_TILE >> 4) << 24);
-      auto id_o = [&](int n) { return (1u << 4) | fmt | (1u << 16) | ((uint32_t)((n + 15) / 16 * 2) << 17) | ((LP_TILE >> 4) << 24); };
-      const int gu = ku + vu;
-      // every lane waits and the warp agrees on the outcome, so no lane leaves a loop alone
-      auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
+      // keys of step j go out before the values of step j - 1: the scores of a step are computed first
+      int gk = 0, gv = 0;
       bool ok = true;
-      int cleared = -1;
-      auto scores = [&](int t, int j) {             // S_t = Q_t K_j^T
-        for (int s = 0; s < ku; ++s) {
-          const int g = j * gu + s;
-          if (!wait(&sh->full[g % LP_RING], (g / LP_RING) & 1)) { ok = false; return; }
-          tc_fence_after();
-          const uint32_t qa = qbase + (t * 3 + s) * LP_UNIT, kb = ring + (g % LP_RING) * LP_UNIT;
-          const int cols = s < kn ? min(64, a.nope_dim - s * 64) : a.rope_dim;
-          if (lane == 0)
-            for (int ks = 0; ks * 16 < cols; ++ks)
-              umma_ss(tmem + t * 128, umma_desc_sw128(qa + ks * 32), umma_desc_sw128(kb + ks * 32), id_s, (s | ks) != 0);
+      for (int j = 0; j <= nsteps && ok && !*abort; ++j) {
+        for (int s = 0; s < ku && j < nsteps && ok; ++s, ++gk) {
+          const int slot = gk % LP_KRING;
+          if (gk >= LP_KRING && !mbar_wait(&sh->kempty[slot], ((gk / LP_KRING) - 1) & 1)) { ok = false; break; }
+          mbar_arrive_expect_tx(&sh->kfull[slot], LP_UNIT);
+          tma_load_3d(kring + slot * LP_UNIT, s < kn ? &tk : &tr, s < kn ? s * 64 : 0, s < kn ? h : 0, k0 + j * LP_TILE, &sh->kfull[slot]);
         }
-        if (lane == 0) umma_commit(&sh->sfull[t]);
-      };
-      auto release = [&](int g, int n) {            // units g .. g + n - 1 once the products issued so far are done
-        if (lane == 0)
-          for (int s = 0; s < n; ++s) umma_commit(&sh->empty[(g + s) % LP_RING]);
+        for (int s = 0; s < vu && j > 0 && ok; ++s, ++gv) {
+          const int slot = gv % LP_VRING;
+          if (gv >= LP_VRING && !mbar_wait(&sh->vempty[slot], ((gv / LP_VRING) - 1) & 1)) { ok = false; break; }
+          const bool last = tail && j == nsteps;
+          uint64_t* bar = last ? &sh->vtail : &sh->vfull[slot];
+          if (!last) mbar_arrive_expect_tx(bar, LP_UNIT);
+          else if (s == 0) mbar_arrive_expect_tx(bar, vu * LP_UNIT);
+          tma_load_3d(vring + slot * LP_UNIT, &tv, s * 64, h, k0 + (j - 1) * LP_TILE, bar);
+        }
+      }
+      // no copy is in flight when the block ends
+      if (!ok) *abort = 1;
+      for (int t = 0; t < ntile; ++t) mbar_wait(&sh->qfull[t], 0);
+      for (int q = max(0, gk - LP_KRING); q < gk; ++q) mbar_wait(&sh->kfull[q % LP_KRING], (q / LP_KRING) & 1);
+      if (tail && ok && gv == nsteps * vu) {
+        mbar_wait(&sh->vtail, 0);
+        gv -= vu;
+      }
+      for (int q = max(0, gv - (tail ? LP_VRING - vu : LP_VRING)); q < gv; ++q) mbar_wait(&sh->vfull[q % LP_VRING], (q / LP_VRING) & 1);
+    } else if (warp == 1 && nsteps > 0 && elect_one()) {
+      // ---------------- products. One thread issues them all, beside the softmax warps of its
+      // scheduler, so the loops are unrolled to a few instructions a product.
+      constexpr uint32_t fmt = DT == VQ2_DT_BF16 ? (1u << 7) | (1u << 10) : 0u;
+      constexpr uint32_t id_s = (1u << 4) | fmt | ((LP_TILE >> 3) << 17) | ((LP_TILE >> 4) << 24);
+      const uint32_t id_o = (1u << 4) | fmt | (1u << 16) | ((uint32_t)((a.v_dim + 15) / 16 * 2) << 17) | ((LP_TILE >> 4) << 24);
+      constexpr uint32_t U = LP_UNIT >> 4;
+      const uint32_t qlo = (qbase >> 4) | 1u << 16, klo = (kring >> 4) | 1u << 16, vlo = (vring >> 4) | U << 16;
+      const int lastt = ntile - 1;                  // it has the most steps
+      bool ok = true;
+      auto scores = [&](int t, int j) {             // S_t = Q_t K_j^T
+        int g = j * ku;
+        for (int s = 0; s < ku; ++s, ++g) {
+          const int slot = g % LP_KRING;
+          if (!mbar_wait(&sh->kfull[slot], (g / LP_KRING) & 1)) { ok = false; return; }
+          tc_fence_after();
+          const uint32_t qa = qlo + (t * 3 + s) * U, kb = klo + slot * U;
+          const int cols = s < kn ? min(64, a.nope_dim - s * 64) : a.rope_dim;
+          umma_ss(tmem + t * 128, qa, kb, id_s, s != 0);
+#pragma unroll
+          for (int ks = 1; ks < 4; ++ks)
+            if (ks * 16 < cols) umma_ss(tmem + t * 128, qa + 2 * ks, kb + 2 * ks, id_s, 1);
+          if (t == lastt) umma_commit(&sh->kempty[slot]);        // free once the products issued so far are done
+        }
+        umma_commit(&sh->sfull[t]);
       };
       for (int t = 0; t < ntile && ok; ++t)
-        if (steps[t] > 0) {
-          if (!wait(&sh->qfull[t], 0)) { ok = false; break; }
+        if (n_of(t) > 0) {
+          if (!mbar_wait(&sh->qfull[t], 0)) { ok = false; break; }
           scores(t, 0);
         }
-      release(0, ku);
       for (int j = 0; j < nsteps && ok; ++j) {
-        const int gv = j * gu + ku;
+        const int sv = j * vu % LP_VRING;           // vu == 2: always 0, the two units side by side
         for (int t = 0; t < ntile && ok; ++t) {
-          if (j >= steps[t]) continue;
-          for (int s = 0; s < vu; ++s)
-            if (!wait(&sh->full[(gv + s) % LP_RING], ((gv + s) / LP_RING) & 1)) { ok = false; break; }
-          const int live = nk - j * LP_TILE;
-          if (live < LP_TILE && ok && cleared != j) {
-            cleared = j;
-            // rows past the last key belong to another sequence: their probabilities are 0, but 0 times
-            // a NaN there would reach this one's output, so they are cleared (only ever at the last step)
-            for (int s = 0; s < vu; ++s)
-              for (int i = live * 8 + lane; i < LP_TILE * 8; i += 32)
-                sts128_v(ring + ((gv + s) % LP_RING) * LP_UNIT + i * 16, make_uint4(0, 0, 0, 0));
-            fence_async_smem();
-            __syncwarp();
-          }
-          if (!ok || !wait(&sh->pfull[t], j & 1)) { ok = false; break; }
+          if (j >= n_of(t)) continue;
+          if (tail && j == nsteps - 1) ok = mbar_wait(&sh->cleared, 0);
+          else
+            for (int s = 0; s < vu && ok; ++s) ok = mbar_wait(&sh->vfull[sv + s], ((j * vu + s) / LP_VRING) & 1);
+          if (!ok || !mbar_wait(&sh->pfull[t], j & 1)) { ok = false; break; }
           tc_fence_after();
-          // O_t += P_t V_j: one product over both value units where they lie side by side in the ring
-          const uint32_t v0 = ring + (gv % LP_RING) * LP_UNIT, v1 = ring + ((gv + 1) % LP_RING) * LP_UNIT;
-          const bool whole = vu == 1 || v1 == v0 + LP_UNIT;
-          if (lane == 0)
-            for (int ks = 0; ks < LP_TILE / 16; ++ks) {
-              const uint32_t p = tmem + t * 128 + ks * 8;
-              umma_ts(tmem + 256 + t * 128, p, umma_desc_mn(v0 + ks * 2048, LP_UNIT), id_o(whole ? a.v_dim : 64), (j | ks) != 0);
-              if (!whole) umma_ts(tmem + 320 + t * 128, p, umma_desc_mn(v1 + ks * 2048, LP_UNIT), id_o(a.v_dim - 64), (j | ks) != 0);
-            }
-          if (j + 1 < steps[t]) scores(t, j + 1);
-          else if (lane == 0) umma_commit(&sh->ofull[t]);
+          // O_t += P_t V_j
+          const uint32_t o = tmem + 256 + t * 128, p = tmem + t * 128, vb = vlo + sv * U;
+          umma_ts(o, p, vb, id_o, j != 0);
+#pragma unroll
+          for (int ks = 1; ks < LP_TILE / 16; ++ks) umma_ts(o, p + ks * 8, vb + ks * 128, id_o, 1);
+          if (t == lastt)
+            for (int s = 0; s < vu; ++s) umma_commit(&sh->vempty[sv + s]);
+          if (j + 1 < n_of(t)) scores(t, j + 1);
+          else umma_commit(&sh->ofull[t]);
         }
-        release(gv, vu);
-        if (j + 1 < nsteps) release(gv + vu, ku);
       }
       if (!ok) *abort = 1;
-      if (lane == 0) umma_commit(&sh->drain);
+      umma_commit(&sh->drain);
       mbar_wait(&sh->drain, 0);
+    } else if (warp == 2 && nsteps > 0 && tail) {
+      // ---------------- the last step's value rows past the last key belong to another sequence: their
+      // probabilities are 0, but 0 times a NaN there would reach this one's output, so they are cleared
+      const int sv = (nsteps - 1) * vu % LP_VRING, live = nk - (nsteps - 1) * LP_TILE;
+      if (!__all_sync(0xffffffffu, mbar_wait(&sh->vtail, 0))) *abort = 1;
+      else
+        for (int s = 0; s < vu; ++s)
+          for (int i = live * 8 + lane; i < LP_TILE * 8; i += 32)
+            sts128_v(vring + (sv + s) * LP_UNIT + i * 16, make_uint4(0, 0, 0, 0));
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->cleared);
     }
   } else {
     // ---------------- softmax: thread = query row
@@ -271,7 +296,7 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
     const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * 128;
     const float sl = a.scale * 1.4426950408889634f;
     const int seen = max(0, min(nk, i + 1 + past));           // keys 0 .. seen - 1
-    const int n = steps[t];
+    const int n = n_of(t);
     float m = -INFINITY;                                      // the maximum that P and O are relative to
     float2 l2 = make_float2(0.f, 0.f);
     bool ok = true;
