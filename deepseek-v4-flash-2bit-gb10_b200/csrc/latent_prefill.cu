@@ -15,6 +15,7 @@
 //   warps 4-11   softmax, one thread a query row (4 warps a tile): the row's 128 scores in registers
 // A row's maximum is refreshed only when it rose by more than 2^8 in the exponent: P then stays below
 // 256 (exact enough in 16 bits: the rounding is relative) and O is rarely rescaled.
+#include <type_traits>
 #include "vq2_common.cuh"
 
 namespace vq2 {
@@ -22,19 +23,19 @@ namespace vq2 {
 constexpr int LP_MAX_D = 128;      // values a head: of the positionless key part, and of v
 constexpr int LP_TILE = 128;       // query rows a tile, key rows a step
 constexpr int LP_UNIT = LP_TILE * 128;         // bytes of a unit: 128 rows of 64 16-bit values
-// Units in flight: K in a ring of 6 (two steps of at most 3, so a step's keys load under the step before),
-// V in a ring of 2 (one step of at most 2, loaded between its last product and the next step's first).
-constexpr int LP_KRING = 6, LP_VRING = 2;
+// Steps in flight: 96 KB for keys (2 steps of 192 values, so a step's keys load under the step before),
+// 32 KB for values (1 step of 128, loaded between its last product and the next step's first).
+constexpr int LP_KUNITS = 6, LP_VUNITS = 2, LP_KMAX = 3;
 constexpr int LP_THREADS = 384;
 constexpr float LP_RAISE = 8.f;    // log2 by which a row's maximum may grow before O is rescaled
 
 struct LpShared {
-  uint64_t kfull[LP_KRING], kempty[LP_KRING], vfull[LP_VRING], vempty[LP_VRING];
+  uint64_t kfull[LP_KMAX], kempty[LP_KMAX], vfull[2], vempty[2];
   uint64_t qfull[2], sfull[2], pfull[2], ofull[2], vtail, cleared, drain;
   uint32_t tmem;
   int abort;
 };
-constexpr size_t LP_SMEM = (size_t)(6 + LP_KRING + LP_VRING) * LP_UNIT + sizeof(LpShared) + 1024;
+constexpr size_t LP_SMEM = (size_t)(6 + LP_KUNITS + LP_VUNITS) * LP_UNIT + sizeof(LpShared) + 1024;
 static_assert(LP_SMEM <= 227 * 1024, "latent prefill shared memory");
 
 // Shared-memory descriptors as two words: the low one holds the address (in 16-byte units, so a step
@@ -131,7 +132,21 @@ __device__ __forceinline__ void tmem_ld128(uint32_t t, float* v) {
   for (int i = 0; i < 128; ++i) asm volatile("" : "+f"(v[i]));     // no use of a value moves before the wait
 }
 
-template <int DT>
+// A position in a ring of N stages: the stage and the parity of the phase it is in.
+template <int N>
+struct Ring {
+  int stage = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == N) {
+      stage = 0;
+      parity ^= 1;
+    }
+  }
+};
+
+// KU, VU: units of 64 values in a key row (positionless part, then rotary part) and in a value row.
+template <int DT, int KU, int VU>
 __global__ void __launch_bounds__(LP_THREADS, 1)
 latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                       const __grid_constant__ CUtensorMap tr, const __grid_constant__ CUtensorMap tv) {
@@ -152,15 +167,16 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
   const int nsteps = max(n0, n1);
   const bool tail = nsteps * LP_TILE > nk;        // the last step's values end inside their units
   auto n_of = [&](int t) { return t ? n1 : n0; };
-  const int kn = (a.nope_dim + 63) / 64, ku = kn + (a.rope_dim ? 1 : 0), vu = (a.v_dim + 63) / 64;   // units of a key row, of a value row
+  const int kn = (a.nope_dim + 63) / 64;          // units of the positionless part
+  constexpr int KS = KU == 1 ? LP_KMAX : LP_KUNITS / KU, VS = LP_VUNITS / VU;      // stages
 
   uint8_t* smem = (uint8_t*)(((uintptr_t)lp_smem_raw + 1023) & ~(uintptr_t)1023);
-  const uint32_t qbase = smem_u32(smem), kring = qbase + 6 * LP_UNIT, vring = kring + LP_KRING * LP_UNIT;
-  LpShared* sh = (LpShared*)(smem + (6 + LP_KRING + LP_VRING) * LP_UNIT);
+  const uint32_t qbase = smem_u32(smem), kring = qbase + 6 * LP_UNIT, vring = kring + LP_KUNITS * LP_UNIT;
+  LpShared* sh = (LpShared*)(smem + (6 + LP_KUNITS + LP_VUNITS) * LP_UNIT);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < LP_KRING; ++s) { mbar_init(&sh->kfull[s], 1); mbar_init(&sh->kempty[s], 1); }
-    for (int s = 0; s < LP_VRING; ++s) { mbar_init(&sh->vfull[s], 1); mbar_init(&sh->vempty[s], 1); }
+    for (int s = 0; s < LP_KMAX; ++s) { mbar_init(&sh->kfull[s], 1); mbar_init(&sh->kempty[s], 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&sh->vfull[s], 1); mbar_init(&sh->vempty[s], 1); }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sh->qfull[t], 1);
       mbar_init(&sh->sfull[t], 1);
@@ -184,93 +200,101 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
   volatile int* abort = &sh->abort;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 0 && lane == 0 && nsteps > 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0 && nsteps > 0 && elect_one()) {
       // ---------------- loader
       for (int t = 0; t < ntile; ++t) {
-        mbar_arrive_expect_tx(&sh->qfull[t], ku * LP_UNIT);
-        for (int s = 0; s < ku; ++s)
+        mbar_arrive_expect_tx(&sh->qfull[t], KU * LP_UNIT);
+        for (int s = 0; s < KU; ++s)
           tma_load_3d(qbase + (t * 3 + s) * LP_UNIT, &tq, s < kn ? s * 64 : a.nope_dim, h, q0 + row0 + t * LP_TILE, &sh->qfull[t]);
       }
       // keys of step j go out before the values of step j - 1: the scores of a step are computed first
-      int gk = 0, gv = 0;
+      Ring<KS> rk;
+      Ring<VS> rv;
       bool ok = true;
-      for (int j = 0; j <= nsteps && ok && !*abort; ++j) {
-        for (int s = 0; s < ku && j < nsteps && ok; ++s, ++gk) {
-          const int slot = gk % LP_KRING;
-          if (gk >= LP_KRING && !mbar_wait(&sh->kempty[slot], ((gk / LP_KRING) - 1) & 1)) { ok = false; break; }
-          mbar_arrive_expect_tx(&sh->kfull[slot], LP_UNIT);
-          tma_load_3d(kring + slot * LP_UNIT, s < kn ? &tk : &tr, s < kn ? s * 64 : 0, s < kn ? h : 0, k0 + j * LP_TILE, &sh->kfull[slot]);
+      int nkeys = 0, nvals = 0;                      // steps loaded
+      for (int j = 0; j <= nsteps; ++j) {
+        if (j < nsteps) {
+          if (!(ok = mbar_wait(&sh->kempty[rk.stage], rk.parity ^ 1))) break;       // passes at once in the first round
+          mbar_arrive_expect_tx(&sh->kfull[rk.stage], KU * LP_UNIT);
+#pragma unroll
+          for (int s = 0; s < KU; ++s)
+            tma_load_3d(kring + (rk.stage * KU + s) * LP_UNIT, s < kn ? &tk : &tr, s < kn ? s * 64 : 0, s < kn ? h : 0, k0 + j * LP_TILE,
+                        &sh->kfull[rk.stage]);
+          rk.next();
+          ++nkeys;
         }
-        for (int s = 0; s < vu && j > 0 && ok; ++s, ++gv) {
-          const int slot = gv % LP_VRING;
-          if (gv >= LP_VRING && !mbar_wait(&sh->vempty[slot], ((gv / LP_VRING) - 1) & 1)) { ok = false; break; }
-          const bool last = tail && j == nsteps;
-          uint64_t* bar = last ? &sh->vtail : &sh->vfull[slot];
-          if (!last) mbar_arrive_expect_tx(bar, LP_UNIT);
-          else if (s == 0) mbar_arrive_expect_tx(bar, vu * LP_UNIT);
-          tma_load_3d(vring + slot * LP_UNIT, &tv, s * 64, h, k0 + (j - 1) * LP_TILE, bar);
+        if (j > 0) {
+          if (!(ok = mbar_wait(&sh->vempty[rv.stage], rv.parity ^ 1))) break;
+          uint64_t* bar = tail && j == nsteps ? &sh->vtail : &sh->vfull[rv.stage];
+          mbar_arrive_expect_tx(bar, VU * LP_UNIT);
+#pragma unroll
+          for (int s = 0; s < VU; ++s)
+            tma_load_3d(vring + (rv.stage * VU + s) * LP_UNIT, &tv, s * 64, h, k0 + (j - 1) * LP_TILE, bar);
+          rv.next();
+          ++nvals;
         }
       }
-      // no copy is in flight when the block ends
       if (!ok) *abort = 1;
+      // no copy is in flight when the block ends, also where a wait gave up
       for (int t = 0; t < ntile; ++t) mbar_wait(&sh->qfull[t], 0);
-      for (int q = max(0, gk - LP_KRING); q < gk; ++q) mbar_wait(&sh->kfull[q % LP_KRING], (q / LP_KRING) & 1);
-      if (tail && ok && gv == nsteps * vu) {
-        mbar_wait(&sh->vtail, 0);
-        gv -= vu;
-      }
-      for (int q = max(0, gv - (tail ? LP_VRING - vu : LP_VRING)); q < gv; ++q) mbar_wait(&sh->vfull[q % LP_VRING], (q / LP_VRING) & 1);
+      for (int q = max(0, nkeys - KS); q < nkeys; ++q) mbar_wait(&sh->kfull[q % KS], (q / KS) & 1);
+      for (int q = max(0, nvals - VS); q < nvals; ++q)
+        tail && q == nsteps - 1 ? mbar_wait(&sh->vtail, 0) : mbar_wait(&sh->vfull[q % VS], (q / VS) & 1);
     } else if (warp == 1 && nsteps > 0 && elect_one()) {
-      // ---------------- products. One thread issues them all, beside the softmax warps of its
-      // scheduler, so the loops are unrolled to a few instructions a product.
+      // ---------------- products: one thread issues them all
       constexpr uint32_t fmt = DT == VQ2_DT_BF16 ? (1u << 7) | (1u << 10) : 0u;
       constexpr uint32_t id_s = (1u << 4) | fmt | ((LP_TILE >> 3) << 17) | ((LP_TILE >> 4) << 24);
       const uint32_t id_o = (1u << 4) | fmt | (1u << 16) | ((uint32_t)((a.v_dim + 15) / 16 * 2) << 17) | ((LP_TILE >> 4) << 24);
       constexpr uint32_t U = LP_UNIT >> 4;
       const uint32_t qlo = (qbase >> 4) | 1u << 16, klo = (kring >> 4) | 1u << 16, vlo = (vring >> 4) | U << 16;
       const int lastt = ntile - 1;                  // it has the most steps
+      Ring<KS> rk;
+      Ring<VS> rv;
       bool ok = true;
-      auto scores = [&](int t, int j) {             // S_t = Q_t K_j^T
-        int g = j * ku;
-        for (int s = 0; s < ku; ++s, ++g) {
-          const int slot = g % LP_KRING;
-          if (!mbar_wait(&sh->kfull[slot], (g / LP_KRING) & 1)) { ok = false; return; }
-          tc_fence_after();
-          const uint32_t qa = qlo + (t * 3 + s) * U, kb = klo + slot * U;
-          const int cols = s < kn ? min(64, a.nope_dim - s * 64) : a.rope_dim;
-          umma_ss(tmem + t * 128, qa, kb, id_s, s != 0);
+      auto scores = [&](int t) {                    // S_t = Q_t K^T: columns past a part's end are zeros in K
+        const uint32_t qa = qlo + t * 3 * U, kb = klo + rk.stage * (KU * U);
 #pragma unroll
-          for (int ks = 1; ks < 4; ++ks)
-            if (ks * 16 < cols) umma_ss(tmem + t * 128, qa + 2 * ks, kb + 2 * ks, id_s, 1);
-          if (t == lastt) umma_commit(&sh->kempty[slot]);        // free once the products issued so far are done
-        }
+        for (int s = 0; s < KU; ++s)
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) umma_ss(tmem + t * 128, qa + s * U + 2 * ks, kb + s * U + 2 * ks, id_s, (s | ks) != 0);
         umma_commit(&sh->sfull[t]);
+        if (t == lastt) {                           // the stage is free once the products issued so far are done
+          umma_commit(&sh->kempty[rk.stage]);
+          rk.next();
+        }
       };
-      for (int t = 0; t < ntile && ok; ++t)
-        if (n_of(t) > 0) {
-          if (!mbar_wait(&sh->qfull[t], 0)) { ok = false; break; }
-          scores(t, 0);
-        }
+      ok = mbar_wait(&sh->kfull[0], 0);
+      for (int t = 0; t < ntile && ok; ++t) {
+        ok = mbar_wait(&sh->qfull[t], 0);
+        tc_fence_after();
+        if (ok && (n_of(t) > 0 || t == lastt)) scores(t);
+      }
       for (int j = 0; j < nsteps && ok; ++j) {
-        const int sv = j * vu % LP_VRING;           // vu == 2: always 0, the two units side by side
-        for (int t = 0; t < ntile && ok; ++t) {
-          if (j >= n_of(t)) continue;
-          if (tail && j == nsteps - 1) ok = mbar_wait(&sh->cleared, 0);
-          else
-            for (int s = 0; s < vu && ok; ++s) ok = mbar_wait(&sh->vfull[sv + s], ((j * vu + s) / LP_VRING) & 1);
-          if (!ok || !mbar_wait(&sh->pfull[t], j & 1)) { ok = false; break; }
-          tc_fence_after();
-          // O_t += P_t V_j
-          const uint32_t o = tmem + 256 + t * 128, p = tmem + t * 128, vb = vlo + sv * U;
-          umma_ts(o, p, vb, id_o, j != 0);
+        const uint32_t vb = vlo + rv.stage * (VU * U);
+        ok = tail && j == nsteps - 1 ? mbar_wait(&sh->cleared, 0) : mbar_wait(&sh->vfull[rv.stage], rv.parity);
+        bool loaded = false;
 #pragma unroll
-          for (int ks = 1; ks < LP_TILE / 16; ++ks) umma_ts(o, p + ks * 8, vb + ks * 128, id_o, 1);
-          if (t == lastt)
-            for (int s = 0; s < vu; ++s) umma_commit(&sh->vempty[sv + s]);
-          if (j + 1 < n_of(t)) scores(t, j + 1);
-          else umma_commit(&sh->ofull[t]);
+        for (int t = 0; t < 2; ++t) {
+          if (t > lastt || j >= n_of(t) || !ok) continue;
+          ok = mbar_wait(&sh->pfull[t], j & 1);
+          if (!ok) break;
+          tc_fence_after();
+          // O_t += P_t V
+#pragma unroll
+          for (int ks = 0; ks < LP_TILE / 16; ++ks)
+            umma_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, vb + ks * 128, id_o, ks > 0 ? 1 : j != 0);
+          if (t == lastt) umma_commit(&sh->vempty[rv.stage]);
+          if (j + 1 < n_of(t)) {
+            if (!loaded) ok = loaded = mbar_wait(&sh->kfull[rk.stage], rk.parity);
+            if (!ok) break;
+            tc_fence_after();
+            scores(t);
+          } else {
+            umma_commit(&sh->ofull[t]);
+          }
         }
+        rv.next();
       }
       if (!ok) *abort = 1;
       umma_commit(&sh->drain);
@@ -278,10 +302,10 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
     } else if (warp == 2 && nsteps > 0 && tail) {
       // ---------------- the last step's value rows past the last key belong to another sequence: their
       // probabilities are 0, but 0 times a NaN there would reach this one's output, so they are cleared
-      const int sv = (nsteps - 1) * vu % LP_VRING, live = nk - (nsteps - 1) * LP_TILE;
+      const int sv = (nsteps - 1) % VS * VU, live = nk - (nsteps - 1) * LP_TILE;
       if (!__all_sync(0xffffffffu, mbar_wait(&sh->vtail, 0))) *abort = 1;
       else
-        for (int s = 0; s < vu; ++s)
+        for (int s = 0; s < VU; ++s)
           for (int i = live * 8 + lane; i < LP_TILE * 8; i += 32)
             sts128_v(vring + (sv + s) * LP_UNIT + i * 16, make_uint4(0, 0, 0, 0));
       fence_async_smem();
@@ -290,7 +314,7 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
     }
   } else {
     // ---------------- softmax: thread = query row
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int t = (warp - 4) >> 2, r = (warp & 3) * 32 + lane, i = row0 + t * LP_TILE + r;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * 128;
@@ -425,7 +449,14 @@ extern "C" int vq2_latent_prefill(const vq2_latent_prefill_args* a, void* stream
   if (!rc && any) rc = lp_encode(&tv, a->v, a->v_dim, a->heads, a->total_k, a->v_stride_h, a->v_stride_t);
   if (!rc && any && a->rope_dim) rc = lp_encode(&tr, a->k_rope, a->rope_dim, 1, a->total_k, 0, a->r_stride_t);
   if (rc) return rc;
-  auto kernel = a->dtype == VQ2_DT_BF16 ? latent_prefill_kernel<VQ2_DT_BF16> : latent_prefill_kernel<VQ2_DT_F16>;
+  const int ku = (a->nope_dim + 63) / 64 + (a->rope_dim ? 1 : 0), vu = (a->v_dim + 63) / 64;
+  auto pick = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    return ku == 1 ? (vu == 1 ? latent_prefill_kernel<DT, 1, 1> : latent_prefill_kernel<DT, 1, 2>)
+         : ku == 2 ? (vu == 1 ? latent_prefill_kernel<DT, 2, 1> : latent_prefill_kernel<DT, 2, 2>)
+                   : (vu == 1 ? latent_prefill_kernel<DT, 3, 1> : latent_prefill_kernel<DT, 3, 2>);
+  };
+  auto kernel = a->dtype == VQ2_DT_BF16 ? pick(std::integral_constant<int, VQ2_DT_BF16>()) : pick(std::integral_constant<int, VQ2_DT_F16>());
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)LP_SMEM) != cudaSuccess) return VQ2_ERR_CUDA;
   kernel<<<(unsigned)blocks, LP_THREADS, LP_SMEM, (cudaStream_t)stream>>>(*a, nqb, tq, tk, tr, tv);
   return cudaGetLastError() == cudaSuccess ? VQ2_OK : VQ2_ERR_CUDA;
