@@ -31,7 +31,7 @@ constexpr float LP_RAISE = 8.f;    // log2 by which a row's maximum may grow bef
 
 struct LpShared {
   uint64_t kfull[LP_KMAX], kempty[LP_KMAX], vfull[2], vempty[2];
-  uint64_t qfull[2], sfull[2], pfull[2], ofull[2], vtail, cleared, drain;
+  uint64_t qfull[2], sfull[2], pfull[2][2], ofull[2], vtail, cleared, drain;
   uint32_t tmem;
   int abort;
 };
@@ -103,24 +103,14 @@ __device__ __forceinline__ void tmem_ld64(uint32_t t, float* v) {
                  "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
                : "r"(t));
 }
-__device__ __forceinline__ void tmem_st64(uint32_t t, const uint32_t* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x64.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
-               "%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,"
-               "%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,%64};"
+__device__ __forceinline__ void tmem_st32(uint32_t t, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+               "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
                ::"r"(t), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
                  "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
                  "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
-                 "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]),
-                 "r"(v[32]), "r"(v[33]), "r"(v[34]), "r"(v[35]), "r"(v[36]), "r"(v[37]), "r"(v[38]), "r"(v[39]),
-                 "r"(v[40]), "r"(v[41]), "r"(v[42]), "r"(v[43]), "r"(v[44]), "r"(v[45]), "r"(v[46]), "r"(v[47]),
-                 "r"(v[48]), "r"(v[49]), "r"(v[50]), "r"(v[51]), "r"(v[52]), "r"(v[53]), "r"(v[54]), "r"(v[55]),
-                 "r"(v[56]), "r"(v[57]), "r"(v[58]), "r"(v[59]), "r"(v[60]), "r"(v[61]), "r"(v[62]), "r"(v[63])
+                 "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
                : "memory");
-}
-// keeps 64 registers allocated and unmodified up to this point (a store reads its sources late)
-__device__ __forceinline__ void keep_live64(const uint32_t* v) {
-#pragma unroll
-  for (int i = 0; i < 64; i += 16) keep_live16(v + i);
 }
 
 // A row's 128 scores as registers.
@@ -180,7 +170,8 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sh->qfull[t], 1);
       mbar_init(&sh->sfull[t], 1);
-      mbar_init(&sh->pfull[t], 4);
+      mbar_init(&sh->pfull[t][0], 4);
+      mbar_init(&sh->pfull[t][1], 4);
       mbar_init(&sh->ofull[t], 1);
     }
     mbar_init(&sh->vtail, 1);
@@ -277,13 +268,16 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (t > lastt || j >= n_of(t) || !ok) continue;
-          ok = mbar_wait(&sh->pfull[t], j & 1);
-          if (!ok) break;
-          tc_fence_after();
-          // O_t += P_t V
+          // O_t += P_t V, the first 64 keys as soon as their probabilities are there
 #pragma unroll
-          for (int ks = 0; ks < LP_TILE / 16; ++ks)
-            umma_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, vb + ks * 128, id_o, ks > 0 ? 1 : j != 0);
+          for (int half = 0; half < 2; ++half) {
+            if (!(ok = mbar_wait(&sh->pfull[t][half], j & 1))) break;
+            tc_fence_after();
+#pragma unroll
+            for (int ks = half * 4; ks < half * 4 + 4; ++ks)
+              umma_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, vb + ks * 128, id_o, ks > 0 ? 1 : j != 0);
+          }
+          if (!ok) break;
           if (t == lastt) umma_commit(&sh->vempty[rv.stage]);
           if (j + 1 < n_of(t)) {
             if (!loaded) ok = loaded = mbar_wait(&sh->kfull[rk.stage], rk.parity);
@@ -364,23 +358,27 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
       const float mb = m == -INFINITY ? 0.f : -m * sl;
       const float2 s2 = make_float2(sl, sl), b2 = make_float2(mb, mb);
       float2 sum = make_float2(0.f, 0.f), sumb = sum;
-      uint32_t p[64];
 #pragma unroll
-      for (int c = 0; c < 128; c += 2) {
-        float2 x = ffma2(make_float2(s[c], s[c + 1]), s2, b2);
-        x.x = ex2(x.x);
-        x.y = ex2(x.y);
-        if (c & 2) sumb = fadd2(sumb, x);
-        else sum = fadd2(sum, x);
-        p[c >> 1] = pack2<DT>(x.x, x.y);
+      for (int half = 0; half < 2; ++half) {
+        uint32_t p[32];
+#pragma unroll
+        for (int c = 0; c < 64; c += 2) {
+          float2 x = ffma2(make_float2(s[half * 64 + c], s[half * 64 + c + 1]), s2, b2);
+          x.x = ex2(x.x);
+          x.y = ex2(x.y);
+          if (c & 2) sumb = fadd2(sumb, x);
+          else sum = fadd2(sum, x);
+          p[c >> 1] = pack2<DT>(x.x, x.y);
+        }
+        tmem_st32(ts + half * 32, p);
+        tmem_st_wait();
+        keep_live16(p);
+        keep_live16(p + 16);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->pfull[t][half]);
       }
-      tmem_st64(ts, p);
       l2 = fadd2(l2, fadd2(sum, sumb));
-      tmem_st_wait();
-      keep_live64(p);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->pfull[t]);
     }
     if (ok && n > 0 && !__all_sync(0xffffffffu, mbar_wait(&sh->ofull[t], 0))) ok = false;
     if (!ok) *abort = 1;
