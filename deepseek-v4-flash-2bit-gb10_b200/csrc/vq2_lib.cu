@@ -9,5 +9,5 @@
 #include "pack.cu"
 #include "shared.cu"
 #include "latent_cache.cu"
-#include "latent_decode.cu"
 #include "latent_prefill.cu"
+#include "latent_decode.cu"
