@@ -4,29 +4,31 @@
 // H is symmetric and H H = I, so q_c . c_j = (H q_c) . (n s)_j and out = H sum_j p_j (n s)_j: the
 // kernel rotates the query and the result, never a cached row.
 //
-// Both products run on tcgen05 with the cached rows as the 128-row operand and NQ = 16, 32 or 64 query
-// rows (heads x tokens of one sequence) as the narrow one, so few heads waste nothing:
-//   S^T [128 cached x NQ] = K Q^T      K tile in shared memory, rows = cached rows (K-major)
-//   O^T [L x NQ]         += V^T P^T    the same tile read along the other direction (MN-major): the
+// Both products run on tcgen05 with the cached rows as the wide operand and NQ = 16, 32 or 64 query
+// rows (heads x tokens of one sequence) as the narrow one, so few heads waste little:
+//   S^T [64 cached x NQ] = K Q^T       K tile in shared memory, rows = cached rows (K-major)
+//   O^T [L x NQ]        += V^T P^T     the same tile read along the other direction (MN-major): the
 //                                      latent is key and value, expanded from 4 bits once for both
 // A row is held as n s in fp16, which is exact (|n| <= 7, s has 8 significant bits), q in fp16 with a
 // power-of-two scale a row, P in fp16 with its largest values between 2^10 and 2^15, so that values down to
 // 2^-34 of the largest still count; sums are fp32 in tensor memory.
 //
-// Work: the (sequence, block of NQ query rows, tile of 128 cached rows) triples in order, split evenly over one
+// Work: the (sequence, block of NQ query rows, tile of 64 cached rows) triples in order, split evenly over one
 // block an SM. A block that holds all tiles of a query block writes the result; otherwise it
 // leaves its unnormalised sum, maximum and denominator, and the join kernel adds up the parts in order.
-// Roles: 16 worker warps load 128 rows ahead into registers, expand them into the tile, and do
-// the softmax with a thread per cached row; one thread of a 17th warp issues the products.
+// Roles: 8 worker warps load 64 rows ahead into registers, expand them into one of two tiles, and do the softmax
+// of the tile before with a thread per cached row and column group; one thread of a ninth warp issues
+// S of a tile before P V of the tile before it, so the products run under expansion and softmax.
 #include "vq2_common.cuh"
 
 namespace vq2 {
 
-constexpr int LD_TILE = 128;            // cached rows a tile
-constexpr int LD_WORKERS = 512;
-constexpr int LD_THREADS = LD_WORKERS + 128;     // 96 registers each at launch: 512 x 112 + 128 x 32 afterwards
-constexpr int LD_UNIT = LD_TILE * 128;  // bytes of a unit of the tile: 128 rows of 64 fp16 values
+constexpr int LD_TILE = 64;             // cached rows a tile
+constexpr int LD_WORKERS = 256, LD_WARPS = LD_WORKERS / 32;
+constexpr int LD_THREADS = LD_WORKERS + 128;     // 168 registers each at launch: 256 x 200 + 128 x 104 afterwards
+constexpr int LD_UNIT = LD_TILE * 128;  // bytes of a unit of the tile: 64 rows of 64 fp16 values
 constexpr int LD_UNITS = 9;             // 8 for the latent, 1 for the rotary part (P takes its place once S is done)
+constexpr int LD_KBYTES = LD_UNITS * LD_UNIT;
 constexpr float LD_BIAS = 10.f, LD_RAISE = 5.f;    // P = 2^(z - m + BIAS); m is raised when z exceeds it by RAISE
 
 struct LdArgs {
@@ -43,20 +45,20 @@ struct LdArgs {
 
 template <int NQ>
 struct LdShared {
-  uint64_t kfull, sfull, pfull, pvdone, drain;
+  uint64_t kfull[2], sfull[2], pfull[2], kfree[2], drain;      // by tile buffer
   uint32_t tmem;
-  int abort, first, b0, rb0, tile0, total;
+  int abort, b0, rb0, tile0;
   long long rows[4][LD_TILE];        // byte offset of a cached row, -1: not there (written two tiles ahead, read until the softmax)
-  int bad[LD_TILE];                  // number of the tile in which this row held a non-finite scale
+  int bad[2][LD_TILE];               // number of the tile in which this row held a non-finite scale
   float red[4][NQ];
   float fac[NQ];                     // log2-scaled factor of a query row's logits
-  float ref[NQ];                     // maximum that P and O are relative to
+  float ref[NQ], down[NQ];           // maximum that P and O are relative to; factor of its last change
   float lsum[4][NQ];
   int lim[NQ];                       // cached rows a query row sees
-  int scan[LD_WORKERS / 32];
+  int scan[LD_WARPS];
 };
 template <int NQ>
-constexpr size_t ld_smem() { return (size_t)LD_UNITS * LD_UNIT + (size_t)LD_UNITS * NQ * 128 + sizeof(LdShared<NQ>) + 1024; }
+constexpr size_t ld_smem() { return (size_t)2 * LD_KBYTES + (size_t)LD_UNITS * NQ * 128 + sizeof(LdShared<NQ>) + 1024; }
 static_assert(ld_smem<64>() <= 227 * 1024, "latent decode shared memory");
 
 // Wait that ends early once any thread of the block has given up; it never leaves the caller's loop,
@@ -70,7 +72,7 @@ __device__ __forceinline__ bool ld_wait(uint64_t* bar, uint32_t parity, volatile
   *abort = 1;
   return false;
 }
-__device__ __forceinline__ void ld_sync_workers() { asm volatile("barrier.cta.sync 1, 512;" ::: "memory"); }
+__device__ __forceinline__ void ld_sync_workers() { asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ void ld_sync_group(int g) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(2 + g) : "memory"); }
 __device__ __forceinline__ bool ld_any_group(int g, bool p) {
   uint32_t r;
@@ -80,29 +82,10 @@ __device__ __forceinline__ bool ld_any_group(int g, bool p) {
 }
 template <int N>
 __device__ __forceinline__ void ld_tmem_load(uint32_t t, float* v) {
-  if (N == 16) tmem_ld16(t, v);
-  else if (N == 8) tmem_ld8(t, v);
-  else {
-    uint32_t r[4];
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];\n tcgen05.wait::ld.sync.aligned;"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(t) : "memory");
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
-  }
+  if (N == 32) tmem_ld32(t, v);
+  else if (N == 16) tmem_ld16(t, v);
+  else tmem_ld8(t, v);
 }
-template <int N>
-__device__ __forceinline__ void ld_tmem_store(uint32_t t, const float* v) {
-  const uint32_t* u = (const uint32_t*)v;
-  if (N == 16) tmem_st16(t, u);
-  else if (N == 8) tmem_st8(t, u);
-  else
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(t), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3])
-                 : "memory");
-  tmem_st_wait();
-#pragma unroll
-  for (int i = 0; i < N; ++i) asm volatile("" ::"f"(v[i]));
-}
-
 // Position of a tile: sequence, block of query rows, tile; the order is sequence, block, tile.
 struct LdPos {
   int b, rb, tile, len, tiles;
@@ -122,14 +105,70 @@ struct LdPos {
   }
 };
 
+// D += A B with both descriptors at constant offsets from their bases (added in place: otherwise
+// the compiler keeps a register for each of the unrolled products).
+template <uint32_t A_OFF, uint32_t B_OFF, uint32_t B_HI, uint32_t ID>
+__device__ __forceinline__ void umma_at(uint32_t d, uint32_t a, uint32_t b, uint32_t acc) {
+  asm volatile("{\n .reg .pred p;\n .reg .b64 x, y;\n .reg .b32 u, v;\n setp.ne.b32 p, %7, 0;\n add.u32 u, %1, %3;\n add.u32 v, %2, %4;\n"
+               " mov.b64 x, {u, %5};\n mov.b64 y, {v, %6};\n tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %8, p;\n}"
+               ::"r"(d), "r"(a), "r"(b), "n"(A_OFF), "n"(B_OFF), "n"(LP_DESC_HI), "n"(B_HI), "r"(acc), "r"(ID));
+}
+
+// The products of a tile, unrolled for each number of units: issued by one thread, with nothing but
+// constants added to two addresses, a product takes about 15 cycles to issue (with run-time loops and branches in
+// between about 50, which is more than the product itself takes).
+template <int NQ, int SU, int I = 0>
+__device__ __forceinline__ void ld_scores_n(uint32_t d, uint32_t k, uint32_t q) {
+  constexpr uint32_t id = (1u << 4) | ((uint32_t)(NQ >> 3) << 17) | ((uint32_t)(LD_TILE >> 4) << 24);
+  constexpr int s = I / 4, ks = I % 4;
+  umma_at<s * (LD_UNIT >> 4) + 2 * ks, s * (NQ * 8) + 2 * ks, LP_DESC_HI, id>(d, k, q, I != 0);
+  if constexpr (I + 1 < SU * 4) ld_scores_n<NQ, SU, I + 1>(d, k, q);
+}
+template <int NQ>
+__device__ __forceinline__ void ld_scores(int su, uint32_t d, uint32_t k, uint32_t q) {
+  k |= 1u << 16;
+  q |= 1u << 16;
+  switch (su) {
+    case 1: return ld_scores_n<NQ, 1>(d, k, q);
+    case 2: return ld_scores_n<NQ, 2>(d, k, q);
+    case 3: return ld_scores_n<NQ, 3>(d, k, q);
+    case 4: return ld_scores_n<NQ, 4>(d, k, q);
+    case 5: return ld_scores_n<NQ, 5>(d, k, q);
+    case 6: return ld_scores_n<NQ, 6>(d, k, q);
+    case 7: return ld_scores_n<NQ, 7>(d, k, q);
+    case 8: return ld_scores_n<NQ, 8>(d, k, q);
+    default: return ld_scores_n<NQ, 9>(d, k, q);
+  }
+}
+// O^T += V^T P^T: M = 128 latent values a block (the second unit of the last block may be P itself, where the latent has an
+// odd number of units: its rows of O^T are not read). P lies as rows of 2 NQ bytes in the swizzle of that width.
+template <int NQ, int NB, int I = 0>
+__device__ __forceinline__ void ld_values_n(uint32_t d, uint32_t v, uint32_t p, uint32_t acc) {
+  constexpr uint32_t id = (1u << 4) | (1u << 15) | (1u << 16) | ((uint32_t)(NQ >> 3) << 17) | ((128u >> 4) << 24);
+  constexpr uint32_t p_hi = (uint32_t)(16 * NQ >> 4) | 1u << 14 | (NQ == 64 ? 2u : NQ == 32 ? 4u : 6u) << 29;
+  constexpr int ks = I / NB, m = I % NB;
+  umma_at<m * (2 * LD_UNIT >> 4) + ks * 128, ks * (2 * NQ), p_hi, id>(d + m * NQ, v, p, ks > 0 ? 1 : acc);
+  if constexpr (I + 1 < NB * (LD_TILE / 16)) ld_values_n<NQ, NB, I + 1>(d, v, p, acc);
+}
+template <int NQ>
+__device__ __forceinline__ void ld_values(int nblk, uint32_t d, uint32_t tile, int nl, uint32_t acc) {
+  const uint32_t v = tile | (LD_UNIT >> 4) << 16, p = (tile + nl * (LD_UNIT >> 4)) | 1u << 16;
+  switch (nblk) {
+    case 1: return ld_values_n<NQ, 1>(d, v, p, acc);
+    case 2: return ld_values_n<NQ, 2>(d, v, p, acc);
+    case 3: return ld_values_n<NQ, 3>(d, v, p, acc);
+    default: return ld_values_n<NQ, 4>(d, v, p, acc);
+  }
+}
+
 template <int DT, int NQ>
 __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) {
-  constexpr int CPT = NQ / 4;           // query rows (columns of S^T) a softmax thread
-  constexpr uint32_t COLS = NQ == 64 ? 512 : NQ == 32 ? 256 : 128;    // tensor memory: O^T 4 x NQ columns, S^T NQ
+  constexpr int CPT = NQ / 2, CPH = NQ / 4;     // columns of S^T (query rows) a column group has, a softmax thread takes
+  constexpr uint32_t COLS = NQ == 64 ? 512 : NQ == 32 ? 256 : 128;    // tensor memory: O^T 4 x NQ columns, S^T 2 x NQ
   extern __shared__ __align__(1024) uint8_t ld_smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)ld_smem_raw + 1023) & ~(uintptr_t)1023);
-  const uint32_t kb = smem_u32(smem), qb = kb + LD_UNITS * LD_UNIT;
-  LdShared<NQ>* sh = (LdShared<NQ>*)(smem + LD_UNITS * LD_UNIT + LD_UNITS * NQ * 128);
+  const uint32_t kb = smem_u32(smem), qb = kb + 2 * LD_KBYTES;
+  LdShared<NQ>* sh = (LdShared<NQ>*)(smem + 2 * LD_KBYTES + LD_UNITS * NQ * 128);
   const vq2_latent_decode_args& a = g.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int L = a.latent_dim, R = a.rope_dim, nl = L / 64, nblk = (nl + 1) / 2;
@@ -137,19 +176,21 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
   pdl_launch_dependents();
 
   if (tid == 0) {
-    mbar_init(&sh->kfull, 1);
-    mbar_init(&sh->sfull, 1);
-    mbar_init(&sh->pfull, 1);
-    mbar_init(&sh->pvdone, 1);
+    for (int k = 0; k < 2; ++k) {
+      mbar_init(&sh->kfull[k], 1);
+      mbar_init(&sh->sfull[k], 1);
+      mbar_init(&sh->pfull[k], 1);
+      mbar_init(&sh->kfree[k], 1);
+    }
     mbar_init(&sh->drain, 1);
     sh->abort = 0;
     fence_mbar_init();
   }
-  if (warp == 16) {
+  if (warp == LD_WARPS) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem)), "r"(COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (tid < LD_TILE) sh->bad[tid] = -1;
+  if (tid < 2 * LD_TILE) sh->bad[tid >> 6][tid & 63] = -1;
 
   // ---------------- this block's share of the tiles. Each worker sums a run of sequences, a scan gives
   // the runs' first positions, and the worker whose run holds the block's first tile walks to it.
@@ -167,10 +208,10 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
     const int v = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += v;
   }
-  if (lane == 31 && warp < 16) sh->scan[warp] = inc;
+  if (lane == 31 && warp < LD_WARPS) sh->scan[warp] = inc;
   __syncthreads();
   int before = inc - mine, total = 0;
-  for (int w = 0; w < 16; ++w) {
+  for (int w = 0; w < LD_WARPS; ++w) {
     if (w < warp) before += sh->scan[w];
     total += sh->scan[w];
   }
@@ -200,341 +241,375 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh->tmem, 0);
-  const uint32_t ts = tmem + 4 * NQ;                    // S^T
+  const uint32_t ts = tmem + 4 * NQ;                    // S^T of the two buffers
 
-  if (warp >= 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
-    if (warp == 16 && elect_one()) {
+  if (warp >= LD_WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp == LD_WARPS && count > 0 && elect_one()) {
       // ---------------- products
-      constexpr uint32_t id_s = (1u << 4) | ((uint32_t)(NQ >> 3) << 17) | ((LD_TILE >> 4) << 24);
-      constexpr uint32_t id_o = id_s | (1u << 15) | (1u << 16);        // both operands along the contraction
-      // P [128 cached][NQ]: rows of 2 NQ bytes in the swizzle of that width; 8-row groups 16 NQ bytes apart
-      constexpr uint32_t p_hi = (uint32_t)(16 * NQ >> 4) | 1u << 14 | (NQ == 64 ? 2u : NQ == 32 ? 4u : 6u) << 29;
-      const uint32_t klo = (kb >> 4) | 1u << 16, qlo = (qb >> 4) | 1u << 16, vlo = (kb >> 4) | (LD_UNIT >> 4) << 16;
-      const uint32_t plo = ((kb + nl * LD_UNIT) >> 4) | 1u << 16;
       const int su = nl + (R ? 1 : 0);
+      LdPos p;
+      p.at(g, sh->b0);
+      p.rb = sh->rb0;
+      p.tile = sh->tile0;
+      bool opens = true;             // the tile whose P V comes next is the first of its query block
+      auto values = [&](int i) {     // O^T += V^T P^T of tile i
+        ld_wait(&sh->pfull[i & 1], (i >> 1) & 1, abort);
+        tc_fence_after();
+        ld_values<NQ>(nblk, tmem, (kb + (i & 1) * LD_KBYTES) >> 4, nl, opens ? 0 : 1);
+        umma_commit(&sh->kfree[i & 1]);
+      };
       for (int i = 0; i < count; ++i) {
-        ld_wait(&sh->kfull, i & 1, abort);
+        const bool first = i == 0 || p.tile == 0;
+        // a new query block's tiles come only after the block before is finished
+        if (i > 0 && first) {
+          values(i - 1);
+          opens = true;
+        }
+        ld_wait(&sh->kfull[i & 1], (i >> 1) & 1, abort);
         tc_fence_after();
-        for (int s = 0; s < su; ++s)
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            umma_ss(ts, klo + s * (LD_UNIT >> 4) + 2 * ks, qlo + s * (NQ * 8) + 2 * ks, id_s, (s | ks) != 0);
-        umma_commit(&sh->sfull);
-        const uint32_t acc = *(volatile int*)&sh->first ? 0 : 1;
-        ld_wait(&sh->pfull, i & 1, abort);
-        tc_fence_after();
-        for (int m = 0; m < nblk; ++m)
-#pragma unroll
-          for (int ks = 0; ks < LD_TILE / 16; ++ks)
-            umma_ss2(tmem + m * NQ, vlo + m * (2 * LD_UNIT >> 4) + ks * 128, LP_DESC_HI, plo + ks * (2 * NQ), p_hi, id_o, acc | (ks > 0));
-        umma_commit(&sh->pvdone);
+        ld_scores<NQ>(su, ts + (i & 1) * NQ, (kb + (i & 1) * LD_KBYTES) >> 4, qb >> 4);
+        umma_commit(&sh->sfull[i & 1]);
+        if (i > 0 && !first) {
+          values(i - 1);
+          opens = false;
+        }
+        p.next(g);
       }
+      values(count - 1);
       umma_commit(&sh->drain);
       ld_wait(&sh->drain, 0, abort);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     if (count > 0) {
-    // ---------------- workers
-    const int quarter = warp & 3, grp = warp >> 2, kr = quarter * 32 + lane;   // softmax: cached row kr, columns grp * CPT ..
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const int col0 = grp * CPT;
-    LdPos cur, ahead;
-    cur.at(g, sh->b0);
-    cur.rb = sh->rb0;
-    cur.tile = sh->tile0;
-    ahead = cur;
+      // ---------------- workers
+      // softmax: S^T's row kr is in tensor-memory lane 32 quarter + (kr & 15); the upper 16 lanes of the warp take
+      // half of the column group's columns from the lower ones
+      const int quarter = warp & 3, grp = warp >> 2, kr = quarter * 16 + (lane & 15);
+      const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+      const int col0 = grp * CPT + (lane >> 4) * CPH;
+      LdPos cur, ahead;
+      cur.at(g, sh->b0);
+      cur.rb = sh->rb0;
+      cur.tile = sh->tile0;
+      ahead = cur;
 
-    // row offsets of the tile at `p` into buffer `buf` (the first 128 workers)
-    auto find_rows = [&](const LdPos& p, int buf) {
-      if (tid >= LD_TILE) return;
-      const int j = p.tile * LD_TILE + tid;
-      long long off = -1;
-      if (j < p.len) {
-        const uint32_t page_at = g.page_mul ? __umulhi((uint32_t)j, g.page_mul) >> g.page_shift : (uint32_t)j >> g.page_shift;
-        const long long page = a.block_table[(size_t)p.b * a.max_pages + page_at];
-        if (page < 0 || page >= a.pages) set_status(VQ2_ERR_SHAPE);
-        else off = (page * a.page_size + (j - (int)page_at * a.page_size)) * g.rb;
-      }
-      sh->rows[buf][tid] = off;
-    };
-    // a tile on its way through registers: 16 lanes take a row's latent in pieces of 32 values, 8 lanes its rotary part
-    uint4 lat[4], rope[2];
-    uint32_t sc[4];
-    const int piece = tid & 15, chunk = tid & 7;
-    auto load_rows = [&](int buf) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const long long off = sh->rows[buf][(tid >> 4) + 32 * k];
-        lat[k] = make_uint4(0, 0, 0, 0);
-        sc[k] = 0;
-        if (off >= 0 && piece < 2 * nl) {
-          const uint8_t* r = (const uint8_t*)a.cache + off;
-          lat[k] = __ldg((const uint4*)r + piece);
-          sc[k] = __ldg((const uint16_t*)(r + L / 2 + 2 * R) + (piece >> 1));
+      // row offsets of the tile at `p` into buffer `buf` (the first 64 workers)
+      auto find_rows = [&](const LdPos& p, int buf) {
+        if (tid >= LD_TILE) return;
+        const int j = p.tile * LD_TILE + tid;
+        long long off = -1;
+        if (j < p.len) {
+          const uint32_t page_at = g.page_mul ? __umulhi((uint32_t)j, g.page_mul) >> g.page_shift : (uint32_t)j >> g.page_shift;
+          const long long page = a.block_table[(size_t)p.b * a.max_pages + page_at];
+          if (page < 0 || page >= a.pages) set_status(VQ2_ERR_SHAPE);
+          else off = (page * a.page_size + (j - (int)page_at * a.page_size)) * g.rb;
         }
-      }
+        sh->rows[buf][tid] = off;
+      };
+      // a tile on its way through registers: 16 lanes take a row's latent in pieces of 32 values, 8 lanes its rotary part
+      uint4 lat[4], rope[2];
+      uint32_t sc[4];
+      const int piece = tid & 15, chunk = tid & 7;
+      auto load_rows = [&](int buf) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const long long off = sh->rows[buf][(tid >> 3) + 64 * k];
-        rope[k] = make_uint4(0, 0, 0, 0);
-        if (off >= 0 && chunk * 8 < R) rope[k] = __ldg((const uint4*)((const uint8_t*)a.cache + off + L / 2) + chunk);
-      }
-    };
-    // Registers -> tile. The 16 words' 8-value chunks of 8 neighbouring lanes (one row, pieces p .. p + 7) would fall on
-    // two bank groups; each lane starts at another of its four words, so that they fall on all eight.
-    const int turn = (piece >> 1) & 3;
-    auto expand = [&](int number) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (piece >= 2 * nl) break;
-        const int row = (tid >> 4) + 32 * k;
-        uint32_t s = sc[k];
-        if ((s & 0x7C00u) == 0x7C00u) {       // a non-finite scale: the row reads as NaN, see the softmax
-          s = 0;
-          sh->bad[row] = number;
+        for (int k = 0; k < 4; ++k) {
+          const long long off = sh->rows[buf][(tid >> 4) + 16 * k];
+          lat[k] = make_uint4(0, 0, 0, 0);
+          sc[k] = 0;
+          if (off >= 0 && piece < 2 * nl) {
+            const uint8_t* r = (const uint8_t*)a.cache + off;
+            lat[k] = __ldg((const uint4*)r + piece);
+            sc[k] = __ldg((const uint16_t*)(r + L / 2 + 2 * R) + (piece >> 1));
+          }
         }
-        const __half2 s2 = __half2half2(__ushort_as_half((unsigned short)s)), c2 = __hmul2(s2, __float2half2_rn(-24.f));
-        uint32_t w0 = lat[k].x, w1 = lat[k].y, w2 = lat[k].z, w3 = lat[k].w, t;
-        if (turn & 1) { t = w0; w0 = w1; w1 = w2; w2 = w3; w3 = t; }
-        if (turn & 2) { t = w0; w0 = w2; w2 = t; t = w1; w1 = w3; w3 = t; }
-        const uint32_t w[4] = {w0, w1, w2, w3};
-        const uint32_t base = kb + (piece >> 1) * LD_UNIT + row * 128;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          // nibble u = n + 8 in the top mantissa bits of 16 + u; (16 + u) s - 24 s = n s, exact in fp16
-          const uint32_t h[4] = {(w[q] << 6 & 0x03C003C0u) | 0x4C004C00u, (w[q] << 2 & 0x03C003C0u) | 0x4C004C00u,
-                                 (w[q] >> 2 & 0x03C003C0u) | 0x4C004C00u, (w[q] >> 6 & 0x03C003C0u) | 0x4C004C00u};
-          uint4 v;
-          __half2 x;
-          x = __hfma2(*(const __half2*)&h[0], s2, c2); v.x = *(uint32_t*)&x;
-          x = __hfma2(*(const __half2*)&h[1], s2, c2); v.y = *(uint32_t*)&x;
-          x = __hfma2(*(const __half2*)&h[2], s2, c2); v.z = *(uint32_t*)&x;
-          x = __hfma2(*(const __half2*)&h[3], s2, c2); v.w = *(uint32_t*)&x;
-          const int c = (piece & 1) * 4 + ((q + turn) & 3);
-          sts128_v(base + ((c ^ (row & 7)) << 4), v);
-        }
-      }
-      if (R) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int row = (tid >> 3) + 64 * k;
-          sts128_v(kb + nl * LD_UNIT + row * 128 + ((chunk ^ (row & 7)) << 4), rope[k]);
+          const long long off = sh->rows[buf][(tid >> 3) + 32 * k];
+          rope[k] = make_uint4(0, 0, 0, 0);
+          if (off >= 0 && chunk * 8 < R) rope[k] = __ldg((const uint4*)((const uint8_t*)a.cache + off + L / 2) + chunk);
         }
-      }
-    };
-    // Query rows of block (p.b, p.rb): rotated, scaled to fp16's range by a power of two, into Q's tile; a warp a row.
-    auto stage_q = [&](const LdPos& p) {
-      for (int r = warp; r < NQ; r += 16) {
-        const int row = p.rb * NQ + r, rows = a.T * a.heads;
-        const size_t at = ((size_t)p.b * rows + row) * (L + R);
-        float v[3][8];
-        float m = 0.f;
+      };
+      // Registers -> tile. A piece's four words become four 16-byte chunks; the chunks of 8 neighbouring lanes (one row,
+      // pieces p .. p + 7) would fall on two bank groups, so each lane starts at another of its words: all eight.
+      const int turn = (piece >> 1) & 3;
+      auto expand = [&](int number) {
+        const uint32_t tile = kb + (number & 1) * LD_KBYTES;
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          const int u = k < 2 ? lane + 32 * k : lane;          // 8-value unit: of the latent part, of the rotary part
+        for (int k = 0; k < 4; ++k) {
+          if (piece >= 2 * nl) break;
+          const int row = (tid >> 4) + 16 * k;
+          uint32_t s = sc[k];
+          if ((s & 0x7C00u) == 0x7C00u) {       // a non-finite scale: the row reads as NaN, see the softmax
+            s = 0;
+            sh->bad[number & 1][row] = number;
+          }
+          const __half2 s2 = __half2half2(__ushort_as_half((unsigned short)s)), c2 = __hmul2(s2, __float2half2_rn(-24.f));
+          uint32_t w0 = lat[k].x, w1 = lat[k].y, w2 = lat[k].z, w3 = lat[k].w, t;
+          if (turn & 1) { t = w0; w0 = w1; w1 = w2; w2 = w3; w3 = t; }
+          if (turn & 2) { t = w0; w0 = w2; w2 = t; t = w1; w1 = w3; w3 = t; }
+          const uint32_t w[4] = {w0, w1, w2, w3};
+          const uint32_t base = tile + (piece >> 1) * LD_UNIT + row * 128;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[k][i] = 0.f;
-          if (row < rows && u * 8 < (k < 2 ? L : R)) load8<DT>(a.q, at + (k < 2 ? 0 : L) + u * 8, v[k]);
-          if (k < 2) fwht64_lanes8(v[k]);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[k][i]));
+          for (int q = 0; q < 4; ++q) {
+            // nibble u = n + 8 in the top mantissa bits of 16 + u; (16 + u) s - 24 s = n s, exact in fp16
+            const uint32_t h[4] = {(w[q] << 6 & 0x03C003C0u) | 0x4C004C00u, (w[q] << 2 & 0x03C003C0u) | 0x4C004C00u,
+                                   (w[q] >> 2 & 0x03C003C0u) | 0x4C004C00u, (w[q] >> 6 & 0x03C003C0u) | 0x4C004C00u};
+            uint4 v;
+            __half2 x;
+            x = __hfma2(*(const __half2*)&h[0], s2, c2); v.x = *(uint32_t*)&x;
+            x = __hfma2(*(const __half2*)&h[1], s2, c2); v.y = *(uint32_t*)&x;
+            x = __hfma2(*(const __half2*)&h[2], s2, c2); v.z = *(uint32_t*)&x;
+            x = __hfma2(*(const __half2*)&h[3], s2, c2); v.w = *(uint32_t*)&x;
+            const int c = (piece & 1) * 4 + ((q + turn) & 3);
+            sts128_v(base + ((c ^ (row & 7)) << 4), v);
+          }
         }
-        const float2 f = f16_range_scale(fminf(warp_max(m), 3.0e38f));
+        if (R) {
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          const int u = k < 2 ? lane + 32 * k : lane;
-          const int unit = k < 2 ? u >> 3 : nl, c = u & 7;
-          if (k < 2 ? u * 8 < L : R && u < 8)
-            sts128_v(qb + unit * (NQ * 128) + r * 128 + ((c ^ (r & 7)) << 4),
-                     make_uint4(pack2<VQ2_DT_F16>(v[k][0] * f.x, v[k][1] * f.x), pack2<VQ2_DT_F16>(v[k][2] * f.x, v[k][3] * f.x),
-                                pack2<VQ2_DT_F16>(v[k][4] * f.x, v[k][5] * f.x), pack2<VQ2_DT_F16>(v[k][6] * f.x, v[k][7] * f.x)));
+          for (int k = 0; k < 2; ++k) {
+            const int row = (tid >> 3) + 32 * k;
+            sts128_v(tile + nl * LD_UNIT + row * 128 + ((chunk ^ (row & 7)) << 4), rope[k]);
+          }
         }
-        if (lane == 0) {
-          sh->fac[r] = a.scale * 1.4426950408889634f * f.y;
-          sh->lim[r] = row < rows ? max(0, min(p.len, p.len - a.T + 1 + row / a.heads)) : 0;
+      };
+      // Query rows of block (p.b, p.rb): rotated, scaled to fp16's range by a power of two, into Q's tile; a warp a row.
+      auto stage_q = [&](const LdPos& p) {
+        for (int r = warp; r < NQ; r += LD_WARPS) {
+          const int row = p.rb * NQ + r, rows = a.T * a.heads;
+          const size_t at = ((size_t)p.b * rows + row) * (L + R);
+          float v[3][8];
+          float m = 0.f;
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            const int u = k < 2 ? lane + 32 * k : lane;          // 8-value unit: of the latent part, of the rotary part
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[k][i] = 0.f;
+            if (row < rows && u * 8 < (k < 2 ? L : R)) load8<DT>(a.q, at + (k < 2 ? 0 : L) + u * 8, v[k]);
+            if (k < 2) fwht64_lanes8(v[k]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[k][i]));
+          }
+          const float2 f = f16_range_scale(fminf(warp_max(m), 3.0e38f));
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            const int u = k < 2 ? lane + 32 * k : lane;
+            const int unit = k < 2 ? u >> 3 : nl, c = u & 7;
+            if (k < 2 ? u * 8 < L : R && u < 8)
+              sts128_v(qb + unit * (NQ * 128) + r * 128 + ((c ^ (r & 7)) << 4),
+                       make_uint4(pack2<VQ2_DT_F16>(v[k][0] * f.x, v[k][1] * f.x), pack2<VQ2_DT_F16>(v[k][2] * f.x, v[k][3] * f.x),
+                                  pack2<VQ2_DT_F16>(v[k][4] * f.x, v[k][5] * f.x), pack2<VQ2_DT_F16>(v[k][6] * f.x, v[k][7] * f.x)));
+          }
+          if (lane == 0) {
+            sh->fac[r] = a.scale * 1.4426950408889634f * f.y;
+            sh->lim[r] = row < rows ? max(0, min(p.len, p.len - a.T + 1 + row / a.heads)) : 0;
+          }
         }
-      }
-    };
-    float l[CPT];
-    // O^T, with its maxima and denominators -> the result, or this block's part of it
-    auto finish = [&](const LdPos& p, int seg, bool whole) {
-#pragma unroll
-      for (int c = 0; c < CPT; ++c) {
-        const float s = warp_sum(l[c]);
-        if (lane == 0) sh->lsum[quarter][col0 + c] = s;
-      }
-      ld_sync_workers();
-      if (!whole) {
-        const size_t slot = 2 * (size_t)blockIdx.x + (seg > 0);
-        if (tid < NQ) g.ml[slot * NQ + tid] = make_float2(sh->ref[tid], (sh->lsum[0][tid] + sh->lsum[1][tid]) + (sh->lsum[2][tid] + sh->lsum[3][tid]));
-        for (int m = 0; m < nblk; ++m) {
-          float o[CPT];
-          ld_tmem_load<CPT>(tmem + lanes + m * NQ + col0, o);
-          const int d = m * 128 + kr;
-          if (d < L)
-#pragma unroll
-            for (int c = 0; c < CPT; ++c) g.part[(slot * NQ + col0 + c) * L + d] = o[c];
-        }
-        tc_fence_before();
-        return;
-      }
-      // through shared memory (the tile is free), 128 values a step, to have a row's group of 64 side by side
-      float* buf = (float*)smem;
-      constexpr int PITCH = 132;
-      for (int m = 0; m < nblk; ++m) {
-        float o[CPT];
-        ld_tmem_load<CPT>(tmem + lanes + m * NQ + col0, o);
-#pragma unroll
-        for (int c = 0; c < CPT; ++c) buf[(col0 + c) * PITCH + kr] = o[c];
-        ld_sync_workers();
-        for (int u = tid; u < NQ * 16; u += LD_WORKERS) {
-          const int r = u >> 4, d = (u & 15) * 8, row = p.rb * NQ + r;
-          const float den = (sh->lsum[0][r] + sh->lsum[1][r]) + (sh->lsum[2][r] + sh->lsum[3][r]);
-          const float inv = den != 0.f ? 1.f / den : 0.f;
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = den != 0.f ? buf[r * PITCH + d + i] * inv : 0.f;
-          fwht64_lanes8(v);
-          if (row < a.T * a.heads && m * 128 + d < L) store8<DT>(a.out, ((size_t)p.b * a.T * a.heads + row) * L + m * 128 + d, v);
-        }
-        ld_sync_workers();
-      }
-      tc_fence_before();
-    };
-
-    find_rows(ahead, 0);
-    ld_sync_workers();
-    load_rows(0);
-    if (count > 1) {
-      ahead.next(g);
-      find_rows(ahead, 1);
-    }
-    int seg = 0;
-    bool first = true, whole = false;
-    LdPos prev = cur;
-    for (int i = 0; i < count; ++i) {
-      if (i > 0) {
-        ld_wait(&sh->pvdone, (i - 1) & 1, abort);
+      };
+      float l[CPH];
+      // The softmax of tile i at p: logits from tensor memory, P into the rotary unit's place.
+      auto softmax = [&](int i, const LdPos& p, bool opens) {
+        ld_wait(&sh->sfull[i & 1], (i >> 1) & 1, abort);
         tc_fence_after();
-      }
-      if (first) {
-        if (i > 0) {
-          finish(prev, seg, whole);
-          ++seg;
-          ld_sync_workers();
+        float z[CPH], ref[CPH];
+        {
+          float full[CPT];
+          ld_tmem_load<CPT>(ts + (i & 1) * NQ + lanes + grp * CPT, full);
+#pragma unroll
+          for (int c = 0; c < CPH; ++c) {
+            const float up = __shfl_sync(0xffffffffu, full[CPH + c], lane & 15);
+            z[c] = lane < 16 ? full[c] : up;
+          }
         }
-        stage_q(cur);
-        whole = cur.tile == 0 && i + cur.tiles <= count;
+        const int j = p.tile * LD_TILE + kr;
+        const bool edge = (p.tile + 1) * LD_TILE > p.len - a.T + 1;           // some row sees part of the tile only
+        const bool gone = sh->rows[i & 3][kr] < 0;
+        bool raise = opens;
 #pragma unroll
-        for (int c = 0; c < CPT; ++c) l[c] = 0.f;
-      }
-      expand(i);
-      if (tid == 0) sh->first = first;
-      fence_async_smem();
-      tc_fence_before();
-      ld_sync_workers();
-      if (tid == 0) mbar_arrive(&sh->kfull);
-      // the next tile's loads go out now and land under the products
-      if (i + 1 < count) load_rows((i + 1) & 3);
-      if (i + 2 < count) {
-        ahead.next(g);
-        find_rows(ahead, (i + 2) & 3);
-      }
-      ld_wait(&sh->sfull, i & 1, abort);
-      tc_fence_after();
-      // ---------------- softmax of the tile: cached row kr, query rows col0 .. col0 + CPT - 1
-      float z[CPT], ref[CPT];
-      ld_tmem_load<CPT>(ts + lanes + col0, z);
-      const int j = cur.tile * LD_TILE + kr;
-      const bool edge = (cur.tile + 1) * LD_TILE > cur.len - a.T + 1;       // some row sees part of the tile only
-      const bool gone = sh->rows[i & 3][kr] < 0;
-      bool raise = first;
-#pragma unroll
-      for (int c = 0; c < CPT; ++c) {
-        z[c] *= sh->fac[col0 + c];
-        if (gone || (edge && j >= sh->lim[col0 + c])) z[c] = -INFINITY;
-        ref[c] = first ? -INFINITY : sh->ref[col0 + c];
-        raise |= z[c] > ref[c] + LD_RAISE;
-      }
-      if (sh->bad[kr] == i) {
-        // the latent is key and value: every query row that sees this one is NaN as a whole; its values
-        // were expanded to zeros, so that rows that do not see it are untouched
-#pragma unroll
-        for (int c = 0; c < CPT; ++c) {
-          if (z[c] != -INFINITY) l[c] = __int_as_float(0x7FFFFFFF);
-          z[c] = -INFINITY;
+        for (int c = 0; c < CPH; ++c) {
+          z[c] *= sh->fac[col0 + c];
+          if (gone || (edge && j >= sh->lim[col0 + c])) z[c] = -INFINITY;
+          ref[c] = opens ? -INFINITY : sh->ref[col0 + c];
+          raise |= z[c] > ref[c] + LD_RAISE;
         }
-      }
-      if (ld_any_group(grp, raise)) {
-        float mx[CPT];
+        if (sh->bad[i & 1][kr] == i) {
+          // the latent is key and value: every query row that sees this one is NaN as a whole; its values
+          // were expanded to zeros, so that rows that do not see it are untouched
 #pragma unroll
-        for (int c = 0; c < CPT; ++c) mx[c] = warp_max(z[c]);
-        if (lane == 0)
-#pragma unroll
-          for (int c = 0; c < CPT; ++c) sh->red[quarter][col0 + c] = mx[c];
-        ld_sync_group(grp);
-        float f[CPT];
-#pragma unroll
-        for (int c = 0; c < CPT; ++c) {
-          const float m = fmaxf(fmaxf(fmaxf(sh->red[0][col0 + c], sh->red[1][col0 + c]), fmaxf(sh->red[2][col0 + c], sh->red[3][col0 + c])),
-                                ref[c]);
-          f[c] = ref[c] == -INFINITY ? 0.f : ex2(ref[c] - m);
-          if (ref[c] == m) f[c] = 1.f;
-          ref[c] = m;
-          l[c] = l[c] == 0.f ? 0.f : l[c] * f[c];
+          for (int c = 0; c < CPH; ++c) {
+            if (z[c] != -INFINITY) l[c] = __int_as_float(0x7FFFFFFF);
+            z[c] = -INFINITY;
+          }
         }
-        if (!first)
+        if (ld_any_group(grp, raise)) {
+          float f[CPH];
+#pragma unroll
+          for (int c = 0; c < CPH; ++c) {
+            float m = z[c];
+#pragma unroll
+            for (int o = 8; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if ((lane & 15) == 0) sh->red[quarter][col0 + c] = m;
+          }
+          // O is rescaled below: every product into it so far has to be done (P V of the tile before)
+          if (!opens) ld_wait(&sh->kfree[(i - 1) & 1], ((i - 1) >> 1) & 1, abort);
+          tc_fence_after();
+          ld_sync_group(grp);
+#pragma unroll
+          for (int c = 0; c < CPH; ++c) {
+            const int k = col0 + c;
+            const float m = fmaxf(fmaxf(fmaxf(sh->red[0][k], sh->red[1][k]), fmaxf(sh->red[2][k], sh->red[3][k])), ref[c]);
+            f[c] = ref[c] == m ? 1.f : ref[c] == -INFINITY ? 0.f : ex2(ref[c] - m);
+            ref[c] = m;
+            l[c] = l[c] == 0.f ? 0.f : l[c] * f[c];
+          }
+          if (quarter == 0 && (lane & 15) == 0)
+#pragma unroll
+            for (int c = 0; c < CPH; ++c) sh->down[col0 + c] = f[c];
+          ld_sync_group(grp);                  // everyone has read the old maxima and the partial ones
+          if (!opens)
+#pragma unroll 1
+            for (int k = 0; k < nblk * (CPT / 8); ++k) {
+              const int c8 = grp * CPT + k % (CPT / 8) * 8;
+              const uint32_t at = tmem + lanes + k / (CPT / 8) * NQ + c8;
+              float o[8];
+              tmem_ld8(at, o);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) o[c] *= sh->down[c8 + c];
+              tmem_st8(at, (const uint32_t*)o);
+              tmem_st_wait();
+              keep_live8((const uint32_t*)o);
+            }
+          if (quarter == 0 && (lane & 15) == 0)
+#pragma unroll
+            for (int c = 0; c < CPH; ++c) sh->ref[col0 + c] = ref[c];
+        }
+        uint32_t ph[CPH / 2];
+#pragma unroll
+        for (int c = 0; c < CPH; c += 2) {
+          const float p0 = ex2(z[c] - ((ref[c] == -INFINITY ? 0.f : ref[c]) - LD_BIAS));
+          const float p1 = ex2(z[c + 1] - ((ref[c + 1] == -INFINITY ? 0.f : ref[c + 1]) - LD_BIAS));
+          l[c] += p0;
+          l[c + 1] += p1;
+          ph[c / 2] = pack2<VQ2_DT_F16>(p0, p1);
+        }
+        // rows of 2 NQ bytes, 16-byte chunks swizzled as the descriptor says
+        const uint32_t prow = kb + (i & 1) * LD_KBYTES + nl * LD_UNIT + kr * (2 * NQ), at = col0 * 2;
+        if (NQ == 64) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            sts128_v(prow + ((((at >> 4) + k) ^ (kr & 7)) << 4), make_uint4(ph[4 * k % (CPH / 2)], ph[(4 * k + 1) % (CPH / 2)],
+                                                                            ph[(4 * k + 2) % (CPH / 2)], ph[(4 * k + 3) % (CPH / 2)]));
+        } else if (NQ == 32) {
+          sts128_v(prow + (((at >> 4) ^ ((kr >> 1) & 3)) << 4), make_uint4(ph[0], ph[1], ph[2 % (CPH / 2)], ph[3 % (CPH / 2)]));
+        } else {
+          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(prow + (((at >> 4) ^ ((kr >> 2) & 1)) << 4) + (at & 15)), "r"(ph[0]), "r"(ph[1])
+                       : "memory");
+        }
+        fence_async_smem();
+        tc_fence_before();
+        ld_sync_workers();
+        if (tid == 0) mbar_arrive(&sh->pfull[i & 1]);
+      };
+      // O^T, with its maxima and denominators -> the result, or this block's part of it
+      auto finish = [&](const LdPos& p, int seg, bool whole) {
+#pragma unroll
+        for (int c = 0; c < CPH; ++c) {
+          float s = l[c];
+#pragma unroll
+          for (int o = 8; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          if ((lane & 15) == 0) sh->lsum[quarter][col0 + c] = s;
+        }
+        ld_sync_workers();
+        const int dl = quarter * 32 + lane;       // row of O^T within a block of 128
+        if (!whole) {
+          const size_t slot = 2 * (size_t)blockIdx.x + (seg > 0);
+          if (tid < NQ)
+            g.ml[slot * NQ + tid] = make_float2(sh->ref[tid], (sh->lsum[0][tid] + sh->lsum[1][tid]) + (sh->lsum[2][tid] + sh->lsum[3][tid]));
           for (int m = 0; m < nblk; ++m) {
             float o[CPT];
-            ld_tmem_load<CPT>(tmem + lanes + m * NQ + col0, o);
+            ld_tmem_load<CPT>(tmem + lanes + m * NQ + grp * CPT, o);
+            const int d = m * 128 + dl;
+            if (d < L)
 #pragma unroll
-            for (int c = 0; c < CPT; ++c) o[c] *= f[c];
-            ld_tmem_store<CPT>(tmem + lanes + m * NQ + col0, o);
+              for (int c = 0; c < CPT; ++c) g.part[(slot * NQ + grp * CPT + c) * L + d] = o[c];
           }
-        ld_sync_group(grp);                  // everyone has read the old maxima and the partial ones
-        if (quarter == 0 && lane == 0)
+          return;
+        }
+        // through shared memory (the tiles are free), 128 values a step, to have a row's group of 64 side by side
+        float* buf = (float*)smem;
+        constexpr int PITCH = 132;
+        for (int m = 0; m < nblk; ++m) {
+          float o[CPT];
+          ld_tmem_load<CPT>(tmem + lanes + m * NQ + grp * CPT, o);
 #pragma unroll
-          for (int c = 0; c < CPT; ++c) sh->ref[col0 + c] = ref[c];
-      }
-      uint32_t ph[CPT / 2];
+          for (int c = 0; c < CPT; ++c) buf[(grp * CPT + c) * PITCH + dl] = o[c];
+          ld_sync_workers();
+          for (int u = tid; u < NQ * 16; u += LD_WORKERS) {
+            const int r = u >> 4, d = (u & 15) * 8, row = p.rb * NQ + r;
+            const float den = (sh->lsum[0][r] + sh->lsum[1][r]) + (sh->lsum[2][r] + sh->lsum[3][r]);
+            const float inv = den != 0.f ? 1.f / den : 0.f;
+            float v[8];
 #pragma unroll
-      for (int c = 0; c < CPT; c += 2) {
-        float p0 = ex2(z[c] - (ref[c] == -INFINITY ? 0.f : ref[c]) + LD_BIAS);
-        float p1 = ex2(z[c + 1] - (ref[c + 1] == -INFINITY ? 0.f : ref[c + 1]) + LD_BIAS);
-        l[c] += p0;
-        l[c + 1] += p1;
-        ph[c / 2] = pack2<VQ2_DT_F16>(p0, p1);
-      }
-      // P takes the place of the rotary unit: rows of 2 NQ bytes, 16-byte chunks swizzled as the descriptor says
-      const uint32_t prow = kb + nl * LD_UNIT + kr * (2 * NQ);
-      if (NQ == 64) {
-        sts128_v(prow + (((2 * grp) ^ (kr & 7)) << 4), make_uint4(ph[0], ph[1], ph[2], ph[3]));
-        sts128_v(prow + (((2 * grp + 1) ^ (kr & 7)) << 4), make_uint4(ph[4 % (CPT / 2)], ph[5 % (CPT / 2)], ph[6 % (CPT / 2)], ph[7 % (CPT / 2)]));
-      } else if (NQ == 32) {
-        sts128_v(prow + ((grp ^ ((kr >> 1) & 3)) << 4), make_uint4(ph[0], ph[1], ph[2 % (CPT / 2)], ph[3 % (CPT / 2)]));
-      } else {
-        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(prow + (((grp >> 1) ^ ((kr >> 2) & 1)) << 4) + (grp & 1) * 8), "r"(ph[0]), "r"(ph[1])
-                     : "memory");
-      }
-      fence_async_smem();
-      tc_fence_before();
+            for (int i = 0; i < 8; ++i) v[i] = den != 0.f ? buf[r * PITCH + d + i] * inv : 0.f;
+            fwht64_lanes8(v);
+            if (row < a.T * a.heads && m * 128 + d < L) store8<DT>(a.out, ((size_t)p.b * a.T * a.heads + row) * L + m * 128 + d, v);
+          }
+          ld_sync_workers();
+        }
+      };
+
+      find_rows(ahead, 0);
       ld_sync_workers();
-      if (tid == 0) mbar_arrive(&sh->pfull);
-      prev = cur;
-      cur.next(g);
-      first = cur.tile == 0 || i + 1 == count;
-    }
-    ld_wait(&sh->pvdone, (count - 1) & 1, abort);
-    tc_fence_after();
-    finish(prev, seg, whole);
+      load_rows(0);
+      if (count > 1) {
+        ahead.next(g);
+        find_rows(ahead, 1);
+      }
+      int seg = 0;
+      bool whole = false, opens = true;        // of the tile before: its query block is all here; it is its first tile
+      LdPos prev = cur;
+      for (int i = 0; i <= count; ++i) {
+        const bool first = i < count && (i == 0 || cur.tile == 0);
+        if (i > 0 && (first || i == count)) {  // the query block before ends with tile i - 1
+          softmax(i - 1, prev, opens);
+          ld_wait(&sh->kfree[(i - 1) & 1], ((i - 1) >> 1) & 1, abort);
+          tc_fence_after();
+          finish(prev, seg, whole);
+          tc_fence_before();
+          ++seg;
+          if (i < count) ld_sync_workers();
+        }
+        if (i == count) break;
+        if (first) {
+          stage_q(cur);
+          whole = cur.tile == 0 && i + cur.tiles <= count;
+#pragma unroll
+          for (int c = 0; c < CPH; ++c) l[c] = 0.f;
+        }
+        if (i > 1) ld_wait(&sh->kfree[i & 1], ((i >> 1) - 1) & 1, abort);
+        expand(i);
+        fence_async_smem();
+        tc_fence_before();
+        ld_sync_workers();
+        if (tid == 0) mbar_arrive(&sh->kfull[i & 1]);
+        // the next tile's loads go out now and land under the products
+        if (i + 1 < count) load_rows((i + 1) & 3);
+        if (i + 2 < count) {
+          ahead.next(g);
+          find_rows(ahead, (i + 2) & 3);
+        }
+        if (i > 0 && !first) softmax(i - 1, prev, opens);
+        opens = first;
+        prev = cur;
+        cur.next(g);
+      }
     }
   }
   tc_fence_before();
   __syncthreads();
   __syncwarp();
-  if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS));
+  if (warp == LD_WARPS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS));
 }
 
 // Joins the parts of query blocks that several blocks worked on, in order; writes zeros for empty sequences. A thread

@@ -48,11 +48,6 @@ __device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint
                " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n}"
                ::"r"(d), "r"(a), "r"(b), "r"(LP_DESC_HI), "r"(idesc), "r"(acc));
 }
-__device__ __forceinline__ void umma_ss2(uint32_t d, uint32_t a, uint32_t a_hi, uint32_t b, uint32_t b_hi, uint32_t idesc, uint32_t acc) {
-  asm volatile("{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %6, 0;\n mov.b64 x, {%1, %2};\n mov.b64 y, {%3, %4};\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, p;\n}"
-               ::"r"(d), "r"(a), "r"(a_hi), "r"(b), "r"(b_hi), "r"(idesc), "r"(acc));
-}
 __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile("{\n .reg .pred p;\n .reg .b64 y;\n setp.ne.b32 p, %5, 0;\n mov.b64 y, {%2, %3};\n"
                " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n}"
