@@ -27,16 +27,9 @@ __host__ __device__ __forceinline__ bool latent_dims_ok(int L, int R) {
   return L > 0 && L <= LC_MAX_L && L % 64 == 0 && R >= 0 && R <= LC_MAX_R && R % 8 == 0;
 }
 
-// Eight consecutive activations (16-byte aligned for the 2-byte types, 32 for fp32).
+// Eight 16-bit values to fp32.
 template <int DT>
-__device__ __forceinline__ void load8(const void* p, size_t i, float* v) {
-  if (DT == VQ2_DT_F32) {
-    const float4* f = (const float4*)((const float*)p + i);
-    const float4 a = __ldg(f), b = __ldg(f + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    return;
-  }
-  const uint4 r = __ldg((const uint4*)((const uint16_t*)p + i));
+__device__ __forceinline__ void unpack8(const uint4& r, float* v) {
   const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -50,6 +43,18 @@ __device__ __forceinline__ void load8(const void* p, size_t i, float* v) {
     v[2 * k] = f.x;
     v[2 * k + 1] = f.y;
   }
+}
+
+// Eight consecutive activations (16-byte aligned for the 2-byte types, 32 for fp32).
+template <int DT>
+__device__ __forceinline__ void load8(const void* p, size_t i, float* v) {
+  if (DT == VQ2_DT_F32) {
+    const float4* f = (const float4*)((const float*)p + i);
+    const float4 a = __ldg(f), b = __ldg(f + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    return;
+  }
+  unpack8<DT>(__ldg((const uint4*)((const uint16_t*)p + i)), v);
 }
 
 // Two fp32 values rounded to a 16-bit type and packed.

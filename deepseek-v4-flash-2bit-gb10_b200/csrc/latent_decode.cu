@@ -14,11 +14,16 @@
 // 2^-34 of the largest still count; sums are fp32 in tensor memory.
 //
 // Work: the (sequence, block of NQ query rows, tile of 64 cached rows) triples in order, split evenly over one
-// block an SM. A block that holds all tiles of a query block writes the result; otherwise it
-// leaves its unnormalised sum, maximum and denominator, and the join kernel adds up the parts in order.
-// Roles: 8 worker warps load 64 rows ahead into registers, expand them into one of two tiles, and do the softmax
-// of the tile before with a thread per cached row and column group; one thread of a ninth warp issues
-// S of a tile before P V of the tile before it, so the products run under expansion and softmax.
+// block an SM; each block leaves, for every query block it worked on, its unnormalised sum, maximum and denominator.
+// Three launches, chained by programmatic dependent launch: `query` rotates and scales the query rows once and lays
+// them out as the product wants them (in each block, on 8 warps, that took 13,000 cycles a query block), the main kernel, and
+// `join`, which adds up the parts in order and rotates the result.
+// Roles: a loader warp brings in the cached rows as they are, one bulk copy a row (loads through
+// L1 have too few lines to be in flight beside 220 KB of shared memory); 8 worker warps expand a tile of 64 rows and do its softmax;
+// one thread issues the products. Both products are bound by reading the tile from shared memory, so that
+// path is kept busy: a tile is handed over in parts of 128 latent values, S starts on the first part, and
+// a part is filled again as soon as P V has used it. Up to 32 query rows there is room for two tiles, and the softmax of a
+// tile runs under the products of the next. In the steady state no barrier spans the block.
 #include "vq2_common.cuh"
 
 namespace vq2 {
@@ -39,38 +44,47 @@ struct LdArgs {
   long long capacity;   // cached rows
   uint32_t page_mul, page_shift;   // j / page_size = (j * mul) >> 32 >> shift (or j >> shift where mul is 0)
   int* start;           // [B + 1] first position of each sequence
-  float2* ml;           // [2 grid][NQ] maximum and denominator of a part
-  float* part;          // [2 grid][NQ][L]
+  float2* ml;           // [parts][NQ] maximum and denominator of a part
+  float* part;          // [parts][L][NQ]; a block's part of query block n is number n + block
+  uint8_t* q;           // [query blocks][units][NQ][128 bytes] rotated query rows, fp16, swizzled
+  float2* meta;         // [query blocks][NQ] factor of a row's logits, and its token (as int bits)
 };
+
+constexpr int LD_PARTS = 4;             // of a tile: two units each, the last with the rotary unit
+// A raw row in shared memory every 448 bytes (at most 400 are used): with 64 modulo 128, the 64-byte pieces that 4 lanes each
+// read of two neighbouring rows fall on different banks.
+constexpr int LD_RAW_ROW = 448, LD_RAW = LD_TILE * LD_RAW_ROW;
+// Tiles and raw tiles that fit beside Q (NQ x 1152 bytes) in 227 KB.
+template <int NQ> constexpr int LD_TILES = NQ == 64 ? 1 : 2;
+template <int NQ> constexpr int LD_RAWS = NQ == 32 ? 1 : 2;
 
 template <int NQ>
 struct LdShared {
-  uint64_t kfull[2], sfull[2], pfull[2], kfree[2], drain;      // by tile buffer
+  uint64_t kfull[2][LD_PARTS], kfree[2][LD_PARTS], sfull[2], pfull[2], drain;      // by tile buffer
+  uint64_t rfull[2], rfree[2];       // by raw tile
+  uint64_t qfull, qfree;
+  int there[2][LD_TILE];             // whether a raw row was found
   uint32_t tmem;
   int abort, b0, rb0, tile0;
-  long long rows[4][LD_TILE];        // byte offset of a cached row, -1: not there (written two tiles ahead, read until the softmax)
-  int bad[2][LD_TILE];               // number of the tile in which this row held a non-finite scale
+  int flag[2][LD_TILE];              // 2 i: the row is not there in tile i; 2 i + 1: it holds a non-finite scale
   float red[4][NQ];
-  float fac[NQ];                     // log2-scaled factor of a query row's logits
+  alignas(16) float2 meta[2][NQ];    // of this query block and the next
   float ref[NQ], down[NQ];           // maximum that P and O are relative to; factor of its last change
   float lsum[4][NQ];
-  int lim[NQ];                       // cached rows a query row sees
   int scan[LD_WARPS];
 };
 template <int NQ>
-constexpr size_t ld_smem() { return (size_t)2 * LD_KBYTES + (size_t)LD_UNITS * NQ * 128 + sizeof(LdShared<NQ>) + 1024; }
-static_assert(ld_smem<64>() <= 227 * 1024, "latent decode shared memory");
+constexpr size_t ld_smem() { return (size_t)LD_TILES<NQ> * LD_KBYTES + (size_t)LD_RAWS<NQ> * LD_RAW + (size_t)LD_UNITS * NQ * 128 + sizeof(LdShared<NQ>) + 1024; }
+static_assert(ld_smem<64>() <= 227 * 1024 && ld_smem<32>() <= 227 * 1024 && ld_smem<16>() <= 227 * 1024, "latent decode shared memory");
 
 // Wait that ends early once any thread of the block has given up; it never leaves the caller's loop,
-// so every thread keeps to the same sequence of block barriers.
-__device__ __forceinline__ bool ld_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  for (uint32_t i = 0; i < VQ2_WAIT_LIMIT; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 63) == 63 && *abort) return false;
-  }
-  set_status(VQ2_ERR_TIMEOUT);
-  *abort = 1;
-  return false;
+// so every thread keeps to the same sequence of block barriers. The block's last lines report the abort.
+__device__ __forceinline__ void ld_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  for (uint32_t i = 1; !mbar_try_wait(bar, parity); ++i)
+    if ((i & 63) == 0 && (*abort || i >= VQ2_WAIT_LIMIT)) {
+      *abort = 1;
+      return;
+    }
 }
 __device__ __forceinline__ void ld_sync_workers() { asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ void ld_sync_group(int g) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(2 + g) : "memory"); }
@@ -86,6 +100,12 @@ __device__ __forceinline__ void ld_tmem_load(uint32_t t, float* v) {
   else if (N == 16) tmem_ld16(t, v);
   else tmem_ld8(t, v);
 }
+// 32 bytes of fp32 in one store (a whole sector).
+__device__ __forceinline__ void store32(float* p, const float* v) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
+               "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
+}
+
 // Position of a tile: sequence, block of query rows, tile; the order is sequence, block, tile.
 struct LdPos {
   int b, rb, tile, len, tiles;
@@ -117,58 +137,75 @@ __device__ __forceinline__ void umma_at(uint32_t d, uint32_t a, uint32_t b, uint
 // The products of a tile, unrolled for each number of units: issued by one thread, with nothing but
 // constants added to two addresses, a product takes about 15 cycles to issue (with run-time loops and branches in
 // between about 50, which is more than the product itself takes).
-template <int NQ, int SU, int I = 0>
-__device__ __forceinline__ void ld_scores_n(uint32_t d, uint32_t k, uint32_t q) {
+template <int NQ, int U, int KS = 0>
+__device__ __forceinline__ void ld_score_unit(uint32_t d, uint32_t k, uint32_t q, uint32_t acc) {
   constexpr uint32_t id = (1u << 4) | ((uint32_t)(NQ >> 3) << 17) | ((uint32_t)(LD_TILE >> 4) << 24);
-  constexpr int s = I / 4, ks = I % 4;
-  umma_at<s * (LD_UNIT >> 4) + 2 * ks, s * (NQ * 8) + 2 * ks, LP_DESC_HI, id>(d, k, q, I != 0);
-  if constexpr (I + 1 < SU * 4) ld_scores_n<NQ, SU, I + 1>(d, k, q);
+  umma_at<U * (LD_UNIT >> 4) + 2 * KS, U * (NQ * 8) + 2 * KS, LP_DESC_HI, id>(d, k, q, U + KS > 0 ? 1 : acc);
+  if constexpr (KS < 3) ld_score_unit<NQ, U, KS + 1>(d, k, q, acc);
 }
+// Unit u of S, u known at run time (the rotary unit, or a last single one).
 template <int NQ>
-__device__ __forceinline__ void ld_scores(int su, uint32_t d, uint32_t k, uint32_t q) {
-  k |= 1u << 16;
-  q |= 1u << 16;
-  switch (su) {
-    case 1: return ld_scores_n<NQ, 1>(d, k, q);
-    case 2: return ld_scores_n<NQ, 2>(d, k, q);
-    case 3: return ld_scores_n<NQ, 3>(d, k, q);
-    case 4: return ld_scores_n<NQ, 4>(d, k, q);
-    case 5: return ld_scores_n<NQ, 5>(d, k, q);
-    case 6: return ld_scores_n<NQ, 6>(d, k, q);
-    case 7: return ld_scores_n<NQ, 7>(d, k, q);
-    case 8: return ld_scores_n<NQ, 8>(d, k, q);
-    default: return ld_scores_n<NQ, 9>(d, k, q);
-  }
+__device__ __forceinline__ void ld_score_any(int u, uint32_t d, uint32_t k, uint32_t q) {
+  ld_score_unit<NQ, 0>(d, k + u * (LD_UNIT >> 4), q + u * (NQ * 8), u > 0);
 }
-// O^T += V^T P^T: M = 128 latent values a block (the second unit of the last block may be P itself, where the latent has an
-// odd number of units: its rows of O^T are not read). P lies as rows of 2 NQ bytes in the swizzle of that width.
-template <int NQ, int NB, int I = 0>
-__device__ __forceinline__ void ld_values_n(uint32_t d, uint32_t v, uint32_t p, uint32_t acc) {
+// O^T block M += V^T P^T: 128 latent values (the second unit of the last block may be P itself, where the latent has an odd
+// number of units: its rows of O^T are not read). P lies as rows of 2 NQ bytes in the swizzle of that width.
+template <int NQ, int M, int KS = 0>
+__device__ __forceinline__ void ld_value_block(uint32_t d, uint32_t v, uint32_t p, uint32_t acc) {
   constexpr uint32_t id = (1u << 4) | (1u << 15) | (1u << 16) | ((uint32_t)(NQ >> 3) << 17) | ((128u >> 4) << 24);
   constexpr uint32_t p_hi = (uint32_t)(16 * NQ >> 4) | 1u << 14 | (NQ == 64 ? 2u : NQ == 32 ? 4u : 6u) << 29;
-  constexpr int ks = I / NB, m = I % NB;
-  umma_at<m * (2 * LD_UNIT >> 4) + ks * 128, ks * (2 * NQ), p_hi, id>(d + m * NQ, v, p, ks > 0 ? 1 : acc);
-  if constexpr (I + 1 < NB * (LD_TILE / 16)) ld_values_n<NQ, NB, I + 1>(d, v, p, acc);
-}
-template <int NQ>
-__device__ __forceinline__ void ld_values(int nblk, uint32_t d, uint32_t tile, int nl, uint32_t acc) {
-  const uint32_t v = tile | (LD_UNIT >> 4) << 16, p = (tile + nl * (LD_UNIT >> 4)) | 1u << 16;
-  switch (nblk) {
-    case 1: return ld_values_n<NQ, 1>(d, v, p, acc);
-    case 2: return ld_values_n<NQ, 2>(d, v, p, acc);
-    case 3: return ld_values_n<NQ, 3>(d, v, p, acc);
-    default: return ld_values_n<NQ, 4>(d, v, p, acc);
-  }
+  umma_at<M * (2 * LD_UNIT >> 4) + KS * 128, KS * (2 * NQ), p_hi, id>(d + M * NQ, v, p, KS > 0 ? 1 : acc);
+  if constexpr (KS + 1 < LD_TILE / 16) ld_value_block<NQ, M, KS + 1>(d, v, p, acc);
 }
 
+// Query rows -> the layout of Q's tile, one warp a row: latent part rotated, all scaled into fp16's range by a power of two.
+constexpr int LQ_WARPS = 4;
 template <int DT, int NQ>
+__global__ void __launch_bounds__(LQ_WARPS * 32) latent_query_kernel(LdArgs g) {
+  pdl_launch_dependents();
+  const vq2_latent_decode_args& a = g.a;
+  const int lane = threadIdx.x & 31, L = a.latent_dim, R = a.rope_dim, nl = L / 64, units = nl + (R ? 1 : 0), rows = a.T * a.heads;
+  const int at = blockIdx.x * LQ_WARPS + (threadIdx.x >> 5), item = at / NQ, r = at % NQ;          // query block, row in it
+  const int b = item / g.nrb, row = item % g.nrb * NQ + r;
+  const size_t q0 = ((size_t)b * rows + row) * (L + R);
+  float v[3][8], m = 0.f;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const int u = k < 2 ? lane + 32 * k : lane;          // 8-value unit: of the latent part, of the rotary part
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[k][i] = 0.f;
+    if (row < rows && u * 8 < (k < 2 ? L : R)) load8<DT>(a.q, q0 + (k < 2 ? 0 : L) + u * 8, v[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    if (k < 2) fwht64_lanes8(v[k]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[k][i]));
+  }
+  const float2 f = f16_range_scale(fminf(warp_max(m), 3.0e38f));
+  uint8_t* dst = g.q + (size_t)item * units * (NQ * 128) + r * 128;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const int u = k < 2 ? lane + 32 * k : lane, unit = k < 2 ? u >> 3 : nl, c = u & 7;
+    if (k < 2 ? u * 8 < L : R && u < 8)
+      *(uint4*)(dst + (size_t)unit * (NQ * 128) + ((c ^ (r & 7)) << 4)) =
+          make_uint4(pack2<VQ2_DT_F16>(v[k][0] * f.x, v[k][1] * f.x), pack2<VQ2_DT_F16>(v[k][2] * f.x, v[k][3] * f.x),
+                     pack2<VQ2_DT_F16>(v[k][4] * f.x, v[k][5] * f.x), pack2<VQ2_DT_F16>(v[k][6] * f.x, v[k][7] * f.x));
+  }
+  // a row that pads the block sees nothing
+  if (lane == 0)
+    g.meta[at] = make_float2(a.scale * 1.4426950408889634f * f.y, __int_as_float(row < rows ? row / a.heads : -(1 << 30)));
+}
+
+template <int NQ>
 __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) {
+  constexpr int TILES = LD_TILES<NQ>, RAWS = LD_RAWS<NQ>;
   constexpr int CPT = NQ / 2, CPH = NQ / 4;     // columns of S^T (query rows) a column group has, a softmax thread takes
   constexpr uint32_t COLS = NQ == 64 ? 512 : NQ == 32 ? 256 : 128;    // tensor memory: O^T 4 x NQ columns, S^T 2 x NQ
   extern __shared__ __align__(1024) uint8_t ld_smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)ld_smem_raw + 1023) & ~(uintptr_t)1023);
-  const uint32_t kb = smem_u32(smem), qb = kb + 2 * LD_KBYTES;
-  LdShared<NQ>* sh = (LdShared<NQ>*)(smem + 2 * LD_KBYTES + LD_UNITS * NQ * 128);
+  const uint32_t kb = smem_u32(smem), qb = kb + TILES * LD_KBYTES, raw = qb + LD_UNITS * NQ * 128;
+  LdShared<NQ>* sh = (LdShared<NQ>*)(smem + TILES * LD_KBYTES + LD_UNITS * NQ * 128 + RAWS * LD_RAW);
   const vq2_latent_decode_args& a = g.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int L = a.latent_dim, R = a.rope_dim, nl = L / 64, nblk = (nl + 1) / 2;
@@ -177,11 +214,17 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
 
   if (tid == 0) {
     for (int k = 0; k < 2; ++k) {
-      mbar_init(&sh->kfull[k], 1);
+      for (int m = 0; m < LD_PARTS; ++m) {
+        mbar_init(&sh->kfull[k][m], LD_WARPS);
+        mbar_init(&sh->kfree[k][m], 1);
+      }
       mbar_init(&sh->sfull[k], 1);
-      mbar_init(&sh->pfull[k], 1);
-      mbar_init(&sh->kfree[k], 1);
+      mbar_init(&sh->pfull[k], LD_WARPS);
+      mbar_init(&sh->rfull[k], 1);
+      mbar_init(&sh->rfree[k], LD_WARPS);
     }
+    mbar_init(&sh->qfull, 1);
+    mbar_init(&sh->qfree, 1);
     mbar_init(&sh->drain, 1);
     sh->abort = 0;
     fence_mbar_init();
@@ -190,7 +233,7 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem)), "r"(COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (tid < 2 * LD_TILE) sh->bad[tid >> 6][tid & 63] = -1;
+  if (tid < 2 * LD_TILE) sh->flag[tid >> 6][tid & 63] = -1;
 
   // ---------------- this block's share of the tiles. Each worker sums a run of sequences, a scan gives
   // the runs' first positions, and the worker whose run holds the block's first tile walks to it.
@@ -247,38 +290,136 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == LD_WARPS && count > 0 && elect_one()) {
       // ---------------- products
-      const int su = nl + (R ? 1 : 0);
       LdPos p;
       p.at(g, sh->b0);
       p.rb = sh->rb0;
       p.tile = sh->tile0;
       bool opens = true;             // the tile whose P V comes next is the first of its query block
-      auto values = [&](int i) {     // O^T += V^T P^T of tile i
-        ld_wait(&sh->pfull[i & 1], (i >> 1) & 1, abort);
+      auto values = [&](int i) {     // O^T += V^T P^T of tile i, a block of 128 values after another
+        const int b = i % TILES;
+        ld_wait(&sh->pfull[b], (i / TILES) & 1, abort);
         tc_fence_after();
-        ld_values<NQ>(nblk, tmem, (kb + (i & 1) * LD_KBYTES) >> 4, nl, opens ? 0 : 1);
-        umma_commit(&sh->kfree[i & 1]);
+        const uint32_t t = (kb + b * LD_KBYTES) >> 4, v = t | (LD_UNIT >> 4) << 16, pd = (t + nl * (LD_UNIT >> 4)) | 1u << 16;
+        const uint32_t acc = opens ? 0 : 1;
+        ld_value_block<NQ, 0>(tmem, v, pd, acc);
+        umma_commit(&sh->kfree[b][0]);
+        if (nblk > 1) {
+          ld_value_block<NQ, 1>(tmem, v, pd, acc);
+          umma_commit(&sh->kfree[b][1]);
+        }
+        if (nblk > 2) {
+          ld_value_block<NQ, 2>(tmem, v, pd, acc);
+          umma_commit(&sh->kfree[b][2]);
+        }
+        if (nblk > 3) {
+          ld_value_block<NQ, 3>(tmem, v, pd, acc);
+          umma_commit(&sh->kfree[b][3]);
+        }
       };
+      auto scores = [&](int i) {     // S^T = K Q^T of tile i, part by part as it arrives
+        const int b = i % TILES;
+        const uint32_t k = ((kb + b * LD_KBYTES) >> 4) | 1u << 16, q = (qb >> 4) | 1u << 16, d = ts + b * NQ;
+        auto part = [&](int m) {
+          ld_wait(&sh->kfull[b][m], (i / TILES) & 1, abort);
+          tc_fence_after();
+        };
+        part(0);
+        ld_score_unit<NQ, 0>(d, k, q, 0);
+        if (nl > 1) ld_score_unit<NQ, 1>(d, k, q, 1);
+        if (nl > 2) {
+          part(1);
+          ld_score_unit<NQ, 2>(d, k, q, 1);
+          if (nl > 3) ld_score_unit<NQ, 3>(d, k, q, 1);
+        }
+        if (nl > 4) {
+          part(2);
+          ld_score_unit<NQ, 4>(d, k, q, 1);
+          if (nl > 5) ld_score_unit<NQ, 5>(d, k, q, 1);
+        }
+        if (nl > 6) {
+          part(3);
+          ld_score_unit<NQ, 6>(d, k, q, 1);
+          if (nl > 7) ld_score_unit<NQ, 7>(d, k, q, 1);
+        }
+        if (R) ld_score_any<NQ>(nl, d, k, q);
+        umma_commit(&sh->sfull[b]);
+      };
+      int seg = -1;
       for (int i = 0; i < count; ++i) {
-        const bool first = i == 0 || p.tile == 0;
+        const bool first = i == 0 || p.tile == 0, last = i + 1 == count || p.tile + 1 == p.tiles;
         // a new query block's tiles come only after the block before is finished
-        if (i > 0 && first) {
+        if (TILES == 2 && i > 0 && first) {
           values(i - 1);
           opens = true;
         }
-        ld_wait(&sh->kfull[i & 1], (i >> 1) & 1, abort);
-        tc_fence_after();
-        ld_scores<NQ>(su, ts + (i & 1) * NQ, (kb + (i & 1) * LD_KBYTES) >> 4, qb >> 4);
-        umma_commit(&sh->sfull[i & 1]);
-        if (i > 0 && !first) {
+        if (TILES == 1) opens = first;
+        if (first) ld_wait(&sh->qfull, ++seg & 1, abort);
+        scores(i);
+        if (last) umma_commit(&sh->qfree);
+        if (TILES == 1) {
+          values(i);
+        } else if (i > 0 && !first) {
           values(i - 1);
           opens = false;
         }
         p.next(g);
       }
-      values(count - 1);
+      if (TILES == 2) values(count - 1);
       umma_commit(&sh->drain);
       ld_wait(&sh->drain, 0, abort);
+    } else if (warp == LD_WARPS + 1 && count > 0) {
+      // ---------------- loader: the whole warp, two rows a lane. Page numbers are read a tile ahead.
+      LdPos p;
+      p.at(g, sh->b0);
+      p.rb = sh->rb0;
+      p.tile = sh->tile0;
+      int j[2], page_at[2], page[2];
+      auto find = [&]() {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          j[k] = p.tile * LD_TILE + lane + 32 * k;
+          page_at[k] = (int)(g.page_mul ? __umulhi((uint32_t)j[k], g.page_mul) >> g.page_shift : (uint32_t)j[k] >> g.page_shift);
+          page[k] = j[k] < p.len ? __ldg(a.block_table + (size_t)p.b * a.max_pages + page_at[k]) : -1;
+        }
+      };
+      find();
+      int seg = -1;
+      for (int i = 0; i < count; ++i) {
+        const int st = i % RAWS;
+        if (i == 0 || p.tile == 0) {
+          // a query block's rows, once the products with the block before are done
+          const int bytes = (nl + (R ? 1 : 0)) * NQ * 128, item = p.b * g.nrb + p.rb;
+          if (++seg == 0) pdl_wait();
+          else ld_wait(&sh->qfree, (seg - 1) & 1, abort);
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&sh->qfull, bytes + NQ * 8);
+            bulk_g2s(smem + (qb - kb), g.q + (size_t)item * bytes, bytes, &sh->qfull);
+            bulk_g2s(sh->meta[seg & 1], g.meta + (size_t)item * NQ, NQ * 8, &sh->qfull);
+          }
+        }
+        long long off[2];
+        int rows = 0;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const bool in = page[k] >= 0 && page[k] < a.pages;
+          if (!in && j[k] < p.len) set_status(VQ2_ERR_SHAPE);
+          off[k] = in ? ((long long)page[k] * a.page_size + (j[k] - page_at[k] * a.page_size)) * g.rb : -1;
+          rows += __popc(__ballot_sync(0xffffffffu, in));
+        }
+        p.next(g);
+        if (i + 1 < count) find();
+        ld_wait(&sh->rfree[st], ((i / RAWS) & 1) ^ 1, abort);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) sh->there[st][lane + 32 * k] = off[k] >= 0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(&sh->rfull[st], rows * g.rb);
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (off[k] >= 0) bulk_g2s(smem + (raw - kb) + st * LD_RAW + (lane + 32 * k) * LD_RAW_ROW, (const uint8_t*)a.cache + off[k], g.rb, &sh->rfull[st]);
+      }
+      for (int i = max(0, count - RAWS); i < count; ++i) ld_wait(&sh->rfull[i % RAWS], (i / RAWS) & 1, abort);   // no copy left in flight
+      ld_wait(&sh->qfull, seg & 1, abort);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
@@ -289,151 +430,110 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
       const int quarter = warp & 3, grp = warp >> 2, kr = quarter * 16 + (lane & 15);
       const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
       const int col0 = grp * CPT + (lane >> 4) * CPH;
-      LdPos cur, ahead;
-      cur.at(g, sh->b0);
-      cur.rb = sh->rb0;
-      cur.tile = sh->tile0;
-      ahead = cur;
-
-      // row offsets of the tile at `p` into buffer `buf` (the first 64 workers)
-      auto find_rows = [&](const LdPos& p, int buf) {
-        if (tid >= LD_TILE) return;
-        const int j = p.tile * LD_TILE + tid;
-        long long off = -1;
-        if (j < p.len) {
-          const uint32_t page_at = g.page_mul ? __umulhi((uint32_t)j, g.page_mul) >> g.page_shift : (uint32_t)j >> g.page_shift;
-          const long long page = a.block_table[(size_t)p.b * a.max_pages + page_at];
-          if (page < 0 || page >= a.pages) set_status(VQ2_ERR_SHAPE);
-          else off = (page * a.page_size + (j - (int)page_at * a.page_size)) * g.rb;
-        }
-        sh->rows[buf][tid] = off;
-      };
-      // a tile on its way through registers: 16 lanes take a row's latent in pieces of 32 values, 8 lanes its rotary part
-      uint4 lat[4], rope[2];
-      uint32_t sc[4];
-      const int piece = tid & 15, chunk = tid & 7;
-      auto load_rows = [&](int buf) {
+      // A warp takes 8 rows of a tile: 4 lanes a row's latent, 64 bytes (two units) a part, and its scales; 8 lanes its
+      // rotary part. The raw tile goes into registers as a whole, so that its place is free for the one after.
+      uint4 lat[LD_PARTS], rope[2], sc;
+      bool here = false;
+      const int lrow = lane >> 2, piece = lane & 3, chunk = lane & 7;
+      auto read_raw = [&](int i) {
+        const int st = i % RAWS;
+        ld_wait(&sh->rfull[st], (i / RAWS) & 1, abort);
+        here = sh->there[st][warp * 8 + lrow] != 0;
+        const uint32_t r = raw + st * LD_RAW + (warp * 8 + lrow) * LD_RAW_ROW;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const long long off = sh->rows[buf][(tid >> 4) + 16 * k];
-          lat[k] = make_uint4(0, 0, 0, 0);
-          sc[k] = 0;
-          if (off >= 0 && piece < 2 * nl) {
-            const uint8_t* r = (const uint8_t*)a.cache + off;
-            lat[k] = __ldg((const uint4*)r + piece);
-            sc[k] = __ldg((const uint16_t*)(r + L / 2 + 2 * R) + (piece >> 1));
-          }
+        for (int m = 0; m < LD_PARTS; ++m) {
+          lat[m] = make_uint4(0, 0, 0, 0);
+          if (here && 4 * m + piece < 2 * nl) lat[m] = lds128_v(r + 64 * m + 16 * piece);
         }
+        sc = make_uint4(0, 0, 0, 0);
+        if (here) sc = lds128_v(r + L / 2 + 2 * R);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const long long off = sh->rows[buf][(tid >> 3) + 32 * k];
+          const int row = warp * 8 + (lane >> 3) + 4 * k;
           rope[k] = make_uint4(0, 0, 0, 0);
-          if (off >= 0 && chunk * 8 < R) rope[k] = __ldg((const uint4*)((const uint8_t*)a.cache + off + L / 2) + chunk);
+          if (chunk * 8 < R && sh->there[st][row]) rope[k] = lds128_v(raw + st * LD_RAW + row * LD_RAW_ROW + L / 2 + 16 * chunk);
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->rfree[st]);
       };
-      // Registers -> tile. A piece's four words become four 16-byte chunks; the chunks of 8 neighbouring lanes (one row,
-      // pieces p .. p + 7) would fall on two bank groups, so each lane starts at another of its words: all eight.
-      const int turn = (piece >> 1) & 3;
+      // Registers -> tile, a part after another. A piece's four words become four 16-byte chunks of a 128-byte row; lanes of the
+      // part's second unit take their words in another order, so that 8 neighbouring lanes fall on all bank groups.
       auto expand = [&](int number) {
-        const uint32_t tile = kb + (number & 1) * LD_KBYTES;
+        const int b = number % TILES, row = warp * 8 + lrow;
+        const uint32_t tile = kb + b * LD_KBYTES;
+        const uint32_t scale[LD_PARTS] = {sc.x, sc.y, sc.z, sc.w};
+        if (!here && piece == 0) sh->flag[b][row] = 2 * number;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (piece >= 2 * nl) break;
-          const int row = (tid >> 4) + 16 * k;
-          uint32_t s = sc[k];
-          if ((s & 0x7C00u) == 0x7C00u) {       // a non-finite scale: the row reads as NaN, see the softmax
-            s = 0;
-            sh->bad[number & 1][row] = number;
+        for (int m = 0; m < LD_PARTS; ++m) {
+          if (m >= nblk) break;
+          if (number >= TILES) ld_wait(&sh->kfree[b][m], (number / TILES - 1) & 1, abort);
+          uint32_t s = piece & 2 ? scale[m] >> 16 : scale[m] & 0xFFFFu;
+          if (4 * m + piece < 2 * nl) {
+            if ((s & 0x7C00u) == 0x7C00u) {       // a non-finite scale: the row reads as NaN, see the softmax
+              s = 0;
+              sh->flag[b][row] = 2 * number + 1;
+            }
+            const __half2 s2 = __half2half2(__ushort_as_half((unsigned short)s)), c2 = __hmul2(s2, __float2half2_rn(-24.f));
+            const uint32_t w[4] = {piece & 2 ? lat[m].z : lat[m].x, piece & 2 ? lat[m].w : lat[m].y, piece & 2 ? lat[m].x : lat[m].z,
+                                   piece & 2 ? lat[m].y : lat[m].w};
+            const uint32_t base = tile + (2 * m + (piece >> 1)) * LD_UNIT + row * 128;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              // nibble u = n + 8 in the top mantissa bits of 16 + u; (16 + u) s - 24 s = n s, exact in fp16
+              const uint32_t h[4] = {(w[q] << 6 & 0x03C003C0u) | 0x4C004C00u, (w[q] << 2 & 0x03C003C0u) | 0x4C004C00u,
+                                     (w[q] >> 2 & 0x03C003C0u) | 0x4C004C00u, (w[q] >> 6 & 0x03C003C0u) | 0x4C004C00u};
+              uint4 v;
+              __half2 x;
+              x = __hfma2(*(const __half2*)&h[0], s2, c2); v.x = *(uint32_t*)&x;
+              x = __hfma2(*(const __half2*)&h[1], s2, c2); v.y = *(uint32_t*)&x;
+              x = __hfma2(*(const __half2*)&h[2], s2, c2); v.z = *(uint32_t*)&x;
+              x = __hfma2(*(const __half2*)&h[3], s2, c2); v.w = *(uint32_t*)&x;
+              const int c = (piece & 1) * 4 + (q ^ (piece & 2));
+              sts128_v(base + ((c ^ (row & 7)) << 4), v);
+            }
           }
-          const __half2 s2 = __half2half2(__ushort_as_half((unsigned short)s)), c2 = __hmul2(s2, __float2half2_rn(-24.f));
-          uint32_t w0 = lat[k].x, w1 = lat[k].y, w2 = lat[k].z, w3 = lat[k].w, t;
-          if (turn & 1) { t = w0; w0 = w1; w1 = w2; w2 = w3; w3 = t; }
-          if (turn & 2) { t = w0; w0 = w2; w2 = t; t = w1; w1 = w3; w3 = t; }
-          const uint32_t w[4] = {w0, w1, w2, w3};
-          const uint32_t base = tile + (piece >> 1) * LD_UNIT + row * 128;
+          if (m == nblk - 1 && R) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            // nibble u = n + 8 in the top mantissa bits of 16 + u; (16 + u) s - 24 s = n s, exact in fp16
-            const uint32_t h[4] = {(w[q] << 6 & 0x03C003C0u) | 0x4C004C00u, (w[q] << 2 & 0x03C003C0u) | 0x4C004C00u,
-                                   (w[q] >> 2 & 0x03C003C0u) | 0x4C004C00u, (w[q] >> 6 & 0x03C003C0u) | 0x4C004C00u};
-            uint4 v;
-            __half2 x;
-            x = __hfma2(*(const __half2*)&h[0], s2, c2); v.x = *(uint32_t*)&x;
-            x = __hfma2(*(const __half2*)&h[1], s2, c2); v.y = *(uint32_t*)&x;
-            x = __hfma2(*(const __half2*)&h[2], s2, c2); v.z = *(uint32_t*)&x;
-            x = __hfma2(*(const __half2*)&h[3], s2, c2); v.w = *(uint32_t*)&x;
-            const int c = (piece & 1) * 4 + ((q + turn) & 3);
-            sts128_v(base + ((c ^ (row & 7)) << 4), v);
+            for (int k = 0; k < 2; ++k) {
+              const int r = warp * 8 + (lane >> 3) + 4 * k;
+              sts128_v(tile + nl * LD_UNIT + r * 128 + ((chunk ^ (r & 7)) << 4), rope[k]);
+            }
           }
-        }
-        if (R) {
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int row = (tid >> 3) + 32 * k;
-            sts128_v(tile + nl * LD_UNIT + row * 128 + ((chunk ^ (row & 7)) << 4), rope[k]);
-          }
-        }
-      };
-      // Query rows of block (p.b, p.rb): rotated, scaled to fp16's range by a power of two, into Q's tile; a warp a row.
-      auto stage_q = [&](const LdPos& p) {
-        for (int r = warp; r < NQ; r += LD_WARPS) {
-          const int row = p.rb * NQ + r, rows = a.T * a.heads;
-          const size_t at = ((size_t)p.b * rows + row) * (L + R);
-          float v[3][8];
-          float m = 0.f;
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            const int u = k < 2 ? lane + 32 * k : lane;          // 8-value unit: of the latent part, of the rotary part
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[k][i] = 0.f;
-            if (row < rows && u * 8 < (k < 2 ? L : R)) load8<DT>(a.q, at + (k < 2 ? 0 : L) + u * 8, v[k]);
-            if (k < 2) fwht64_lanes8(v[k]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[k][i]));
-          }
-          const float2 f = f16_range_scale(fminf(warp_max(m), 3.0e38f));
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            const int u = k < 2 ? lane + 32 * k : lane;
-            const int unit = k < 2 ? u >> 3 : nl, c = u & 7;
-            if (k < 2 ? u * 8 < L : R && u < 8)
-              sts128_v(qb + unit * (NQ * 128) + r * 128 + ((c ^ (r & 7)) << 4),
-                       make_uint4(pack2<VQ2_DT_F16>(v[k][0] * f.x, v[k][1] * f.x), pack2<VQ2_DT_F16>(v[k][2] * f.x, v[k][3] * f.x),
-                                  pack2<VQ2_DT_F16>(v[k][4] * f.x, v[k][5] * f.x), pack2<VQ2_DT_F16>(v[k][6] * f.x, v[k][7] * f.x)));
-          }
-          if (lane == 0) {
-            sh->fac[r] = a.scale * 1.4426950408889634f * f.y;
-            sh->lim[r] = row < rows ? max(0, min(p.len, p.len - a.T + 1 + row / a.heads)) : 0;
-          }
+          fence_async_smem();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->kfull[b][m]);
         }
       };
-      float l[CPH];
+      float l[CPH], ref[CPH], fac[CPH];      // of this thread's query rows: denominator (its cached rows), maximum, factor
       // The softmax of tile i at p: logits from tensor memory, P into the rotary unit's place.
-      auto softmax = [&](int i, const LdPos& p, bool opens) {
-        ld_wait(&sh->sfull[i & 1], (i >> 1) & 1, abort);
+      auto softmax = [&](int i, const LdPos& p, bool opens, int seg) {
+        const int b = i % TILES;
+        ld_wait(&sh->sfull[b], (i / TILES) & 1, abort);
+        ld_wait(&sh->kfull[b][nblk - 1], (i / TILES) & 1, abort);        // long done: orders the other warps' flags before their reads
         tc_fence_after();
-        float z[CPH], ref[CPH];
+        float z[CPH];
         {
           float full[CPT];
-          ld_tmem_load<CPT>(ts + (i & 1) * NQ + lanes + grp * CPT, full);
+          ld_tmem_load<CPT>(ts + b * NQ + lanes + grp * CPT, full);
 #pragma unroll
           for (int c = 0; c < CPH; ++c) {
             const float up = __shfl_sync(0xffffffffu, full[CPH + c], lane & 15);
-            z[c] = lane < 16 ? full[c] : up;
+            z[c] = (lane < 16 ? full[c] : up) * fac[c];
           }
         }
-        const int j = p.tile * LD_TILE + kr;
-        const bool edge = (p.tile + 1) * LD_TILE > p.len - a.T + 1;           // some row sees part of the tile only
-        const bool gone = sh->rows[i & 3][kr] < 0;
-        bool raise = opens;
+        const int flag = sh->flag[b][kr];
+        if ((p.tile + 1) * LD_TILE > p.len - a.T + 1) {              // some query row sees part of the tile only
+          const int j = p.tile * LD_TILE + kr;
 #pragma unroll
-        for (int c = 0; c < CPH; ++c) {
-          z[c] *= sh->fac[col0 + c];
-          if (gone || (edge && j >= sh->lim[col0 + c])) z[c] = -INFINITY;
-          ref[c] = opens ? -INFINITY : sh->ref[col0 + c];
-          raise |= z[c] > ref[c] + LD_RAISE;
+          for (int c = 0; c < CPH; ++c)
+            if (j > p.len - a.T + __float_as_int(sh->meta[seg & 1][col0 + c].y) || j >= p.len) z[c] = -INFINITY;
         }
-        if (sh->bad[i & 1][kr] == i) {
+        if (flag == 2 * i) {
+#pragma unroll
+          for (int c = 0; c < CPH; ++c) z[c] = -INFINITY;
+        }
+        if (flag == 2 * i + 1) {
           // the latent is key and value: every query row that sees this one is NaN as a whole; its values
           // were expanded to zeros, so that rows that do not see it are untouched
 #pragma unroll
@@ -442,6 +542,9 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
             z[c] = -INFINITY;
           }
         }
+        bool raise = opens;
+#pragma unroll
+        for (int c = 0; c < CPH; ++c) raise |= z[c] > ref[c] + LD_RAISE;
         if (ld_any_group(grp, raise)) {
           float f[CPH];
 #pragma unroll
@@ -452,7 +555,7 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
             if ((lane & 15) == 0) sh->red[quarter][col0 + c] = m;
           }
           // O is rescaled below: every product into it so far has to be done (P V of the tile before)
-          if (!opens) ld_wait(&sh->kfree[(i - 1) & 1], ((i - 1) >> 1) & 1, abort);
+          if (!opens) ld_wait(&sh->kfree[(i - 1) % TILES][nblk - 1], ((i - 1) / TILES) & 1, abort);
           tc_fence_after();
           ld_sync_group(grp);
 #pragma unroll
@@ -480,9 +583,6 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
               tmem_st_wait();
               keep_live8((const uint32_t*)o);
             }
-          if (quarter == 0 && (lane & 15) == 0)
-#pragma unroll
-            for (int c = 0; c < CPH; ++c) sh->ref[col0 + c] = ref[c];
         }
         uint32_t ph[CPH / 2];
 #pragma unroll
@@ -494,7 +594,7 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
           ph[c / 2] = pack2<VQ2_DT_F16>(p0, p1);
         }
         // rows of 2 NQ bytes, 16-byte chunks swizzled as the descriptor says
-        const uint32_t prow = kb + (i & 1) * LD_KBYTES + nl * LD_UNIT + kr * (2 * NQ), at = col0 * 2;
+        const uint32_t prow = kb + b * LD_KBYTES + nl * LD_UNIT + kr * (2 * NQ), at = col0 * 2;
         if (NQ == 64) {
 #pragma unroll
           for (int k = 0; k < 2; ++k)
@@ -508,146 +608,151 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
         }
         fence_async_smem();
         tc_fence_before();
-        ld_sync_workers();
-        if (tid == 0) mbar_arrive(&sh->pfull[i & 1]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->pfull[b]);
       };
-      // O^T, with its maxima and denominators -> the result, or this block's part of it
-      auto finish = [&](const LdPos& p, int seg, bool whole) {
+      // O^T with its maxima and denominators -> this block's part of the query block
+      auto finish = [&](const LdPos& p) {
+        const size_t slot = (size_t)(p.b * g.nrb + p.rb) + blockIdx.x;
 #pragma unroll
         for (int c = 0; c < CPH; ++c) {
           float s = l[c];
 #pragma unroll
           for (int o = 8; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-          if ((lane & 15) == 0) sh->lsum[quarter][col0 + c] = s;
-        }
-        ld_sync_workers();
-        const int dl = quarter * 32 + lane;       // row of O^T within a block of 128
-        if (!whole) {
-          const size_t slot = 2 * (size_t)blockIdx.x + (seg > 0);
-          if (tid < NQ)
-            g.ml[slot * NQ + tid] = make_float2(sh->ref[tid], (sh->lsum[0][tid] + sh->lsum[1][tid]) + (sh->lsum[2][tid] + sh->lsum[3][tid]));
-          for (int m = 0; m < nblk; ++m) {
-            float o[CPT];
-            ld_tmem_load<CPT>(tmem + lanes + m * NQ + grp * CPT, o);
-            const int d = m * 128 + dl;
-            if (d < L)
-#pragma unroll
-              for (int c = 0; c < CPT; ++c) g.part[(slot * NQ + grp * CPT + c) * L + d] = o[c];
+          if ((lane & 15) == 0) {
+            sh->lsum[quarter][col0 + c] = s;
+            if (quarter == 0) sh->ref[col0 + c] = ref[c];
           }
-          return;
         }
-        // through shared memory (the tiles are free), 128 values a step, to have a row's group of 64 side by side
-        float* buf = (float*)smem;
-        constexpr int PITCH = 132;
+#pragma unroll 1
         for (int m = 0; m < nblk; ++m) {
           float o[CPT];
           ld_tmem_load<CPT>(tmem + lanes + m * NQ + grp * CPT, o);
+          const int d = m * 128 + quarter * 32 + lane;
+          if (d < L)
 #pragma unroll
-          for (int c = 0; c < CPT; ++c) buf[(grp * CPT + c) * PITCH + dl] = o[c];
-          ld_sync_workers();
-          for (int u = tid; u < NQ * 16; u += LD_WORKERS) {
-            const int r = u >> 4, d = (u & 15) * 8, row = p.rb * NQ + r;
-            const float den = (sh->lsum[0][r] + sh->lsum[1][r]) + (sh->lsum[2][r] + sh->lsum[3][r]);
-            const float inv = den != 0.f ? 1.f / den : 0.f;
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = den != 0.f ? buf[r * PITCH + d + i] * inv : 0.f;
-            fwht64_lanes8(v);
-            if (row < a.T * a.heads && m * 128 + d < L) store8<DT>(a.out, ((size_t)p.b * a.T * a.heads + row) * L + m * 128 + d, v);
-          }
-          ld_sync_workers();
+            for (int c = 0; c < CPT; c += 8) store32(g.part + (slot * L + d) * NQ + grp * CPT + c, o + c);
         }
+        ld_sync_workers();
+        if (tid < NQ)
+          g.ml[slot * NQ + tid] = make_float2(sh->ref[tid], (sh->lsum[0][tid] + sh->lsum[1][tid]) + (sh->lsum[2][tid] + sh->lsum[3][tid]));
+        ld_sync_workers();
       };
 
-      find_rows(ahead, 0);
-      ld_sync_workers();
-      load_rows(0);
-      if (count > 1) {
-        ahead.next(g);
-        find_rows(ahead, 1);
-      }
-      int seg = 0;
-      bool whole = false, opens = true;        // of the tile before: its query block is all here; it is its first tile
-      LdPos prev = cur;
-      for (int i = 0; i <= count; ++i) {
-        const bool first = i < count && (i == 0 || cur.tile == 0);
-        if (i > 0 && (first || i == count)) {  // the query block before ends with tile i - 1
-          softmax(i - 1, prev, opens);
-          ld_wait(&sh->kfree[(i - 1) & 1], ((i - 1) >> 1) & 1, abort);
-          tc_fence_after();
-          finish(prev, seg, whole);
-          tc_fence_before();
-          ++seg;
-          if (i < count) ld_sync_workers();
-        }
-        if (i == count) break;
-        if (first) {
-          stage_q(cur);
-          whole = cur.tile == 0 && i + cur.tiles <= count;
+      // Tiles are expanded up to TILES ahead of the softmax, but not past the end of a query block (pe, ps: the next of each).
+      LdPos pe, ps;
+      pe.at(g, sh->b0);
+      pe.rb = sh->rb0;
+      pe.tile = sh->tile0;
+      ps = pe;
+      int ie = 0, is = 0, seg = -1;
+      read_raw(0);
+      while (is < count) {
+        const bool first = ie == 0 || pe.tile == 0;
+        if (ie < count && ie - is < TILES && (!first || ie == is)) {
+          if (first) {
+            ld_wait(&sh->qfull, ++seg & 1, abort);
 #pragma unroll
-          for (int c = 0; c < CPH; ++c) l[c] = 0.f;
+            for (int c = 0; c < CPH; ++c) {
+              l[c] = 0.f;
+              ref[c] = -INFINITY;
+              fac[c] = sh->meta[seg & 1][col0 + c].x;
+            }
+          }
+          expand(ie);
+          if (++ie < count) read_raw(ie);
+          pe.next(g);
+          if (ie < count && ie - is < TILES && pe.tile != 0) continue;
         }
-        if (i > 1) ld_wait(&sh->kfree[i & 1], ((i >> 1) - 1) & 1, abort);
-        expand(i);
-        fence_async_smem();
-        tc_fence_before();
-        ld_sync_workers();
-        if (tid == 0) mbar_arrive(&sh->kfull[i & 1]);
-        // the next tile's loads go out now and land under the products
-        if (i + 1 < count) load_rows((i + 1) & 3);
-        if (i + 2 < count) {
-          ahead.next(g);
-          find_rows(ahead, (i + 2) & 3);
+        softmax(is, ps, is == 0 || ps.tile == 0, seg);
+        if (is + 1 == count || ps.tile + 1 == ps.tiles) {
+          ld_wait(&sh->kfree[is % TILES][nblk - 1], (is / TILES) & 1, abort);
+          tc_fence_after();
+          finish(ps);
+          tc_fence_before();
         }
-        if (i > 0 && !first) softmax(i - 1, prev, opens);
-        opens = first;
-        prev = cur;
-        cur.next(g);
+        ++is;
+        ps.next(g);
       }
     }
   }
   tc_fence_before();
   __syncthreads();
   __syncwarp();
+  if (tid == 0 && *abort) set_status(VQ2_ERR_TIMEOUT);
+  pdl_wait();        // also where there was nothing to do: the query kernel is done when this one is
   if (warp == LD_WARPS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS));
 }
 
-// Joins the parts of query blocks that several blocks worked on, in order; writes zeros for empty sequences. A thread
-// takes 8 values of a query row.
+// Adds up the parts of a query block in order, divides and rotates; writes zeros for empty sequences. A block takes
+// 64 values of NQ query rows: a thread 8 of the values of some rows, first along the rows (as the parts lie), then, through
+// shared memory, along the values (for the rotation).
+constexpr int LJ_THREADS = 128;
 template <int DT, int NQ>
-__global__ void __launch_bounds__(256) latent_join_kernel(LdArgs g) {
+__global__ void __launch_bounds__(LJ_THREADS) latent_join_kernel(LdArgs g) {
+  constexpr int LANES = NQ / 4, DS = LJ_THREADS / LANES;      // threads along the rows (4 each), values side by side
+  __shared__ float buf[NQ][65];
+  __shared__ float den[NQ];
   pdl_wait();
   const vq2_latent_decode_args& a = g.a;
-  const int L = a.latent_dim, U = L / 8, rows = a.T * a.heads;
-  const long long idx = (long long)blockIdx.x * 256 + threadIdx.x, row = idx / U;
-  const int d = (int)(idx - row * U) * 8;
-  const bool in = row < (long long)a.B * rows;
-  const int b = in ? (int)(row / rows) : 0, r = in ? (int)(row - (long long)b * rows) : 0;
+  const int L = a.latent_dim, rows = a.T * a.heads, tid = threadIdx.x;
+  const int item = blockIdx.x / (L / 64), d0 = blockIdx.x % (L / 64) * 64, b = item / g.nrb, rb = item % g.nrb;
   const int total = g.start[a.B], quota = max(1, (total + g.grid - 1) / g.grid);
   const int s0 = g.start[b], tiles = (g.start[b + 1] - s0) / g.nrb;
-  const int begin = s0 + r / NQ * tiles, end = begin + tiles;
+  const int begin = s0 + rb * tiles, end = begin + tiles;
   const int c0 = begin / quota, c1 = tiles ? (end - 1) / quota : c0;
-  const bool mine = in && (tiles == 0 || c1 > c0);
-  if (!__any_sync(0xffffffffu, mine)) return;
-  float v[8] = {}, m = -INFINITY, l = 0.f;
-  if (mine && tiles) {
-    for (int c = c0; c <= c1; ++c) m = fmaxf(m, g.ml[(2 * c + (c == c0 && begin != c * quota)) * NQ + r % NQ].x);
+  const int r4 = tid % LANES * 4, dl = tid / LANES;
+  auto slot = [&](int c) { return (size_t)item + c; };
+  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, l[4] = {};
+  float4 v[64 / DS];
+#pragma unroll
+  for (int k = 0; k < 64 / DS; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (tiles) {
+    for (int c = c0; c <= c1; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m[i] = fmaxf(m[i], g.ml[slot(c) * NQ + r4 + i].x);
+#pragma unroll 2
     for (int c = c0; c <= c1; ++c) {
-      const size_t at = (size_t)(2 * c + (c == c0 && begin != c * quota)) * NQ + r % NQ;
-      const float2 ml = g.ml[at];
-      const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - m);
-      l += ml.y * f;
-      const float4* p = (const float4*)(g.part + at * L + d);
-      const float4 x = p[0], y = p[1];
-      v[0] = fmaf(f, x.x, v[0]); v[1] = fmaf(f, x.y, v[1]); v[2] = fmaf(f, x.z, v[2]); v[3] = fmaf(f, x.w, v[3]);
-      v[4] = fmaf(f, y.x, v[4]); v[5] = fmaf(f, y.y, v[5]); v[6] = fmaf(f, y.z, v[6]); v[7] = fmaf(f, y.w, v[7]);
+      const float4* p = (const float4*)(g.part + (slot(c) * L + d0 + dl) * NQ + r4);
+      float4 x[64 / DS];
+#pragma unroll
+      for (int k = 0; k < 64 / DS; ++k) x[k] = __ldg(p + (size_t)k * DS * (NQ / 4));
+      float f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 ml = g.ml[slot(c) * NQ + r4 + i];
+        f[i] = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - m[i]);
+        l[i] += ml.y * f[i];
+      }
+#pragma unroll
+      for (int k = 0; k < 64 / DS; ++k) {
+        v[k].x = fmaf(f[0], x[k].x, v[k].x);
+        v[k].y = fmaf(f[1], x[k].y, v[k].y);
+        v[k].z = fmaf(f[2], x[k].z, v[k].z);
+        v[k].w = fmaf(f[3], x[k].w, v[k].w);
+      }
     }
   }
-  const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = l != 0.f ? v[i] * inv : 0.f;
-  fwht64_lanes8(v);
-  if (mine) store8<DT>(a.out, (size_t)row * L + d, v);
+  for (int k = 0; k < 64 / DS; ++k) {
+    buf[r4][dl + k * DS] = v[k].x;
+    buf[r4 + 1][dl + k * DS] = v[k].y;
+    buf[r4 + 2][dl + k * DS] = v[k].z;
+    buf[r4 + 3][dl + k * DS] = v[k].w;
+  }
+  if (dl == 0)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) den[r4 + i] = l[i];
+  __syncthreads();
+  for (int u = tid; u < NQ * 8; u += LJ_THREADS) {
+    const int r = u >> 3, row = rb * NQ + r;
+    const float q = den[r], inv = q != 0.f ? 1.f / q : 0.f;
+    float o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = q != 0.f ? buf[r][(u & 7) * 8 + i] * inv : 0.f;
+    fwht64_lanes8(o);
+    if (row < rows) store8<DT>(a.out, ((size_t)b * rows + row) * L + d0 + (u & 7) * 8, o);
+  }
 }
 
 static int ld_nq(int T, int heads) {
@@ -656,34 +761,48 @@ static int ld_nq(int T, int heads) {
 }
 
 struct LdLayout {
-  size_t start, ml, part, total;
+  size_t start, ml, meta, q, part, total;
 };
-static LdLayout ld_layout(int B, int nq, int L, int grid) {
+static LdLayout ld_layout(int B, int nq, int nrb, int L, int R, int grid) {
+  const size_t items = (size_t)B * nrb, parts = items + grid;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t p = at;
+    at += (bytes + 255) / 256 * 256;
+    return p;
+  };
   LdLayout w;
-  w.start = 0;
-  w.ml = ((size_t)(B + 1) * 4 + 255) / 256 * 256;
-  w.part = w.ml + ((size_t)2 * grid * nq * 8 + 255) / 256 * 256;
-  w.total = w.part + (size_t)2 * grid * nq * L * 4 + 256;
+  w.start = take((size_t)(B + 1) * 4);
+  w.ml = take(parts * nq * 8);
+  w.meta = take(items * nq * 8);
+  w.q = take(items * (L / 64 + (R ? 1 : 0)) * nq * 128);
+  w.part = take(parts * nq * L * 4);
+  w.total = at + 256;
   return w;
 }
 constexpr int LD_MAX_GRID = 148;        // workspace is sized without a device; a B200 has 148 SMs
 
 template <int DT, int NQ>
 static int ld_launch(const LdArgs& g, cudaStream_t st) {
-  auto kernel = latent_decode_kernel<DT, NQ>;
+  auto kernel = latent_decode_kernel<NQ>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ld_smem<NQ>()) != cudaSuccess) return VQ2_ERR_CUDA;
-  kernel<<<g.grid, LD_THREADS, ld_smem<NQ>(), st>>>(g);
+  const int items = g.a.B * g.nrb;
+  latent_query_kernel<DT, NQ><<<items * NQ / LQ_WARPS, LQ_WARPS * 32, 0, st>>>(g);
   if (cudaGetLastError() != cudaSuccess) return VQ2_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
-  const long long threads = (long long)g.a.B * g.a.T * g.a.heads * (g.a.latent_dim / 8);
-  cfg.gridDim = dim3((unsigned)((threads + 255) / 256));
-  cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  cfg.gridDim = dim3(g.grid);
+  cfg.blockDim = dim3(LD_THREADS);
+  cfg.dynamicSmemBytes = ld_smem<NQ>();
+  if (cudaLaunchKernelEx(&cfg, kernel, g) != cudaSuccess) return VQ2_ERR_CUDA;
+  cfg.gridDim = dim3((unsigned)(items * (g.a.latent_dim / 64)));
+  cfg.blockDim = dim3(LJ_THREADS);
+  cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, latent_join_kernel<DT, NQ>, g) == cudaSuccess ? VQ2_OK : VQ2_ERR_CUDA;
 }
 
@@ -692,15 +811,18 @@ static int ld_launch(const LdArgs& g, cudaStream_t st) {
 using namespace vq2;
 
 extern "C" size_t vq2_latent_decode_workspace_size(int B, int T, int heads, int latent_dim, int rope_dim) {
-  if (B <= 0 || T <= 0 || heads <= 0 || !latent_dims_ok(latent_dim, rope_dim)) return 0;
-  return ld_layout(B, ld_nq(T, heads), latent_dim, LD_MAX_GRID).total;
+  if (B <= 0 || T <= 0 || heads <= 0 || !latent_dims_ok(latent_dim, rope_dim) || (long long)T * heads > 1 << 20 ||
+      (long long)B * ((long long)T * heads + 64) >= 1LL << 28)
+    return 0;
+  const int nq = ld_nq(T, heads);
+  return ld_layout(B, nq, (int)(((long long)T * heads + nq - 1) / nq), latent_dim, rope_dim, LD_MAX_GRID).total;
 }
 
 extern "C" int vq2_latent_decode(const vq2_latent_decode_args* a, void* ws, size_t ws_bytes, void* stream) {
   if (!a || !a->q || !a->cache || !a->block_table || !a->kv_len || !a->out) return VQ2_ERR_NULL;
   if (a->B <= 0 || a->T <= 0 || a->heads <= 0 || a->page_size <= 0 || a->max_pages <= 0 || a->pages <= 0 ||
       !latent_dims_ok(a->latent_dim, a->rope_dim) || !(a->scale > 0.f) || (long long)a->T * a->heads > 1 << 20 ||
-      (long long)a->B * a->T * a->heads * (a->latent_dim / 8) / 256 >= 0x7FFFFFFFLL)
+      (long long)a->B * ((long long)a->T * a->heads + 64) >= 1LL << 28)
     return VQ2_ERR_SHAPE;
   if (a->dtype != VQ2_DT_BF16 && a->dtype != VQ2_DT_F16) return VQ2_ERR_DTYPE;
   if (((uintptr_t)a->q | (uintptr_t)a->cache | (uintptr_t)a->out) & 15) return VQ2_ERR_ALIGN;
@@ -724,11 +846,13 @@ extern "C" int vq2_latent_decode(const vq2_latent_decode_args* a, void* ws, size
     g.page_mul = (uint32_t)(((1ULL << (31 + s)) + a->page_size - 1) / a->page_size);
     g.page_shift = s - 1;
   }
-  const LdLayout w = ld_layout(a->B, nq, a->latent_dim, g.grid);
+  const LdLayout w = ld_layout(a->B, nq, g.nrb, a->latent_dim, a->rope_dim, g.grid);
   uint8_t* base = (uint8_t*)(((uintptr_t)ws + 255) & ~(uintptr_t)255);
   g.start = (int*)(base + w.start);
   g.ml = (float2*)(base + w.ml);
   g.part = (float*)(base + w.part);
+  g.q = base + w.q;
+  g.meta = (float2*)(base + w.meta);
   cudaStream_t st = (cudaStream_t)stream;
   const bool bf = a->dtype == VQ2_DT_BF16;
   if (nq == 16) return bf ? ld_launch<VQ2_DT_BF16, 16>(g, st) : ld_launch<VQ2_DT_F16, 16>(g, st);
