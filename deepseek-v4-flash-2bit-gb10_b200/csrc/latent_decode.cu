@@ -10,8 +10,8 @@
 //   O^T [L x NQ]        += V^T P^T     the same tile read along the other direction (MN-major): the
 //                                      latent is key and value, expanded from 4 bits once for both
 // A row is held as n s in fp16, which is exact (|n| <= 7, s has 8 significant bits), q in fp16 with a
-// power-of-two scale a row, P in fp16 with its largest values between 2^10 and 2^15, so that values down to
-// 2^-34 of the largest still count; sums are fp32 in tensor memory.
+// power-of-two scale a row, P in fp16 with its largest values between 2^5 and 2^15, so that values down to
+// 2^-29 of the largest still count; sums are fp32 in tensor memory.
 //
 // Work: the (sequence, block of NQ query rows, tile of 64 cached rows) triples in order, split evenly over one
 // block an SM; each block leaves, for every query block it worked on, its unnormalised sum, maximum and denominator.
@@ -34,7 +34,7 @@ constexpr int LD_THREADS = LD_WORKERS + 128;     // 168 registers each at launch
 constexpr int LD_UNIT = LD_TILE * 128;  // bytes of a unit of the tile: 64 rows of 64 fp16 values
 constexpr int LD_UNITS = 9;             // 8 for the latent, 1 for the rotary part (P takes its place once S is done)
 constexpr int LD_KBYTES = LD_UNITS * LD_UNIT;
-constexpr float LD_BIAS = 10.f, LD_RAISE = 5.f;    // P = 2^(z - m + BIAS); m is raised when z exceeds it by RAISE
+constexpr float LD_BIAS = 5.f, LD_RAISE = 10.f;    // P = 2^(z - m + BIAS); m is raised when z exceeds it by RAISE
 
 struct LdArgs {
   vq2_latent_decode_args a;
@@ -684,75 +684,74 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
   if (warp == LD_WARPS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS));
 }
 
-// Adds up the parts of a query block in order, divides and rotates; writes zeros for empty sequences. A block takes
-// 64 values of NQ query rows: a thread 8 of the values of some rows, first along the rows (as the parts lie), then, through
-// shared memory, along the values (for the rotation).
-constexpr int LJ_THREADS = 128;
+// Adds up the parts of a query block, divides and rotates; writes zeros for empty sequences. A block takes 64 values of 8 query
+// rows: a warp every eighth part (a lane reads the 8 rows' values side by side, a sector), joined in the warps' order.
+constexpr int LJ_WARPS = 8;
 template <int DT, int NQ>
-__global__ void __launch_bounds__(LJ_THREADS) latent_join_kernel(LdArgs g) {
-  constexpr int LANES = NQ / 4, DS = LJ_THREADS / LANES;      // threads along the rows (4 each), values side by side
-  __shared__ float buf[NQ][65];
-  __shared__ float den[NQ];
+__global__ void __launch_bounds__(LJ_WARPS * 32) latent_join_kernel(LdArgs g) {
+  __shared__ float buf[LJ_WARPS][8][65];
+  __shared__ float den[LJ_WARPS][8];
   pdl_wait();
   const vq2_latent_decode_args& a = g.a;
-  const int L = a.latent_dim, rows = a.T * a.heads, tid = threadIdx.x;
-  const int item = blockIdx.x / (L / 64), d0 = blockIdx.x % (L / 64) * 64, b = item / g.nrb, rb = item % g.nrb;
+  const int L = a.latent_dim, rows = a.T * a.heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int r0 = blockIdx.x % (NQ / 8) * 8, d0 = blockIdx.x / (NQ / 8) % (L / 64) * 64, item = blockIdx.x / (NQ / 8) / (L / 64);
+  const int b = item / g.nrb, rb = item % g.nrb;
+  if (rb * NQ + r0 >= rows) return;
   const int total = g.start[a.B], quota = max(1, (total + g.grid - 1) / g.grid);
   const int s0 = g.start[b], tiles = (g.start[b + 1] - s0) / g.nrb;
-  const int begin = s0 + rb * tiles, end = begin + tiles;
-  const int c0 = begin / quota, c1 = tiles ? (end - 1) / quota : c0;
-  const int r4 = tid % LANES * 4, dl = tid / LANES;
-  auto slot = [&](int c) { return (size_t)item + c; };
-  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, l[4] = {};
-  float4 v[64 / DS];
+  const int begin = s0 + rb * tiles, c0 = begin / quota, c1 = tiles ? (begin + tiles - 1) / quota : c0 - 1;
+  float m[8], l[8], v[2][8];
 #pragma unroll
-  for (int k = 0; k < 64 / DS; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (tiles) {
-    for (int c = c0; c <= c1; ++c)
+  for (int i = 0; i < 8; ++i) {
+    m[i] = -INFINITY;
+    l[i] = v[0][i] = v[1][i] = 0.f;
+  }
+  for (int c = c0 + lane; c <= c1; c += 32)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) m[i] = fmaxf(m[i], g.ml[slot(c) * NQ + r4 + i].x);
+    for (int i = 0; i < 8; ++i) m[i] = fmaxf(m[i], g.ml[(size_t)(item + c) * NQ + r0 + i].x);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m[i] = warp_max(m[i]);
 #pragma unroll 2
-    for (int c = c0; c <= c1; ++c) {
-      const float4* p = (const float4*)(g.part + (slot(c) * L + d0 + dl) * NQ + r4);
-      float4 x[64 / DS];
+  for (int c = c0 + warp; c <= c1; c += LJ_WARPS) {
+    const size_t at = (size_t)(item + c);
+    float x[2][8];
 #pragma unroll
-      for (int k = 0; k < 64 / DS; ++k) x[k] = __ldg(p + (size_t)k * DS * (NQ / 4));
-      float f[4];
+    for (int k = 0; k < 2; ++k) {
+      const float4* p = (const float4*)(g.part + (at * L + d0 + lane + 32 * k) * NQ + r0);
+      const float4 y = __ldg(p), z = __ldg(p + 1);
+      x[k][0] = y.x; x[k][1] = y.y; x[k][2] = y.z; x[k][3] = y.w;
+      x[k][4] = z.x; x[k][5] = z.y; x[k][6] = z.z; x[k][7] = z.w;
+    }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 ml = g.ml[slot(c) * NQ + r4 + i];
-        f[i] = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - m[i]);
-        l[i] += ml.y * f[i];
-      }
-#pragma unroll
-      for (int k = 0; k < 64 / DS; ++k) {
-        v[k].x = fmaf(f[0], x[k].x, v[k].x);
-        v[k].y = fmaf(f[1], x[k].y, v[k].y);
-        v[k].z = fmaf(f[2], x[k].z, v[k].z);
-        v[k].w = fmaf(f[3], x[k].w, v[k].w);
-      }
+    for (int i = 0; i < 8; ++i) {
+      const float2 ml = __ldg(g.ml + at * NQ + r0 + i);
+      const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - m[i]);
+      l[i] += ml.y * f;
+      v[0][i] = fmaf(f, x[0][i], v[0][i]);
+      v[1][i] = fmaf(f, x[1][i], v[1][i]);
     }
   }
 #pragma unroll
-  for (int k = 0; k < 64 / DS; ++k) {
-    buf[r4][dl + k * DS] = v[k].x;
-    buf[r4 + 1][dl + k * DS] = v[k].y;
-    buf[r4 + 2][dl + k * DS] = v[k].z;
-    buf[r4 + 3][dl + k * DS] = v[k].w;
+  for (int i = 0; i < 8; ++i) {
+    buf[warp][i][lane] = v[0][i];
+    buf[warp][i][lane + 32] = v[1][i];
+    if (lane == 0) den[warp][i] = l[i];
   }
-  if (dl == 0)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) den[r4 + i] = l[i];
   __syncthreads();
-  for (int u = tid; u < NQ * 8; u += LJ_THREADS) {
-    const int r = u >> 3, row = rb * NQ + r;
-    const float q = den[r], inv = q != 0.f ? 1.f / q : 0.f;
-    float o[8];
+  if (tid >= 64) return;
+  const int r = tid >> 3, d = (tid & 7) * 8, row = rb * NQ + r0 + r;
+  float q = 0.f, o[8] = {};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = q != 0.f ? buf[r][(u & 7) * 8 + i] * inv : 0.f;
-    fwht64_lanes8(o);
-    if (row < rows) store8<DT>(a.out, ((size_t)b * rows + row) * L + d0 + (u & 7) * 8, o);
+  for (int w = 0; w < LJ_WARPS; ++w) {
+    q += den[w][r];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] += buf[w][r][d + i];
   }
+  const float inv = q != 0.f ? 1.f / q : 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = q != 0.f ? o[i] * inv : 0.f;
+  fwht64_lanes8(o);
+  if (row < rows) store8<DT>(a.out, ((size_t)b * rows + row) * L + d0 + d, o);
 }
 
 static int ld_nq(int T, int heads) {
@@ -800,8 +799,8 @@ static int ld_launch(const LdArgs& g, cudaStream_t st) {
   cfg.blockDim = dim3(LD_THREADS);
   cfg.dynamicSmemBytes = ld_smem<NQ>();
   if (cudaLaunchKernelEx(&cfg, kernel, g) != cudaSuccess) return VQ2_ERR_CUDA;
-  cfg.gridDim = dim3((unsigned)(items * (g.a.latent_dim / 64)));
-  cfg.blockDim = dim3(LJ_THREADS);
+  cfg.gridDim = dim3((unsigned)(items * (g.a.latent_dim / 64) * (NQ / 8)));
+  cfg.blockDim = dim3(LJ_WARPS * 32);
   cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, latent_join_kernel<DT, NQ>, g) == cudaSuccess ? VQ2_OK : VQ2_ERR_CUDA;
 }
@@ -812,7 +811,7 @@ using namespace vq2;
 
 extern "C" size_t vq2_latent_decode_workspace_size(int B, int T, int heads, int latent_dim, int rope_dim) {
   if (B <= 0 || T <= 0 || heads <= 0 || !latent_dims_ok(latent_dim, rope_dim) || (long long)T * heads > 1 << 20 ||
-      (long long)B * ((long long)T * heads + 64) >= 1LL << 28)
+      (long long)B * ((long long)T * heads + 64) >= 1LL << 27)
     return 0;
   const int nq = ld_nq(T, heads);
   return ld_layout(B, nq, (int)(((long long)T * heads + nq - 1) / nq), latent_dim, rope_dim, LD_MAX_GRID).total;
@@ -822,7 +821,7 @@ extern "C" int vq2_latent_decode(const vq2_latent_decode_args* a, void* ws, size
   if (!a || !a->q || !a->cache || !a->block_table || !a->kv_len || !a->out) return VQ2_ERR_NULL;
   if (a->B <= 0 || a->T <= 0 || a->heads <= 0 || a->page_size <= 0 || a->max_pages <= 0 || a->pages <= 0 ||
       !latent_dims_ok(a->latent_dim, a->rope_dim) || !(a->scale > 0.f) || (long long)a->T * a->heads > 1 << 20 ||
-      (long long)a->B * ((long long)a->T * a->heads + 64) >= 1LL << 28)
+      (long long)a->B * ((long long)a->T * a->heads + 64) >= 1LL << 27)
     return VQ2_ERR_SHAPE;
   if (a->dtype != VQ2_DT_BF16 && a->dtype != VQ2_DT_F16) return VQ2_ERR_DTYPE;
   if (((uintptr_t)a->q | (uintptr_t)a->cache | (uintptr_t)a->out) & 15) return VQ2_ERR_ALIGN;
