@@ -784,7 +784,8 @@ constexpr int LD_MAX_GRID = 148;        // workspace is sized without a device; 
 template <int DT, int NQ>
 static int ld_launch(const LdArgs& g, cudaStream_t st) {
   auto kernel = latent_decode_kernel<NQ>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ld_smem<NQ>()) != cudaSuccess) return VQ2_ERR_CUDA;
+  static bool raised[64];
+  if (!smem_limit_once(kernel, ld_smem<NQ>(), raised)) return VQ2_ERR_CUDA;
   const int items = g.a.B * g.nrb;
   latent_query_kernel<DT, NQ><<<items * NQ / LQ_WARPS, LQ_WARPS * 32, 0, st>>>(g);
   if (cudaGetLastError() != cudaSuccess) return VQ2_ERR_CUDA;

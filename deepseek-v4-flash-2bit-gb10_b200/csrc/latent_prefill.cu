@@ -191,7 +191,7 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
   volatile int* abort = &sh->abort;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0 && nsteps > 0 && elect_one()) {
       // ---------------- loader
       for (int t = 0; t < ntile; ++t) {
@@ -308,7 +308,7 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
     }
   } else {
     // ---------------- softmax: thread = query row
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int t = (warp - 4) >> 2, r = (warp & 3) * 32 + lane, i = row0 + t * LP_TILE + r;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * 128;
@@ -448,14 +448,17 @@ extern "C" int vq2_latent_prefill(const vq2_latent_prefill_args* a, void* stream
   if (!rc && any && a->rope_dim) rc = lp_encode(&tr, a->k_rope, a->rope_dim, 1, a->total_k, 0, a->r_stride_t);
   if (rc) return rc;
   const int ku = (a->nope_dim + 63) / 64 + (a->rope_dim ? 1 : 0), vu = (a->v_dim + 63) / 64;
+  auto launch = [&](auto kernel, bool* raised) {
+    if (!smem_limit_once(kernel, LP_SMEM, raised)) return VQ2_ERR_CUDA;
+    kernel<<<(unsigned)blocks, LP_THREADS, LP_SMEM, (cudaStream_t)stream>>>(*a, nqb, tq, tk, tr, tv);
+    return cudaGetLastError() == cudaSuccess ? VQ2_OK : VQ2_ERR_CUDA;
+  };
   auto pick = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    return ku == 1 ? (vu == 1 ? latent_prefill_kernel<DT, 1, 1> : latent_prefill_kernel<DT, 1, 2>)
-         : ku == 2 ? (vu == 1 ? latent_prefill_kernel<DT, 2, 1> : latent_prefill_kernel<DT, 2, 2>)
-                   : (vu == 1 ? latent_prefill_kernel<DT, 3, 1> : latent_prefill_kernel<DT, 3, 2>);
+    static bool raised[6][64];
+    return ku == 1 ? (vu == 1 ? launch(latent_prefill_kernel<DT, 1, 1>, raised[0]) : launch(latent_prefill_kernel<DT, 1, 2>, raised[1]))
+         : ku == 2 ? (vu == 1 ? launch(latent_prefill_kernel<DT, 2, 1>, raised[2]) : launch(latent_prefill_kernel<DT, 2, 2>, raised[3]))
+                   : (vu == 1 ? launch(latent_prefill_kernel<DT, 3, 1>, raised[4]) : launch(latent_prefill_kernel<DT, 3, 2>, raised[5]));
   };
-  auto kernel = a->dtype == VQ2_DT_BF16 ? pick(std::integral_constant<int, VQ2_DT_BF16>()) : pick(std::integral_constant<int, VQ2_DT_F16>());
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)LP_SMEM) != cudaSuccess) return VQ2_ERR_CUDA;
-  kernel<<<(unsigned)blocks, LP_THREADS, LP_SMEM, (cudaStream_t)stream>>>(*a, nqb, tq, tk, tr, tv);
-  return cudaGetLastError() == cudaSuccess ? VQ2_OK : VQ2_ERR_CUDA;
+  return a->dtype == VQ2_DT_BF16 ? pick(std::integral_constant<int, VQ2_DT_BF16>()) : pick(std::integral_constant<int, VQ2_DT_F16>());
 }

@@ -233,6 +233,15 @@ inline int device_sm_count() {
   return counts[dev];
 }
 
+// Raises a kernel's dynamic shared-memory limit, once per kernel and device (`done`: one static array per kernel).
+template <typename K>
+inline bool smem_limit_once(K kernel, size_t bytes, bool* done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  if (!done[dev]) done[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess;
+  return done[dev];
+}
+
 // Packed fp32 multiply of two pairs (Blackwell mul.rn.f32x2: each half rounded on its own).
 __device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
   unsigned long long d, x, y;

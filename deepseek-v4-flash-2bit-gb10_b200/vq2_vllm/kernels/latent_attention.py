@@ -9,6 +9,8 @@ result (``q_c = q_nope @ W_uk[h]^T``, ``o @ W_uv[h]``), and attention reads the 
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import _lib
@@ -21,7 +23,12 @@ MAX_HEAD_DIM = 128
 def _i32(t: torch.Tensor, dim: int, what: str):
     if t.dim() != dim or t.dtype not in _lib.ID:
         raise ValueError(f"vq2 latent attention: {what} must be an int32 tensor of {dim} dimension(s)")
-    return t.to(torch.int32).contiguous()
+    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_size(B: int, T: int, heads: int, L: int, R: int) -> int:
+    return _lib.lib().vq2_latent_decode_workspace_size(B, T, heads, L, R)
 
 
 def latent_attention_decode(q: torch.Tensor, cache: LatentCache, block_table: torch.Tensor, kv_len: torch.Tensor,
@@ -49,17 +56,16 @@ def latent_attention_decode(q: torch.Tensor, cache: LatentCache, block_table: to
     out = torch.empty(B, T, heads, L, dtype=q.dtype, device=q.device)
     if not out.numel():
         return out
-    with torch.cuda.device(dev):
-        q = q.contiguous()
-        if q.data_ptr() % 16:
-            q = q.clone()
-        lib = _lib.lib()
-        stream = _lib.stream_ptr(dev)
-        ws = _lib.workspace(lib.vq2_latent_decode_workspace_size(B, T, heads, L, R), q.device, stream)
+    with _lib.on_device(dev):
+        if q.data_ptr() % 16 or not q.is_contiguous():
+            q = q.clone(memory_format=torch.contiguous_format)
+        lib, stream = _lib.lib(), _lib.raw_stream(dev)
+        ws = _lib.workspace(_workspace_size(B, T, heads, L, R), q.device, stream)
         pages, page_size, _ = cache.data.shape
         a = _lib.Vq2LatentDecodeArgs(B, T, heads, L, R, page_size, block_table.shape[1], _DT[q.dtype], pages, scale, q.data_ptr(),
                                      cache.args.data, block_table.data_ptr(), kv_len.data_ptr(), out.data_ptr())
-        _lib.check(lib.vq2_latent_decode(a, ws.data_ptr(), ws.numel(), stream), "vq2_latent_decode")
+        rc = lib.vq2_latent_decode(a, ws.data_ptr(), ws.numel(), stream)
+    _lib.check(rc, "vq2_latent_decode")
     return out
 
 
@@ -107,13 +113,14 @@ def latent_attention_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_rope: torc
     out = torch.empty(Tq, heads, dv, dtype=q.dtype, device=q.device)
     if not out.numel() or not B:
         return out
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         q, k_nope, v = _heads(q, "q"), _heads(k_nope, "k_nope", Tk, heads), _heads(v, "v", Tk, heads)
         if R:
-            k_rope = _heads(k_rope[:, None, :], "k_rope")[:, 0]
+            k_rope = _heads(k_rope[:, None, :], "k_rope")
         a = _lib.Vq2LatentPrefillArgs(B, heads, dn, R, dv, max_q, _DT[q.dtype], Tq, Tk, scale, q.stride(0), q.stride(1),
                                       k_nope.stride(0), k_nope.stride(1), v.stride(0), v.stride(1), k_rope.stride(0) if R else 0,
                                       q.data_ptr(), k_nope.data_ptr(), k_rope.data_ptr() if R else None, v.data_ptr(),
                                       cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr())
-        _lib.check(_lib.lib().vq2_latent_prefill(a, _lib.stream_ptr(dev)), "vq2_latent_prefill")
+        rc = _lib.lib().vq2_latent_prefill(a, _lib.raw_stream(dev))
+    _lib.check(rc, "vq2_latent_prefill")
     return out

@@ -48,15 +48,15 @@ class LatentCache:
 def _slots(slots: torch.Tensor):
     if slots.dim() != 1 or slots.dtype not in _lib.ID:
         raise ValueError("vq2 latent cache: slots must be int32 or int64 [N]")
-    return slots.contiguous()
+    return slots if slots.is_contiguous() else slots.contiguous()
 
 
 def _rows(x: torch.Tensor):
     """x [N, D] as rows the kernels can load 16 bytes at a time (a copy only where they cannot)."""
-    step = 16 // x.element_size()
-    ok = (x.shape[1] == 0 or x.stride(1) == 1 or x.shape[1] == 1) and x.stride(0) >= x.shape[1] and x.stride(0) % max(step, 8) == 0
-    if not ok or x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
+    if x.data_ptr() % 16 or not x.is_contiguous():        # contiguous rows of a multiple of 8 values always serve
+        s0, s1 = x.stride()
+        if x.data_ptr() % 16 or s1 != 1 or s0 < x.shape[1] or s0 % 8:
+            x = x.clone(memory_format=torch.contiguous_format)
     return x
 
 
@@ -65,7 +65,8 @@ def latent_cache_write(cache: LatentCache, c: torch.Tensor, k_rope: torch.Tensor
     None where rope_dim is 0) into the cache rows ``slots`` [N] (int32 / int64; negative: skipped). A slot
     beyond the cache is skipped and reported by ``vq2_device_status``. Slots in one call must differ."""
     L, R = cache.latent_dim, cache.rope_dim
-    if c.dim() != 2 or c.shape[1] != L or c.dtype not in _lib.DT:
+    dt = _lib.DT.get(c.dtype)
+    if c.dim() != 2 or c.shape[1] != L or dt is None:
         raise ValueError(f"vq2 latent cache: c must be bf16 / fp16 / fp32 [N, {L}]")
     N = c.shape[0]
     if R and (k_rope is None or k_rope.shape != (N, R) or k_rope.dtype != c.dtype):
@@ -75,33 +76,38 @@ def latent_cache_write(cache: LatentCache, c: torch.Tensor, k_rope: torch.Tensor
         raise ValueError("vq2 latent cache: one slot per row expected")
     _lib.require_cuda(cache.data)
     dev = cache.data.get_device()
-    _lib.require_cuda(c, slots, *((k_rope,) if R else ()), device=dev)
+    _lib.require_cuda(c, slots, device=dev)
+    if R:
+        _lib.require_cuda(k_rope, device=dev)
     if not N:
         return
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         c = _rows(c)
-        k_rope = _rows(k_rope) if R else None
-        _lib.check(_lib.lib().vq2_latent_cache_write(cache.args, c.data_ptr(), _lib.ptr(k_rope), _lib.DT[c.dtype], c.stride(0),
-                                                     k_rope.stride(0) if R else 0, slots.data_ptr(), _lib.ID[slots.dtype], N,
-                                                     _lib.stream_ptr(dev)), "vq2_latent_cache_write")
+        if R:
+            k_rope = _rows(k_rope)
+        rc = _lib.lib().vq2_latent_cache_write(cache.args, c.data_ptr(), k_rope.data_ptr() if R else None, dt, c.stride(0),
+                                               k_rope.stride(0) if R else 0, slots.data_ptr(), _lib.ID[slots.dtype], N,
+                                               _lib.raw_stream(dev))
+    _lib.check(rc, "vq2_latent_cache_write")
 
 
 def latent_cache_read(cache: LatentCache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
     """The values that cache rows ``slots`` [N] stand for -> (c [N, latent_dim], k_rope [N, rope_dim]) of
     ``dtype`` (bf16 / fp16 / fp32): what the expanded form projects up for a cached prefix. A negative slot
     gives zeros."""
-    if dtype not in _lib.DT:
+    dt = _lib.DT.get(dtype)
+    if dt is None:
         raise ValueError("vq2 latent cache: dtype must be bf16, fp16 or fp32")
     slots = _slots(slots)
     _lib.require_cuda(cache.data)
     dev = cache.data.get_device()
     _lib.require_cuda(slots, device=dev)
     N = slots.shape[0]
-    c = torch.empty(N, cache.latent_dim, dtype=dtype, device=slots.device)
-    k_rope = torch.empty(N, cache.rope_dim, dtype=dtype, device=slots.device)
+    c = torch.empty((N, cache.latent_dim), dtype=dtype, device=slots.device)
+    k_rope = torch.empty((N, cache.rope_dim), dtype=dtype, device=slots.device)
     if N:
-        with torch.cuda.device(dev):
-            _lib.check(_lib.lib().vq2_latent_cache_read(cache.args, slots.data_ptr(), _lib.ID[slots.dtype], N, c.data_ptr(),
-                                                        k_rope.data_ptr() or None, _lib.DT[dtype], _lib.stream_ptr(dev)),
-                       "vq2_latent_cache_read")
+        with _lib.on_device(dev):
+            rc = _lib.lib().vq2_latent_cache_read(cache.args, slots.data_ptr(), _lib.ID[slots.dtype], N, c.data_ptr(),
+                                                  k_rope.data_ptr() or None, dt, _lib.raw_stream(dev))
+        _lib.check(rc, "vq2_latent_cache_read")
     return c, k_rope
