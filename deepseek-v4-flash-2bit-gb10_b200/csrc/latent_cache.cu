@@ -168,43 +168,91 @@ __global__ void __launch_bounds__(LC_THREADS) latent_write_kernel(const void* __
   }
 }
 
-// The inverse: a thread expands one word to 8 values n s, the group is rotated back, 16 bytes go out.
+// H x for 64 values of one thread as 32 packed pairs (2 i, 2 i + 1), butterflies over strides 1, 2, 4, .. 32 in that order,
+// without the 1/8: the same sums, bit for bit, as fwht64_lanes8 makes.
+__device__ __forceinline__ void fwht64_pairs(float2* p) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) p[i] = make_float2(p[i].x + p[i].y, p[i].x - p[i].y);
+  const float2 minus = make_float2(-1.f, -1.f);
+#pragma unroll
+  for (int len = 1; len < 32; len <<= 1)
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (!(i & len)) {
+        const float2 a = p[i], b = p[i + len];
+        p[i] = fadd2(a, b);
+        p[i + len] = ffma2(b, minus, a);
+      }
+}
+
+// 32 bytes: eight fp32 values, or sixteen of a 16-bit type (whole sectors, so that a thread may write its run alone).
+__device__ __forceinline__ void store_sector(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+               "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+
+// The inverse. A thread expands a whole group (32 bytes of nibbles, one scale) and rotates it in registers, so that no
+// value crosses lanes: with a group over 8 lanes the shuffles alone were half the instructions and the kernel, not memory, the
+// bound (65,536 rows of 512 + 64 values: 44 us against 16 us of memory traffic). R/16 more threads a row (rounded up) copy
+// 16 rotary values each.
 template <int DT>
 __global__ void __launch_bounds__(LC_THREADS) latent_read_kernel(const uint8_t* __restrict__ cache, const void* __restrict__ slots,
                                                                  int slot_dtype, int n, int L, int R, long long capacity,
                                                                  void* __restrict__ c, void* __restrict__ kr) {
-  const int U = L / 8 + (R ? 8 : 0), rb = latent_row_bytes(L, R);
+  const int nl = L / 64, U = nl + (R + 15) / 16, rb = latent_row_bytes(L, R);
   const long long idx = (long long)blockIdx.x * LC_THREADS + threadIdx.x;
   const long long tok = idx / U;
   const int u = (int)(idx - tok * U);
-  const bool in = tok < n;
-  long long slot = -1;
-  if (in) slot = slot_dtype == VQ2_ID_I64 ? ((const long long*)slots)[tok] : ((const int*)slots)[tok];
+  if (tok >= n) return;
+  long long slot = slot_dtype == VQ2_ID_I64 ? ((const long long*)slots)[tok] : ((const int*)slots)[tok];
   if (slot >= capacity) {
     set_status(VQ2_ERR_SHAPE);
     slot = -1;
   }
   const uint8_t* row = cache + (slot < 0 ? 0 : slot) * rb;
-  const bool rope = u >= L / 8;
-  const int part = rope ? u - L / 8 : u;
-  float v[8] = {};
-  if (slot >= 0) {
-    if (!rope) {
-      const uint32_t w = __ldg((const uint32_t*)row + part);
-      const float s = __half2float(__ushort_as_half(__ldg((const uint16_t*)(row + L / 2 + 2 * R) + (part >> 3))));
+  if (u >= nl) {
+    const int d = (u - nl) * 16;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = (float)((int)((w >> (4 * (i >> 1) + 16 * (i & 1))) & 15u) - 8) * s;
-    } else if (part * 8 < R) {
-      load8<VQ2_DT_F16>(row + L / 2, part * 8, v);
+    for (int k = 0; k < 16; k += 8)
+      if (d + k < R) {
+        float v[8] = {};
+        if (slot >= 0) load8<VQ2_DT_F16>(row + L / 2, d + k, v);
+        store8<DT>(kr, (size_t)tok * R + d + k, v);
+      }
+    return;
+  }
+  uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
+  float s = 0.f;
+  if (slot >= 0) {
+    w0 = __ldg((const uint4*)row + 2 * u);
+    w1 = __ldg((const uint4*)row + 2 * u + 1);
+    s = __half2float(__ushort_as_half(__ldg((const uint16_t*)(row + L / 2 + 2 * R) + u))) * 0.125f;
+  }
+  const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+  const float2 s2 = make_float2(s, s), c2 = make_float2(-24.f * s, -24.f * s);
+  float2 p[32];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // nibble u = n + 8 in the top mantissa bits of 16 + u; (16 + u) s/8 - 24 s/8 = n s/8, exact
+      const uint32_t lo = w[i] << (19 - 4 * j) & 0x00780000u, hi = (j ? w[i] >> (4 * j - 3) : w[i] << 3) & 0x00780000u;
+      p[i * 4 + j] = ffma2(make_float2(__uint_as_float(lo | 0x41800000u), __uint_as_float(hi | 0x41800000u)), s2, c2);
+    }
+  fwht64_pairs(p);
+  const size_t at = (size_t)tok * L + u * 64;
+  if (DT == VQ2_DT_F32) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) store_sector((float*)c + at + k * 8, (const uint32_t*)(p + 4 * k));
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = pack2<DT>(p[8 * k + i].x, p[8 * k + i].y);
+      store_sector((uint16_t*)c + at + k * 16, v);
     }
   }
-  float y[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = v[i];
-  fwht64_lanes8(y);
-  if (!in) return;
-  if (!rope) store8<DT>(c, (size_t)tok * L + part * 8, y);
-  else if (part * 8 < R) store8<DT>(kr, (size_t)tok * R + part * 8, v);
 }
 
 static int latent_check(const vq2_latent_cache* k) {
@@ -251,8 +299,8 @@ extern "C" int vq2_latent_cache_read(const vq2_latent_cache* k, const void* slot
   if (n == 0) return VQ2_OK;
   const int L = k->latent_dim, R = k->rope_dim;
   if (!c || !slots || (R && !k_rope)) return VQ2_ERR_NULL;
-  if (((uintptr_t)c | (uintptr_t)(R ? k_rope : nullptr)) & 15) return VQ2_ERR_ALIGN;
-  const long long cap = k->pages * k->page_size, threads = (long long)n * (L / 8 + (R ? 8 : 0));
+  if (((uintptr_t)c & 31) | ((uintptr_t)(R ? k_rope : nullptr) & 15)) return VQ2_ERR_ALIGN;
+  const long long cap = k->pages * k->page_size, threads = (long long)n * (L / 64 + (R + 15) / 16);
   const long long blocks = (threads + LC_THREADS - 1) / LC_THREADS;
   if (blocks > 0x7FFFFFFFLL) return VQ2_ERR_SHAPE;
   auto kernel = dtype == VQ2_DT_BF16 ? latent_read_kernel<VQ2_DT_BF16>

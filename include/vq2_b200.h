@@ -271,7 +271,8 @@ size_t vq2_latent_row_bytes(int latent_dim, int rope_dim);   /* 0 for unsupporte
    occur twice hold either row. */
 int vq2_latent_cache_write(const vq2_latent_cache* cache, const void* c, const void* k_rope, int dtype, long long c_stride,
                            long long rope_stride, const void* slots, int slot_dtype, int n, void* stream);
-/* What slots[i] stand for: c [n][L] and k_rope [n][R] of VQ2_DT_* (zeros for a slot that write skips). */
+/* What slots[i] stand for: c [n][L] (32-byte aligned) and k_rope [n][R] of VQ2_DT_* (zeros for a slot that write
+   skips). */
 int vq2_latent_cache_read(const vq2_latent_cache* cache, const void* slots, int slot_dtype, int n, void* c, void* k_rope,
                           int dtype, void* stream);
 
