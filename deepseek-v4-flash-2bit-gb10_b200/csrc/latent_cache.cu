@@ -168,21 +168,28 @@ __global__ void __launch_bounds__(LC_THREADS) latent_write_kernel(const void* __
   }
 }
 
-// H x for 64 values of one thread as 32 packed pairs (2 i, 2 i + 1), butterflies over strides 1, 2, 4, .. 32 in that order,
-// without the 1/8: the same sums, bit for bit, as fwht64_lanes8 makes.
-__device__ __forceinline__ void fwht64_pairs(float2* p) {
+// H x for a 64-group over two neighbouring lanes, 32 values a lane as 16 packed pairs (2 i, 2 i + 1): butterflies over strides
+// 1, 2, 4, 8, 16 in registers and 32 over the lanes, without the 1/8: the same sums, bit for bit, as fwht64_lanes8 makes.
+__device__ __forceinline__ void fwht64_lanes2(float2* p) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) p[i] = make_float2(p[i].x + p[i].y, p[i].x - p[i].y);
+  for (int i = 0; i < 16; ++i) p[i] = make_float2(p[i].x + p[i].y, p[i].x - p[i].y);
   const float2 minus = make_float2(-1.f, -1.f);
 #pragma unroll
-  for (int len = 1; len < 32; len <<= 1)
+  for (int len = 1; len < 16; len <<= 1)
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < 16; ++i)
       if (!(i & len)) {
         const float2 a = p[i], b = p[i + len];
         p[i] = fadd2(a, b);
         p[i + len] = ffma2(b, minus, a);
       }
+  const float sign = threadIdx.x & 1 ? -1.f : 1.f;           // the high lane: other - own
+  const float2 s2 = make_float2(sign, sign);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float2 o = make_float2(__shfl_xor_sync(0xffffffffu, p[i].x, 1), __shfl_xor_sync(0xffffffffu, p[i].y, 1));
+    p[i] = ffma2(p[i], s2, o);
+  }
 }
 
 // 32 bytes: eight fp32 values, or sixteen of a 16-bit type (whole sectors, so that a thread may write its run alone).
@@ -191,62 +198,60 @@ __device__ __forceinline__ void store_sector(void* p, const uint32_t* v) {
                "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 
-// The inverse. A thread expands a whole group (32 bytes of nibbles, one scale) and rotates it in registers, so that no
-// value crosses lanes: with a group over 8 lanes the shuffles alone were half the instructions and the kernel, not memory, the
-// bound (65,536 rows of 512 + 64 values: 44 us against 16 us of memory traffic). R/16 more threads a row (rounded up) copy
-// 16 rotary values each.
+// The inverse. A thread expands half a group (16 bytes of nibbles) and rotates it with its neighbour's half: one shuffle a value
+// (with a group over 8 lanes it is three, half the instructions), and few enough registers for 1280 threads an SM to cover the
+// two dependent reads. All rows' groups come first, then all rows' rotary parts, so that a warp has one kind of work.
 template <int DT>
-__global__ void __launch_bounds__(LC_THREADS) latent_read_kernel(const uint8_t* __restrict__ cache, const void* __restrict__ slots,
-                                                                 int slot_dtype, int n, int L, int R, long long capacity,
-                                                                 void* __restrict__ c, void* __restrict__ kr) {
-  const int nl = L / 64, U = nl + (R + 15) / 16, rb = latent_row_bytes(L, R);
-  const long long idx = (long long)blockIdx.x * LC_THREADS + threadIdx.x;
-  const long long tok = idx / U;
-  const int u = (int)(idx - tok * U);
-  if (tok >= n) return;
-  long long slot = slot_dtype == VQ2_ID_I64 ? ((const long long*)slots)[tok] : ((const int*)slots)[tok];
+__global__ void __launch_bounds__(LC_THREADS, 5) latent_read_kernel(const uint8_t* __restrict__ cache, const void* __restrict__ slots,
+                                                                    int slot_dtype, uint32_t n, int L, int R, long long capacity,
+                                                                    void* __restrict__ c, void* __restrict__ kr) {
+  const int rb = latent_row_bytes(L, R);
+  const uint32_t halves = L / 32, pieces = R / 8, groups = (n * halves + 31) / 32 * 32;     // whole warps
+  uint32_t idx = blockIdx.x * LC_THREADS + threadIdx.x;
+  const bool rotary = idx >= groups;
+  if (rotary) idx -= groups;
+  const uint32_t per = rotary ? pieces : halves;
+  if (rotary && idx >= n * pieces) return;
+  const uint32_t tok = idx / per, u = idx - tok * per;
+  long long slot = -1;
+  if (tok < n) slot = slot_dtype == VQ2_ID_I64 ? __ldg((const long long*)slots + tok) : __ldg((const int*)slots + tok);
   if (slot >= capacity) {
     set_status(VQ2_ERR_SHAPE);
     slot = -1;
   }
   const uint8_t* row = cache + (slot < 0 ? 0 : slot) * rb;
-  if (u >= nl) {
-    const int d = (u - nl) * 16;
-#pragma unroll
-    for (int k = 0; k < 16; k += 8)
-      if (d + k < R) {
-        float v[8] = {};
-        if (slot >= 0) load8<VQ2_DT_F16>(row + L / 2, d + k, v);
-        store8<DT>(kr, (size_t)tok * R + d + k, v);
-      }
+  if (rotary) {
+    float v[8] = {};
+    if (slot >= 0) load8<VQ2_DT_F16>(row + L / 2, u * 8, v);
+    store8<DT>(kr, (size_t)tok * R + u * 8, v);
     return;
   }
-  uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
+  uint4 q = make_uint4(0, 0, 0, 0);
   float s = 0.f;
   if (slot >= 0) {
-    w0 = __ldg((const uint4*)row + 2 * u);
-    w1 = __ldg((const uint4*)row + 2 * u + 1);
-    s = __half2float(__ushort_as_half(__ldg((const uint16_t*)(row + L / 2 + 2 * R) + u))) * 0.125f;
+    q = __ldg((const uint4*)row + u);
+    s = __half2float(__ushort_as_half(__ldg((const uint16_t*)(row + L / 2 + 2 * R) + (u >> 1)))) * 0.125f;
   }
-  const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
   const float2 s2 = make_float2(s, s), c2 = make_float2(-24.f * s, -24.f * s);
-  float2 p[32];
+  float2 p[16];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       // nibble u = n + 8 in the top mantissa bits of 16 + u; (16 + u) s/8 - 24 s/8 = n s/8, exact
       const uint32_t lo = w[i] << (19 - 4 * j) & 0x00780000u, hi = (j ? w[i] >> (4 * j - 3) : w[i] << 3) & 0x00780000u;
       p[i * 4 + j] = ffma2(make_float2(__uint_as_float(lo | 0x41800000u), __uint_as_float(hi | 0x41800000u)), s2, c2);
     }
-  fwht64_pairs(p);
-  const size_t at = (size_t)tok * L + u * 64;
+  fwht64_lanes2(p);
+  if (tok >= n) return;
+  const size_t at = (size_t)tok * L + u * 32;
   if (DT == VQ2_DT_F32) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) store_sector((float*)c + at + k * 8, (const uint32_t*)(p + 4 * k));
+    for (int k = 0; k < 4; ++k) store_sector((float*)c + at + k * 8, (const uint32_t*)(p + 4 * k));
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 2; ++k) {
       uint32_t v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = pack2<DT>(p[8 * k + i].x, p[8 * k + i].y);
@@ -294,18 +299,17 @@ extern "C" int vq2_latent_cache_write(const vq2_latent_cache* k, const void* c, 
 extern "C" int vq2_latent_cache_read(const vq2_latent_cache* k, const void* slots, int slot_dtype, int n, void* c, void* k_rope,
                                      int dtype, void* stream) {
   if (const int rc = latent_check(k)) return rc;
-  if (n < 0) return VQ2_ERR_SHAPE;
+  if (n < 0 || n >= 1 << 27) return VQ2_ERR_SHAPE;
   if (dtype < 0 || dtype > 2 || slot_dtype < 0 || slot_dtype > 1) return VQ2_ERR_DTYPE;
   if (n == 0) return VQ2_OK;
   const int L = k->latent_dim, R = k->rope_dim;
   if (!c || !slots || (R && !k_rope)) return VQ2_ERR_NULL;
   if (((uintptr_t)c & 31) | ((uintptr_t)(R ? k_rope : nullptr) & 15)) return VQ2_ERR_ALIGN;
-  const long long cap = k->pages * k->page_size, threads = (long long)n * (L / 64 + (R + 15) / 16);
-  const long long blocks = (threads + LC_THREADS - 1) / LC_THREADS;
-  if (blocks > 0x7FFFFFFFLL) return VQ2_ERR_SHAPE;
+  const long long cap = k->pages * k->page_size;
+  const unsigned blocks = ((unsigned)n * (L / 32) + 31 + (unsigned)n * (R / 8) + LC_THREADS - 1) / LC_THREADS;
   auto kernel = dtype == VQ2_DT_BF16 ? latent_read_kernel<VQ2_DT_BF16>
               : dtype == VQ2_DT_F16 ? latent_read_kernel<VQ2_DT_F16> : latent_read_kernel<VQ2_DT_F32>;
-  kernel<<<(unsigned)blocks, LC_THREADS, 0, (cudaStream_t)stream>>>((const uint8_t*)k->data, slots, slot_dtype, n, L, R, cap, c,
+  kernel<<<blocks, LC_THREADS, 0, (cudaStream_t)stream>>>((const uint8_t*)k->data, slots, slot_dtype, (uint32_t)n, L, R, cap, c,
                                                                     k_rope);
   return cudaGetLastError() == cudaSuccess ? VQ2_OK : VQ2_ERR_CUDA;
 }
