@@ -24,31 +24,16 @@
 // path is kept busy: a tile is handed over in parts of 128 latent values, S starts on the first part, and
 // a part is filled again as soon as P V has used it. Up to 32 query rows there is room for two tiles, and the softmax of a
 // tile runs under the products of the next. In the steady state no barrier spans the block.
-#include "vq2_common.cuh"
+#include "latent_decode.cuh"
 
 namespace vq2 {
 
-constexpr int LD_TILE = 64;             // cached rows a tile
 constexpr int LD_WORKERS = 256, LD_WARPS = LD_WORKERS / 32;
 constexpr int LD_THREADS = LD_WORKERS + 128;     // 168 registers each at launch: 256 x 200 + 128 x 104 afterwards
 constexpr int LD_UNIT = LD_TILE * 128;  // bytes of a unit of the tile: 64 rows of 64 fp16 values
 constexpr int LD_UNITS = 9;             // 8 for the latent, 1 for the rotary part (P takes its place once S is done)
 constexpr int LD_KBYTES = LD_UNITS * LD_UNIT;
 constexpr float LD_BIAS = 5.f, LD_RAISE = 10.f;    // P = 2^(z - m + BIAS); m is raised when z exceeds it by RAISE
-
-struct LdArgs {
-  vq2_latent_decode_args a;
-  int rb;               // bytes of a cached row
-  int nrb;              // blocks of NQ query rows a sequence
-  int grid;             // blocks that share the tiles
-  long long capacity;   // cached rows
-  uint32_t page_mul, page_shift;   // j / page_size = (j * mul) >> 32 >> shift (or j >> shift where mul is 0)
-  int* start;           // [B + 1] first position of each sequence
-  float2* ml;           // [parts][NQ] maximum and denominator of a part
-  float* part;          // [parts][L][NQ]; a block's part of query block n is number n + block
-  uint8_t* q;           // [query blocks][units][NQ][128 bytes] rotated query rows, fp16, swizzled
-  float2* meta;         // [query blocks][NQ] factor of a row's logits, and its token (as int bits)
-};
 
 constexpr int LD_PARTS = 4;             // of a tile: two units each, the last with the rotary unit
 // A raw row in shared memory every 448 bytes (at most 400 are used): with 64 modulo 128, the 64-byte pieces that 4 lanes each
@@ -65,7 +50,8 @@ struct LdShared {
   uint64_t qfull, qfree;
   int there[2][LD_TILE];             // whether a raw row was found
   uint32_t tmem;
-  int abort, b0, rb0, tile0;
+  int abort;
+  LdStart start;
   int flag[2][LD_TILE];              // 2 i: the row is not there in tile i; 2 i + 1: it holds a non-finite scale
   float red[4][NQ];
   alignas(16) float2 meta[2][NQ];    // of this query block and the next
@@ -77,15 +63,6 @@ template <int NQ>
 constexpr size_t ld_smem() { return (size_t)LD_TILES<NQ> * LD_KBYTES + (size_t)LD_RAWS<NQ> * LD_RAW + (size_t)LD_UNITS * NQ * 128 + sizeof(LdShared<NQ>) + 1024; }
 static_assert(ld_smem<64>() <= 227 * 1024 && ld_smem<32>() <= 227 * 1024 && ld_smem<16>() <= 227 * 1024, "latent decode shared memory");
 
-// Wait that ends early once any thread of the block has given up; it never leaves the caller's loop,
-// so every thread keeps to the same sequence of block barriers. The block's last lines report the abort.
-__device__ __forceinline__ void ld_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  for (uint32_t i = 1; !mbar_try_wait(bar, parity); ++i)
-    if ((i & 63) == 0 && (*abort || i >= VQ2_WAIT_LIMIT)) {
-      *abort = 1;
-      return;
-    }
-}
 __device__ __forceinline__ void ld_sync_workers() { asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ void ld_sync_group(int g) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(2 + g) : "memory"); }
 __device__ __forceinline__ bool ld_any_group(int g, bool p) {
@@ -105,25 +82,6 @@ __device__ __forceinline__ void store32(float* p, const float* v) {
   asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
                "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
 }
-
-// Position of a tile: sequence, block of query rows, tile; the order is sequence, block, tile.
-struct LdPos {
-  int b, rb, tile, len, tiles;
-  __device__ __forceinline__ void at(const LdArgs& g, int sequence) {
-    b = sequence;
-    const int most = (int)min((long long)g.a.max_pages * g.a.page_size, 0x7FFFFF00LL);
-    len = b < g.a.B ? min(max(g.a.kv_len[b], 0), most) : 0;
-    tiles = (len + LD_TILE - 1) / LD_TILE;
-  }
-  __device__ __forceinline__ void next(const LdArgs& g) {
-    if (++tile < tiles) return;
-    tile = 0;
-    if (++rb < g.nrb) return;
-    rb = 0;
-    do at(g, b + 1);
-    while (tiles == 0 && b < g.a.B);
-  }
-};
 
 // D += A B with both descriptors at constant offsets from their bases (added in place: otherwise
 // the compiler keeps a register for each of the unrolled products).
@@ -156,45 +114,6 @@ __device__ __forceinline__ void ld_value_block(uint32_t d, uint32_t v, uint32_t 
   constexpr uint32_t p_hi = (uint32_t)(16 * NQ >> 4) | 1u << 14 | (NQ == 64 ? 2u : NQ == 32 ? 4u : 6u) << 29;
   umma_at<M * (2 * LD_UNIT >> 4) + KS * 128, KS * (2 * NQ), p_hi, id>(d + M * NQ, v, p, KS > 0 ? 1 : acc);
   if constexpr (KS + 1 < LD_TILE / 16) ld_value_block<NQ, M, KS + 1>(d, v, p, acc);
-}
-
-// Query rows -> the layout of Q's tile, one warp a row: latent part rotated, all scaled into fp16's range by a power of two.
-constexpr int LQ_WARPS = 4;
-template <int DT, int NQ>
-__global__ void __launch_bounds__(LQ_WARPS * 32) latent_query_kernel(LdArgs g) {
-  pdl_launch_dependents();
-  const vq2_latent_decode_args& a = g.a;
-  const int lane = threadIdx.x & 31, L = a.latent_dim, R = a.rope_dim, nl = L / 64, units = nl + (R ? 1 : 0), rows = a.T * a.heads;
-  const int at = blockIdx.x * LQ_WARPS + (threadIdx.x >> 5), item = at / NQ, r = at % NQ;          // query block, row in it
-  const int b = item / g.nrb, row = item % g.nrb * NQ + r;
-  const size_t q0 = ((size_t)b * rows + row) * (L + R);
-  float v[3][8], m = 0.f;
-#pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    const int u = k < 2 ? lane + 32 * k : lane;          // 8-value unit: of the latent part, of the rotary part
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[k][i] = 0.f;
-    if (row < rows && u * 8 < (k < 2 ? L : R)) load8<DT>(a.q, q0 + (k < 2 ? 0 : L) + u * 8, v[k]);
-  }
-#pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    if (k < 2) fwht64_lanes8(v[k]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[k][i]));
-  }
-  const float2 f = f16_range_scale(fminf(warp_max(m), 3.0e38f));
-  uint8_t* dst = g.q + (size_t)item * units * (NQ * 128) + r * 128;
-#pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    const int u = k < 2 ? lane + 32 * k : lane, unit = k < 2 ? u >> 3 : nl, c = u & 7;
-    if (k < 2 ? u * 8 < L : R && u < 8)
-      *(uint4*)(dst + (size_t)unit * (NQ * 128) + ((c ^ (r & 7)) << 4)) =
-          make_uint4(pack2<VQ2_DT_F16>(v[k][0] * f.x, v[k][1] * f.x), pack2<VQ2_DT_F16>(v[k][2] * f.x, v[k][3] * f.x),
-                     pack2<VQ2_DT_F16>(v[k][4] * f.x, v[k][5] * f.x), pack2<VQ2_DT_F16>(v[k][6] * f.x, v[k][7] * f.x));
-  }
-  // a row that pads the block sees nothing
-  if (lane == 0)
-    g.meta[at] = make_float2(a.scale * 1.4426950408889634f * f.y, __int_as_float(row < rows ? row / a.heads : -(1 << 30)));
 }
 
 template <int NQ>
@@ -235,51 +154,7 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
   }
   if (tid < 2 * LD_TILE) sh->flag[tid >> 6][tid & 63] = -1;
 
-  // ---------------- this block's share of the tiles. Each worker sums a run of sequences, a scan gives
-  // the runs' first positions, and the worker whose run holds the block's first tile walks to it.
-  const int B = a.B, run = (B + LD_WORKERS - 1) / LD_WORKERS;
-  const int r0 = min(B, tid * run), r1 = tid < LD_WORKERS ? min(B, r0 + run) : r0;
-  LdPos pos;
-  int mine = 0;
-  for (int b = r0; b < r1; ++b) {
-    pos.at(g, b);
-    mine += pos.tiles * g.nrb;
-  }
-  int inc = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += v;
-  }
-  if (lane == 31 && warp < LD_WARPS) sh->scan[warp] = inc;
-  __syncthreads();
-  int before = inc - mine, total = 0;
-  for (int w = 0; w < LD_WARPS; ++w) {
-    if (w < warp) before += sh->scan[w];
-    total += sh->scan[w];
-  }
-  const int quota = max(1, (total + g.grid - 1) / g.grid);
-  const int begin = (int)min((long long)blockIdx.x * quota, (long long)total), count = min(quota, total - begin);
-  if (blockIdx.x == 0) {
-    int p = before;
-    for (int b = r0; b < r1; ++b) {
-      g.start[b] = p;
-      pos.at(g, b);
-      p += pos.tiles * g.nrb;
-    }
-    if (tid == 0) g.start[B] = total;
-  }
-  if (count > 0 && begin >= before && begin < before + mine) {
-    int p = before, b = r0;
-    for (;; ++b) {
-      pos.at(g, b);
-      if (begin < p + pos.tiles * g.nrb) break;
-      p += pos.tiles * g.nrb;
-    }
-    sh->b0 = b;
-    sh->rb0 = (begin - p) / pos.tiles;
-    sh->tile0 = (begin - p) % pos.tiles;
-  }
+  const int count = ld_share<LD_WARPS>(g, sh->scan, &sh->start);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -290,10 +165,7 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == LD_WARPS && count > 0 && elect_one()) {
       // ---------------- products
-      LdPos p;
-      p.at(g, sh->b0);
-      p.rb = sh->rb0;
-      p.tile = sh->tile0;
+      LdPos p = sh->start.position(g);
       bool opens = true;             // the tile whose P V comes next is the first of its query block
       auto values = [&](int i) {     // O^T += V^T P^T of tile i, a block of 128 values after another
         const int b = i % TILES;
@@ -369,20 +241,9 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
       ld_wait(&sh->drain, 0, abort);
     } else if (warp == LD_WARPS + 1 && count > 0) {
       // ---------------- loader: the whole warp, two rows a lane. Page numbers are read a tile ahead.
-      LdPos p;
-      p.at(g, sh->b0);
-      p.rb = sh->rb0;
-      p.tile = sh->tile0;
-      int j[2], page_at[2], page[2];
-      auto find = [&]() {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          j[k] = p.tile * LD_TILE + lane + 32 * k;
-          page_at[k] = (int)(g.page_mul ? __umulhi((uint32_t)j[k], g.page_mul) >> g.page_shift : (uint32_t)j[k] >> g.page_shift);
-          page[k] = j[k] < p.len ? __ldg(a.block_table + (size_t)p.b * a.max_pages + page_at[k]) : -1;
-        }
-      };
-      find();
+      LdPos p = sh->start.position(g);
+      LdRows rows;
+      rows.find(g, p);
       int seg = -1;
       for (int i = 0; i < count; ++i) {
         const int st = i % RAWS;
@@ -397,22 +258,15 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
             bulk_g2s(sh->meta[seg & 1], g.meta + (size_t)item * NQ, NQ * 8, &sh->qfull);
           }
         }
-        long long off[2];
-        int rows = 0;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const bool in = page[k] >= 0 && page[k] < a.pages;
-          if (!in && j[k] < p.len) set_status(VQ2_ERR_SHAPE);
-          off[k] = in ? ((long long)page[k] * a.page_size + (j[k] - page_at[k] * a.page_size)) * g.rb : -1;
-          rows += __popc(__ballot_sync(0xffffffffu, in));
-        }
+        const long long off[2] = {rows.offset(g, p, 0), rows.offset(g, p, 1)};
+        const int found = __popc(__ballot_sync(0xffffffffu, off[0] >= 0)) + __popc(__ballot_sync(0xffffffffu, off[1] >= 0));
         p.next(g);
-        if (i + 1 < count) find();
+        if (i + 1 < count) rows.find(g, p);
         ld_wait(&sh->rfree[st], ((i / RAWS) & 1) ^ 1, abort);
 #pragma unroll
         for (int k = 0; k < 2; ++k) sh->there[st][lane + 32 * k] = off[k] >= 0;
         __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(&sh->rfull[st], rows * g.rb);
+        if (lane == 0) mbar_arrive_expect_tx(&sh->rfull[st], found * g.rb);
         __syncwarp();
 #pragma unroll
         for (int k = 0; k < 2; ++k)
@@ -640,11 +494,7 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
       };
 
       // Tiles are expanded up to TILES ahead of the softmax, but not past the end of a query block (pe, ps: the next of each).
-      LdPos pe, ps;
-      pe.at(g, sh->b0);
-      pe.rb = sh->rb0;
-      pe.tile = sh->tile0;
-      ps = pe;
+      LdPos pe = sh->start.position(g), ps = pe;
       int ie = 0, is = 0, seg = -1;
       read_raw(0);
       while (is < count) {
@@ -684,76 +534,6 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
   if (warp == LD_WARPS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS));
 }
 
-// Adds up the parts of a query block, divides and rotates; writes zeros for empty sequences. A block takes 64 values of 8 query
-// rows: a warp every eighth part (a lane reads the 8 rows' values side by side, a sector), joined in the warps' order.
-constexpr int LJ_WARPS = 8;
-template <int DT, int NQ>
-__global__ void __launch_bounds__(LJ_WARPS * 32) latent_join_kernel(LdArgs g) {
-  __shared__ float buf[LJ_WARPS][8][65];
-  __shared__ float den[LJ_WARPS][8];
-  pdl_wait();
-  const vq2_latent_decode_args& a = g.a;
-  const int L = a.latent_dim, rows = a.T * a.heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int r0 = blockIdx.x % (NQ / 8) * 8, d0 = blockIdx.x / (NQ / 8) % (L / 64) * 64, item = blockIdx.x / (NQ / 8) / (L / 64);
-  const int b = item / g.nrb, rb = item % g.nrb;
-  if (rb * NQ + r0 >= rows) return;
-  const int total = g.start[a.B], quota = max(1, (total + g.grid - 1) / g.grid);
-  const int s0 = g.start[b], tiles = (g.start[b + 1] - s0) / g.nrb;
-  const int begin = s0 + rb * tiles, c0 = begin / quota, c1 = tiles ? (begin + tiles - 1) / quota : c0 - 1;
-  float m[8], l[8], v[2][8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    m[i] = -INFINITY;
-    l[i] = v[0][i] = v[1][i] = 0.f;
-  }
-  for (int c = c0 + lane; c <= c1; c += 32)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m[i] = fmaxf(m[i], g.ml[(size_t)(item + c) * NQ + r0 + i].x);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m[i] = warp_max(m[i]);
-#pragma unroll 2
-  for (int c = c0 + warp; c <= c1; c += LJ_WARPS) {
-    const size_t at = (size_t)(item + c);
-    float x[2][8];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float4* p = (const float4*)(g.part + (at * L + d0 + lane + 32 * k) * NQ + r0);
-      const float4 y = __ldg(p), z = __ldg(p + 1);
-      x[k][0] = y.x; x[k][1] = y.y; x[k][2] = y.z; x[k][3] = y.w;
-      x[k][4] = z.x; x[k][5] = z.y; x[k][6] = z.z; x[k][7] = z.w;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 ml = __ldg(g.ml + at * NQ + r0 + i);
-      const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - m[i]);
-      l[i] += ml.y * f;
-      v[0][i] = fmaf(f, x[0][i], v[0][i]);
-      v[1][i] = fmaf(f, x[1][i], v[1][i]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    buf[warp][i][lane] = v[0][i];
-    buf[warp][i][lane + 32] = v[1][i];
-    if (lane == 0) den[warp][i] = l[i];
-  }
-  __syncthreads();
-  if (tid >= 64) return;
-  const int r = tid >> 3, d = (tid & 7) * 8, row = rb * NQ + r0 + r;
-  float q = 0.f, o[8] = {};
-#pragma unroll
-  for (int w = 0; w < LJ_WARPS; ++w) {
-    q += den[w][r];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] += buf[w][r][d + i];
-  }
-  const float inv = q != 0.f ? 1.f / q : 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = q != 0.f ? o[i] * inv : 0.f;
-  fwht64_lanes8(o);
-  if (row < rows) store8<DT>(a.out, ((size_t)b * rows + row) * L + d0 + d, o);
-}
-
 static int ld_nq(int T, int heads) {
   const long long rows = (long long)T * heads;
   return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
@@ -781,13 +561,23 @@ static LdLayout ld_layout(int B, int nq, int nrb, int L, int R, int grid) {
 }
 constexpr int LD_MAX_GRID = 148;        // workspace is sized without a device; a B200 has 148 SMs
 
-template <int DT, int NQ>
+// Three launches: query rows, the main kernel (NQ rows a block; NARROW: the one for 16), the join; the later two by programmatic
+// dependent launch.
+template <int DT, int NQ, bool NARROW>
 static int ld_launch(const LdArgs& g, cudaStream_t st) {
-  auto kernel = latent_decode_kernel<NQ>;
+  void (*kernel)(LdArgs);
+  size_t smem;
+  if constexpr (NARROW) {
+    kernel = latent_decode_narrow_kernel;
+    smem = LN_SMEM;
+  } else {
+    kernel = latent_decode_kernel<NQ>;
+    smem = ld_smem<NQ>();
+  }
   static bool raised[64];
-  if (!smem_limit_once(kernel, ld_smem<NQ>(), raised)) return VQ2_ERR_CUDA;
+  if (!smem_limit_once(kernel, smem, raised)) return VQ2_ERR_CUDA;
   const int items = g.a.B * g.nrb;
-  latent_query_kernel<DT, NQ><<<items * NQ / LQ_WARPS, LQ_WARPS * 32, 0, st>>>(g);
+  latent_query_kernel<DT, NQ, NARROW><<<items * NQ / LQ_WARPS, LQ_WARPS * 32, 0, st>>>(g);
   if (cudaGetLastError() != cudaSuccess) return VQ2_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.stream = st;
@@ -797,8 +587,8 @@ static int ld_launch(const LdArgs& g, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   cfg.gridDim = dim3(g.grid);
-  cfg.blockDim = dim3(LD_THREADS);
-  cfg.dynamicSmemBytes = ld_smem<NQ>();
+  cfg.blockDim = dim3(NARROW ? LN_THREADS : LD_THREADS);
+  cfg.dynamicSmemBytes = smem;
   if (cudaLaunchKernelEx(&cfg, kernel, g) != cudaSuccess) return VQ2_ERR_CUDA;
   cfg.gridDim = dim3((unsigned)(items * (g.a.latent_dim / 64) * (NQ / 8)));
   cfg.blockDim = dim3(LJ_WARPS * 32);
@@ -824,6 +614,9 @@ extern "C" int vq2_latent_decode(const vq2_latent_decode_args* a, void* ws, size
       !latent_dims_ok(a->latent_dim, a->rope_dim) || !(a->scale > 0.f) || (long long)a->T * a->heads > 1 << 20 ||
       (long long)a->B * ((long long)a->T * a->heads + 64) >= 1LL << 27)
     return VQ2_ERR_SHAPE;
+  // positions (tiles of all query blocks in order) are 32-bit numbers
+  if ((double)a->B * (((double)a->max_pages * a->page_size + LD_TILE - 1) / LD_TILE) * ((double)a->T * a->heads / 16 + 1) >= 2147483648.)
+    return VQ2_ERR_SHAPE;
   if (a->dtype != VQ2_DT_BF16 && a->dtype != VQ2_DT_F16) return VQ2_ERR_DTYPE;
   if (((uintptr_t)a->q | (uintptr_t)a->cache | (uintptr_t)a->out) & 15) return VQ2_ERR_ALIGN;
   if (!ws || ws_bytes < vq2_latent_decode_workspace_size(a->B, a->T, a->heads, a->latent_dim, a->rope_dim))
@@ -835,7 +628,6 @@ extern "C" int vq2_latent_decode(const vq2_latent_decode_args* a, void* ws, size
   g.rb = latent_row_bytes(a->latent_dim, a->rope_dim);
   g.nrb = (a->T * a->heads + nq - 1) / nq;
   g.grid = min(sms, LD_MAX_GRID);
-  g.capacity = a->pages * a->page_size;
   // j / page_size for 0 <= j < 2^31: a shift, or with s = ceil(log2 page_size) the high half of j * ceil(2^(31+s) / page_size)
   int s = 0;
   while ((1LL << s) < a->page_size) ++s;
@@ -855,7 +647,7 @@ extern "C" int vq2_latent_decode(const vq2_latent_decode_args* a, void* ws, size
   g.meta = (float2*)(base + w.meta);
   cudaStream_t st = (cudaStream_t)stream;
   const bool bf = a->dtype == VQ2_DT_BF16;
-  if (nq == 16) return bf ? ld_launch<VQ2_DT_BF16, 16>(g, st) : ld_launch<VQ2_DT_F16, 16>(g, st);
-  if (nq == 32) return bf ? ld_launch<VQ2_DT_BF16, 32>(g, st) : ld_launch<VQ2_DT_F16, 32>(g, st);
-  return bf ? ld_launch<VQ2_DT_BF16, 64>(g, st) : ld_launch<VQ2_DT_F16, 64>(g, st);
+  if (nq == 16) return bf ? ld_launch<VQ2_DT_BF16, 16, true>(g, st) : ld_launch<VQ2_DT_F16, 16, true>(g, st);
+  if (nq == 32) return bf ? ld_launch<VQ2_DT_BF16, 32, false>(g, st) : ld_launch<VQ2_DT_F16, 32, false>(g, st);
+  return bf ? ld_launch<VQ2_DT_BF16, 64, false>(g, st) : ld_launch<VQ2_DT_F16, 64, false>(g, st);
 }

@@ -10,4 +10,5 @@
 #include "shared.cu"
 #include "latent_cache.cu"
 #include "latent_prefill.cu"
+#include "latent_decode_narrow.cu"
 #include "latent_decode.cu"
