@@ -568,14 +568,17 @@ static int ld_launch(const LdArgs& g, cudaStream_t st) {
   void (*kernel)(LdArgs);
   size_t smem;
   if constexpr (NARROW) {
-    kernel = latent_decode_narrow_kernel;
+    static void (*const by_groups[8])(LdArgs) = {latent_decode_narrow_kernel<1>, latent_decode_narrow_kernel<2>, latent_decode_narrow_kernel<3>,
+                                                 latent_decode_narrow_kernel<4>, latent_decode_narrow_kernel<5>, latent_decode_narrow_kernel<6>,
+                                                 latent_decode_narrow_kernel<7>, latent_decode_narrow_kernel<8>};
+    kernel = by_groups[g.a.latent_dim / 64 - 1];
     smem = LN_SMEM;
   } else {
     kernel = latent_decode_kernel<NQ>;
     smem = ld_smem<NQ>();
   }
-  static bool raised[64];
-  if (!smem_limit_once(kernel, smem, raised)) return VQ2_ERR_CUDA;
+  static bool raised[8][64];
+  if (!smem_limit_once(kernel, smem, raised[NARROW ? g.a.latent_dim / 64 - 1 : 0])) return VQ2_ERR_CUDA;
   const int items = g.a.B * g.nrb;
   latent_query_kernel<DT, NQ, NARROW><<<items * NQ / LQ_WARPS, LQ_WARPS * 32, 0, st>>>(g);
   if (cudaGetLastError() != cudaSuccess) return VQ2_ERR_CUDA;

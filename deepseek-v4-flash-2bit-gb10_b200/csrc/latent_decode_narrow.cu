@@ -37,7 +37,7 @@ constexpr size_t LN_SMEM = (size_t)LN_STAGES * LN_STAGE + sizeof(LnShared) + 128
 __host__ __device__ __forceinline__ int ln_pitch(int rb) { return (rb / 16 | 1) * 16; }
 
 __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // Nibbles J of both halves of w, as n s in fp16: nibble u = n + 8 in the top mantissa bits of 16 + u; (16 + u) s - 24 s, exact.
@@ -55,13 +55,15 @@ __device__ __forceinline__ bool ln_any(bool p) {
 }
 __device__ __forceinline__ void ln_sync() { asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }
 
+// NL: groups of 64 latent values, known at compile time so that a tile's work is three straight runs of instructions.
+template <int NL>
 __global__ void __launch_bounds__(LN_THREADS, 1) latent_decode_narrow_kernel(LdArgs g) {
   extern __shared__ __align__(128) uint8_t ln_smem[];
-  const uint32_t raw = smem_u32(ln_smem);
   LnShared* sh = (LnShared*)(ln_smem + LN_STAGES * LN_STAGE);
   const vq2_latent_decode_args& a = g.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  const int L = a.latent_dim, R = a.rope_dim, nl = L / 64, pitch = ln_pitch(g.rb), units = nl + (R ? 1 : 0);
+  constexpr int L = NL * 64;
+  const int R = a.rope_dim, pitch = ln_pitch(g.rb), units = NL + (R ? 1 : 0);
   volatile int* abort = &sh->abort;
   pdl_launch_dependents();
   if (tid == 0) {
@@ -115,7 +117,7 @@ __global__ void __launch_bounds__(LN_THREADS, 1) latent_decode_narrow_kernel(LdA
     if (count > 0) {
       const int gr = lane >> 2, t = lane & 3;       // fragment row (query rows gr, gr + 8; S's cached row; O's column) and quarter
       LdPos p = sh->start.position(g);
-      uint4 q[18][2];                               // query rows gr and gr + 8: 16 pieces of 32 latent values, 2 of rotary ones
+      uint4 q[2 * NL + 2][2];                       // query rows gr and gr + 8: pieces of 32 latent values, then 2 of rotary ones
       float o[8][4], l[2], ref[2], fac[2];
       int tok[2];
       bool fresh = true;                            // the query kernel's results not yet waited for
@@ -129,10 +131,7 @@ __global__ void __launch_bounds__(LN_THREADS, 1) latent_decode_narrow_kernel(LdA
             const int row = item * LN_ROWS + gr + 8 * k;
             const uint4* src = (const uint4*)(g.q + (size_t)row * units * 128) + t;
 #pragma unroll
-            for (int n = 0; n < 18; ++n) {
-              const bool has = n < 16 ? n < 2 * nl : (n - 16) * 32 < R;
-              q[n][k] = has ? src[(n < 16 ? n : 2 * nl + n - 16) * 4] : make_uint4(0, 0, 0, 0);
-            }
+            for (int n = 0; n < 2 * NL + 2; ++n) q[n][k] = n < 2 * NL || (n - 2 * NL) * 32 < R ? src[n * 4] : make_uint4(0, 0, 0, 0);
             const float2 m = g.meta[row];
             fac[k] = m.x;
             tok[k] = __float_as_int(m.y);
@@ -143,34 +142,46 @@ __global__ void __launch_bounds__(LN_THREADS, 1) latent_decode_narrow_kernel(LdA
           for (int v = 0; v < 8; ++v) o[v][0] = o[v][1] = o[v][2] = o[v][3] = 0.f;
         }
         ld_wait(&sh->rfull[st], (i / LN_STAGES) & 1, abort);
-        const uint32_t tile = raw + st * LN_STAGE;
+        uint8_t* tile = ln_smem + st * LN_STAGE;
         // ---------------- S: cached row 8 warp + gr against the 16 query rows
         float z[4];
         {
-          const uint32_t row = tile + (warp * 8 + gr) * pitch;
-          const uint4 sc = lds128_v(row + L / 2 + 2 * R);
+          uint8_t* row = tile + (warp * 8 + gr) * pitch;
+          uint4* scales = (uint4*)(row + L / 2 + 2 * R);
+          const uint4 sc = *scales;
           const uint32_t scale[4] = {sc.x, sc.y, sc.z, sc.w};
           float acc[4][4] = {};
 #pragma unroll
-          for (int n = 0; n < 16; ++n) {
-            if (n >= 2 * nl) break;
+          for (int n = 0; n < 2 * NL; ++n) {
             const uint32_t s = __byte_perm(scale[n >> 2], 0, (n >> 1) & 1 ? 0x3232 : 0x1010);
             const __half2 s2 = *(const __half2*)&s, c2 = __hmul2(s2, __float2half2_rn(-24.f));
-            const uint32_t w = lds32_v(row + (4 * n + t) * 4);
+            const uint32_t w = *(const uint32_t*)(row + (4 * n + t) * 4);
             mma16816(acc[2 * (n & 1)], q[n][0].x, q[n][1].x, q[n][0].y, q[n][1].y, ln_pair<0>(w, s2, c2), ln_pair<1>(w, s2, c2));
             mma16816(acc[2 * (n & 1) + 1], q[n][0].z, q[n][1].z, q[n][0].w, q[n][1].w, ln_pair<2>(w, s2, c2), ln_pair<3>(w, s2, c2));
           }
+          if (R) {
 #pragma unroll
-          for (int n = 16; n < 18; ++n) {
-            const int d = (n - 16) * 32 + 8 * t;
-            if ((n - 16) * 32 >= R) break;
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (d < R) w = lds128_v(row + L / 2 + 2 * d);
-            mma16816(acc[2 * (n & 1)], q[n][0].x, q[n][1].x, q[n][0].y, q[n][1].y, w.x, w.y);
-            mma16816(acc[2 * (n & 1) + 1], q[n][0].z, q[n][1].z, q[n][0].w, q[n][1].w, w.z, w.w);
+            for (int k = 0; k < 2; ++k) {
+              const int d = k * 32 + 8 * t, n = 2 * NL + k;
+              uint4 w = make_uint4(0, 0, 0, 0);
+              if (d < R) w = *(const uint4*)(row + L / 2 + 2 * d);
+              mma16816(acc[2 * k], q[n][0].x, q[n][1].x, q[n][0].y, q[n][1].y, w.x, w.y);
+              mma16816(acc[2 * k + 1], q[n][0].z, q[n][1].z, q[n][0].w, q[n][1].w, w.z, w.w);
+            }
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) z[k] = ((acc[0][k] + acc[1][k]) + (acc[2][k] + acc[3][k])) * fac[k >> 1];
+          // A non-finite scale has made the logits NaN for those who see the row; its values must not reach the others.
+          // (An exponent of all ones carries into the top bit when one is added to it.)
+          uint32_t bad = 0;
+#pragma unroll
+          for (int k = 0; k < (NL + 1) / 2; ++k) bad |= ((scale[k] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+          if (__any_sync(0xffffffffu, bad)) {      // (the vote: a row's four lanes have all read its scales)
+            uint16_t* h = (uint16_t*)scales;
+            for (int k = 0; k < 8; ++k)
+              if ((h[k] & 0x7C00u) == 0x7C00u) h[k] = 0;
+            fence_async_smem();          // before a later tile's copy to the same place
+          }
         }
         // ---------------- softmax: query row gr (z[0], z[1]) and gr + 8 (z[2], z[3]), cached rows 8 warp + 2 t and + 1
         const uint32_t there = sh->there[st][warp >> 2] >> ((warp & 3) * 8 + 2 * t);
@@ -181,15 +192,14 @@ __global__ void __launch_bounds__(LN_THREADS, 1) latent_decode_narrow_kernel(LdA
           if (!((there >> (k & 1)) & 1) || j > p.len - a.T + tok[k >> 1]) z[k] = -INFINITY;
           raise |= z[k] > ref[k >> 1] + LN_RAISE;
         }
-        const uint32_t pb = smem_u32(sh->p[i & 1]);
+        uint8_t* pb = sh->p[i & 1];
         float pr[4];
         auto probabilities = [&]() {
 #pragma unroll
           for (int k = 0; k < 4; ++k) pr[k] = ex2(z[k] - ((ref[k >> 1] == -INFINITY ? 0.f : ref[k >> 1]) - LN_BIAS));
 #pragma unroll
           for (int k = 0; k < 2; ++k)
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(pb + (gr + 8 * k) * LN_PPITCH + (warp * 8 + 2 * t) * 2),
-                         "r"(pack2<VQ2_DT_F16>(pr[2 * k], pr[2 * k + 1])) : "memory");
+            *(uint32_t*)(pb + (gr + 8 * k) * LN_PPITCH + (warp * 8 + 2 * t) * 2) = pack2<VQ2_DT_F16>(pr[2 * k], pr[2 * k + 1]);
         };
         probabilities();
         if (ln_any(raise)) {
@@ -222,20 +232,20 @@ __global__ void __launch_bounds__(LN_THREADS, 1) latent_decode_narrow_kernel(LdA
         l[0] += pr[0] + pr[1];
         l[1] += pr[2] + pr[3];
         // ---------------- O: values 64 warp .. 64 warp + 63 of all the tile's rows
-        if (warp < nl) {
-          const uint32_t col = tile + (warp * 8 + gr) * 4, srow = tile + L / 2 + 2 * R + 2 * warp;
+        if (warp < NL) {
+          const uint8_t* col = tile + 2 * t * pitch + (warp * 8 + gr) * 4;
+          const uint8_t* srow = tile + 2 * t * pitch + L / 2 + 2 * R + 2 * warp;
 #pragma unroll
           for (int ks = 0; ks < LD_TILE / 16; ++ks) {
-            const uint32_t pa = pb + gr * LN_PPITCH + (16 * ks + 2 * t) * 2;
-            const uint32_t a0 = lds32_v(pa), a1 = lds32_v(pa + 8 * LN_PPITCH), a2 = lds32_v(pa + 16), a3 = lds32_v(pa + 8 * LN_PPITCH + 16);
+            const uint8_t* pa = pb + gr * LN_PPITCH + (16 * ks + 2 * t) * 2;
+            const uint32_t a0 = *(const uint32_t*)pa, a1 = *(const uint32_t*)(pa + 8 * LN_PPITCH), a2 = *(const uint32_t*)(pa + 16),
+                           a3 = *(const uint32_t*)(pa + 8 * LN_PPITCH + 16);
             uint32_t w[4], s[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const int r = 16 * ks + 2 * t + (k & 1) + 8 * (k >> 1);
-              w[k] = lds32_v(col + r * pitch);
-              s[k] = lds16_v(srow + r * pitch);
-              // a non-finite scale made the logit NaN for those who see the row; its values must not reach the others
-              if ((s[k] & 0x7C00u) == 0x7C00u) s[k] = 0;
+              const int r = (16 * ks + (k & 1) + 8 * (k >> 1)) * pitch;
+              w[k] = *(const uint32_t*)(col + r);
+              s[k] = *(const uint16_t*)(srow + r);
             }
             const uint32_t sa = s[0] | s[1] << 16, sb = s[2] | s[3] << 16;
             const __half2 sa2 = *(const __half2*)&sa, sb2 = *(const __half2*)&sb;
@@ -258,7 +268,7 @@ __global__ void __launch_bounds__(LN_THREADS, 1) latent_decode_narrow_kernel(LdA
         if (i + 1 == count || p.tile + 1 == p.tiles) {
           // ---------------- this block's part of the query block
           const size_t slot = (size_t)item + blockIdx.x;
-          if (warp < nl) {
+          if (warp < NL) {
             float* dst = g.part + (slot * L + (warp * 8 + 2 * t) * 8) * LN_ROWS + gr;
 #pragma unroll
             for (int v = 0; v < 8; ++v)
