@@ -28,27 +28,25 @@
 
 namespace vq2 {
 
-constexpr int LD_WORKERS = 256, LD_WARPS = LD_WORKERS / 32;
-constexpr int LD_THREADS = LD_WORKERS + 128;     // 168 registers each at launch: 256 x 200 + 128 x 104 afterwards
+constexpr int LD_WORKERS = 512, LD_WARPS = LD_WORKERS / 32;
+constexpr int LD_THREADS = LD_WORKERS + 128;     // 96 registers each at launch: 512 x 104 + 128 x 64 afterwards
 constexpr int LD_UNIT = LD_TILE * 128;  // bytes of a unit of the tile: 64 rows of 64 fp16 values
 constexpr int LD_UNITS = 9;             // 8 for the latent, 1 for the rotary part (P takes its place once S is done)
 constexpr int LD_KBYTES = LD_UNITS * LD_UNIT;
 constexpr float LD_BIAS = 5.f, LD_RAISE = 10.f;    // P = 2^(z - m + BIAS); m is raised when z exceeds it by RAISE
 
-constexpr int LD_PARTS = 4;             // of a tile: two units each, the last with the rotary unit
-// A raw row in shared memory every 448 bytes (at most 400 are used): with 64 modulo 128, the 64-byte pieces that 4 lanes each
-// read of two neighbouring rows fall on different banks.
-constexpr int LD_RAW_ROW = 448, LD_RAW = LD_TILE * LD_RAW_ROW;
+constexpr int LD_PARTS = 2;             // of a tile: four units each, the last with the rotary unit
+constexpr int LD_RAW = LD_TILE * 400;   // a tile's raw rows (at most 400 bytes each)
 // Tiles and raw tiles that fit beside Q (NQ x 1152 bytes) in 227 KB.
 template <int NQ> constexpr int LD_TILES = NQ == 64 ? 1 : 2;
-template <int NQ> constexpr int LD_RAWS = NQ == 32 ? 1 : 2;
+template <int NQ> constexpr int LD_RAWS = NQ == 64 ? 3 : 1;
 
 template <int NQ>
 struct LdShared {
   uint64_t kfull[2][LD_PARTS], kfree[2][LD_PARTS], sfull[2], pfull[2], drain;      // by tile buffer
-  uint64_t rfull[2], rfree[2];       // by raw tile
+  uint64_t rfull[3], rfree[3];       // by raw tile
   uint64_t qfull, qfree;
-  int there[2][LD_TILE];             // whether a raw row was found
+  uint32_t there[3][2];              // rows of a raw tile that were found
   uint32_t tmem;
   int abort;
   LdStart start;
@@ -61,9 +59,9 @@ struct LdShared {
 };
 template <int NQ>
 constexpr size_t ld_smem() { return (size_t)LD_TILES<NQ> * LD_KBYTES + (size_t)LD_RAWS<NQ> * LD_RAW + (size_t)LD_UNITS * NQ * 128 + sizeof(LdShared<NQ>) + 1024; }
-static_assert(ld_smem<64>() <= 227 * 1024 && ld_smem<32>() <= 227 * 1024 && ld_smem<16>() <= 227 * 1024, "latent decode shared memory");
+static_assert(ld_smem<64>() <= 227 * 1024 && ld_smem<32>() <= 227 * 1024, "latent decode shared memory");
 
-__device__ __forceinline__ void ld_sync_workers() { asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void ld_sync_workers() { asm volatile("barrier.cta.sync 1, 512;" ::: "memory"); }
 __device__ __forceinline__ void ld_sync_group(int g) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(2 + g) : "memory"); }
 __device__ __forceinline__ bool ld_any_group(int g, bool p) {
   uint32_t r;
@@ -73,8 +71,7 @@ __device__ __forceinline__ bool ld_any_group(int g, bool p) {
 }
 template <int N>
 __device__ __forceinline__ void ld_tmem_load(uint32_t t, float* v) {
-  if (N == 32) tmem_ld32(t, v);
-  else if (N == 16) tmem_ld16(t, v);
+  if (N == 16) tmem_ld16(t, v);
   else tmem_ld8(t, v);
 }
 // 32 bytes of fp32 in one store (a whole sector).
@@ -111,7 +108,7 @@ __device__ __forceinline__ void ld_score_any(int u, uint32_t d, uint32_t k, uint
 template <int NQ, int M, int KS = 0>
 __device__ __forceinline__ void ld_value_block(uint32_t d, uint32_t v, uint32_t p, uint32_t acc) {
   constexpr uint32_t id = (1u << 4) | (1u << 15) | (1u << 16) | ((uint32_t)(NQ >> 3) << 17) | ((128u >> 4) << 24);
-  constexpr uint32_t p_hi = (uint32_t)(16 * NQ >> 4) | 1u << 14 | (NQ == 64 ? 2u : NQ == 32 ? 4u : 6u) << 29;
+  constexpr uint32_t p_hi = (uint32_t)(16 * NQ >> 4) | 1u << 14 | (NQ == 64 ? 2u : 4u) << 29;
   umma_at<M * (2 * LD_UNIT >> 4) + KS * 128, KS * (2 * NQ), p_hi, id>(d + M * NQ, v, p, KS > 0 ? 1 : acc);
   if constexpr (KS + 1 < LD_TILE / 16) ld_value_block<NQ, M, KS + 1>(d, v, p, acc);
 }
@@ -119,15 +116,15 @@ __device__ __forceinline__ void ld_value_block(uint32_t d, uint32_t v, uint32_t 
 template <int NQ>
 __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) {
   constexpr int TILES = LD_TILES<NQ>, RAWS = LD_RAWS<NQ>;
-  constexpr int CPT = NQ / 2, CPH = NQ / 4;     // columns of S^T (query rows) a column group has, a softmax thread takes
-  constexpr uint32_t COLS = NQ == 64 ? 512 : NQ == 32 ? 256 : 128;    // tensor memory: O^T 4 x NQ columns, S^T 2 x NQ
+  constexpr int CPT = NQ / 4, CPH = NQ / 8;     // columns of S^T (query rows) a column group has, a softmax thread takes
+  constexpr uint32_t COLS = NQ == 64 ? 512 : 256;    // tensor memory: O^T 4 x NQ columns, S^T 2 x NQ
   extern __shared__ __align__(1024) uint8_t ld_smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)ld_smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t kb = smem_u32(smem), qb = kb + TILES * LD_KBYTES, raw = qb + LD_UNITS * NQ * 128;
   LdShared<NQ>* sh = (LdShared<NQ>*)(smem + TILES * LD_KBYTES + LD_UNITS * NQ * 128 + RAWS * LD_RAW);
   const vq2_latent_decode_args& a = g.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  const int L = a.latent_dim, R = a.rope_dim, nl = L / 64, nblk = (nl + 1) / 2;
+  const int L = a.latent_dim, R = a.rope_dim, nl = L / 64, nblk = (nl + 1) / 2, parts = (nl + 3) / 4;
   volatile int* abort = &sh->abort;
   pdl_launch_dependents();
 
@@ -139,6 +136,8 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
       }
       mbar_init(&sh->sfull[k], 1);
       mbar_init(&sh->pfull[k], LD_WARPS);
+    }
+    for (int k = 0; k < RAWS; ++k) {
       mbar_init(&sh->rfull[k], 1);
       mbar_init(&sh->rfree[k], LD_WARPS);
     }
@@ -162,7 +161,7 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
   const uint32_t ts = tmem + 4 * NQ;                    // S^T of the two buffers
 
   if (warp >= LD_WARPS) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == LD_WARPS && count > 0 && elect_one()) {
       // ---------------- products
       LdPos p = sh->start.position(g);
@@ -174,43 +173,29 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
         const uint32_t t = (kb + b * LD_KBYTES) >> 4, v = t | (LD_UNIT >> 4) << 16, pd = (t + nl * (LD_UNIT >> 4)) | 1u << 16;
         const uint32_t acc = opens ? 0 : 1;
         ld_value_block<NQ, 0>(tmem, v, pd, acc);
+        if (nblk > 1) ld_value_block<NQ, 1>(tmem, v, pd, acc);
         umma_commit(&sh->kfree[b][0]);
-        if (nblk > 1) {
-          ld_value_block<NQ, 1>(tmem, v, pd, acc);
-          umma_commit(&sh->kfree[b][1]);
-        }
         if (nblk > 2) {
           ld_value_block<NQ, 2>(tmem, v, pd, acc);
-          umma_commit(&sh->kfree[b][2]);
-        }
-        if (nblk > 3) {
-          ld_value_block<NQ, 3>(tmem, v, pd, acc);
-          umma_commit(&sh->kfree[b][3]);
+          if (nblk > 3) ld_value_block<NQ, 3>(tmem, v, pd, acc);
+          umma_commit(&sh->kfree[b][1]);
         }
       };
       auto scores = [&](int i) {     // S^T = K Q^T of tile i, part by part as it arrives
         const int b = i % TILES;
         const uint32_t k = ((kb + b * LD_KBYTES) >> 4) | 1u << 16, q = (qb >> 4) | 1u << 16, d = ts + b * NQ;
-        auto part = [&](int m) {
-          ld_wait(&sh->kfull[b][m], (i / TILES) & 1, abort);
-          tc_fence_after();
-        };
-        part(0);
+        ld_wait(&sh->kfull[b][0], (i / TILES) & 1, abort);
+        tc_fence_after();
         ld_score_unit<NQ, 0>(d, k, q, 0);
         if (nl > 1) ld_score_unit<NQ, 1>(d, k, q, 1);
-        if (nl > 2) {
-          part(1);
-          ld_score_unit<NQ, 2>(d, k, q, 1);
-          if (nl > 3) ld_score_unit<NQ, 3>(d, k, q, 1);
-        }
+        if (nl > 2) ld_score_unit<NQ, 2>(d, k, q, 1);
+        if (nl > 3) ld_score_unit<NQ, 3>(d, k, q, 1);
         if (nl > 4) {
-          part(2);
+          ld_wait(&sh->kfull[b][1], (i / TILES) & 1, abort);
+          tc_fence_after();
           ld_score_unit<NQ, 4>(d, k, q, 1);
           if (nl > 5) ld_score_unit<NQ, 5>(d, k, q, 1);
-        }
-        if (nl > 6) {
-          part(3);
-          ld_score_unit<NQ, 6>(d, k, q, 1);
+          if (nl > 6) ld_score_unit<NQ, 6>(d, k, q, 1);
           if (nl > 7) ld_score_unit<NQ, 7>(d, k, q, 1);
         }
         if (R) ld_score_any<NQ>(nl, d, k, q);
@@ -259,24 +244,30 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
           }
         }
         const long long off[2] = {rows.offset(g, p, 0), rows.offset(g, p, 1)};
-        const int found = __popc(__ballot_sync(0xffffffffu, off[0] >= 0)) + __popc(__ballot_sync(0xffffffffu, off[1] >= 0));
+        const uint32_t in0 = __ballot_sync(0xffffffffu, off[0] >= 0), in1 = __ballot_sync(0xffffffffu, off[1] >= 0);
+        const long long lead = __shfl_sync(0xffffffffu, off[0], 0);
+        const bool run = __all_sync(0xffffffffu, off[0] == lead + (long long)lane * g.rb && off[1] == lead + (long long)(lane + 32) * g.rb);
         p.next(g);
         if (i + 1 < count) rows.find(g, p);
         ld_wait(&sh->rfree[st], ((i / RAWS) & 1) ^ 1, abort);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) sh->there[st][lane + 32 * k] = off[k] >= 0;
+        if (lane < 2) sh->there[st][lane] = lane ? in1 : in0;
         __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(&sh->rfull[st], found * g.rb);
+        if (lane == 0) mbar_arrive_expect_tx(&sh->rfull[st], (__popc(in0) + __popc(in1)) * g.rb);
         __syncwarp();
+        uint8_t* dst = smem + (raw - kb) + st * LD_RAW;
+        if (run) {                         // 64 rows side by side: one copy
+          if (lane == 0) bulk_g2s(dst, (const uint8_t*)a.cache + lead, LD_TILE * g.rb, &sh->rfull[st]);
+        } else {
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-          if (off[k] >= 0) bulk_g2s(smem + (raw - kb) + st * LD_RAW + (lane + 32 * k) * LD_RAW_ROW, (const uint8_t*)a.cache + off[k], g.rb, &sh->rfull[st]);
+          for (int k = 0; k < 2; ++k)
+            if (off[k] >= 0) bulk_g2s(dst + (lane + 32 * k) * g.rb, (const uint8_t*)a.cache + off[k], g.rb, &sh->rfull[st]);
+        }
       }
       for (int i = max(0, count - RAWS); i < count; ++i) ld_wait(&sh->rfull[i % RAWS], (i / RAWS) & 1, abort);   // no copy left in flight
       ld_wait(&sh->qfull, seg & 1, abort);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     if (count > 0) {
       // ---------------- workers
       // softmax: S^T's row kr is in tensor-memory lane 32 quarter + (kr & 15); the upper 16 lanes of the warp take
@@ -284,75 +275,55 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
       const int quarter = warp & 3, grp = warp >> 2, kr = quarter * 16 + (lane & 15);
       const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
       const int col0 = grp * CPT + (lane >> 4) * CPH;
-      // A warp takes 8 rows of a tile: 4 lanes a row's latent, 64 bytes (two units) a part, and its scales; 8 lanes its
-      // rotary part. The raw tile goes into registers as a whole, so that its place is free for the one after.
-      uint4 lat[LD_PARTS], rope[2], sc;
+      // A warp takes 4 rows of a tile, 8 lanes a row: 128 bytes of nibbles (four units) a part, its scales and its rotary part.
+      // The raw tile goes into registers as a whole, so that its place is free for the one after.
+      uint4 lat[LD_PARTS], rope, sc;
       bool here = false;
-      const int lrow = lane >> 2, piece = lane & 3, chunk = lane & 7;
+      const int row = warp * 4 + (lane >> 3), piece = lane & 7;
       auto read_raw = [&](int i) {
         const int st = i % RAWS;
         ld_wait(&sh->rfull[st], (i / RAWS) & 1, abort);
-        here = sh->there[st][warp * 8 + lrow] != 0;
-        const uint32_t r = raw + st * LD_RAW + (warp * 8 + lrow) * LD_RAW_ROW;
+        here = (sh->there[st][row >> 5] >> (row & 31)) & 1;
+        const uint32_t r = raw + st * LD_RAW + row * g.rb;
 #pragma unroll
         for (int m = 0; m < LD_PARTS; ++m) {
           lat[m] = make_uint4(0, 0, 0, 0);
-          if (here && 4 * m + piece < 2 * nl) lat[m] = lds128_v(r + 64 * m + 16 * piece);
+          if (here && 8 * m + piece < 2 * nl) lat[m] = lds128_v(r + 128 * m + 16 * piece);
         }
-        sc = make_uint4(0, 0, 0, 0);
+        sc = rope = make_uint4(0, 0, 0, 0);
         if (here) sc = lds128_v(r + L / 2 + 2 * R);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int row = warp * 8 + (lane >> 3) + 4 * k;
-          rope[k] = make_uint4(0, 0, 0, 0);
-          if (chunk * 8 < R && sh->there[st][row]) rope[k] = lds128_v(raw + st * LD_RAW + row * LD_RAW_ROW + L / 2 + 16 * chunk);
-        }
+        if (here && piece * 8 < R) rope = lds128_v(r + L / 2 + 16 * piece);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->rfree[st]);
       };
-      // Registers -> tile, a part after another. A piece's four words become four 16-byte chunks of a 128-byte row; lanes of the
-      // part's second unit take their words in another order, so that 8 neighbouring lanes fall on all bank groups.
+      // Registers -> tile, a part after another. A piece's four words become four 16-byte chunks of a 128-byte row; each of the
+      // part's four units takes its words in another order, so that 8 neighbouring lanes fall on all bank groups.
       auto expand = [&](int number) {
-        const int b = number % TILES, row = warp * 8 + lrow;
-        const uint32_t tile = kb + b * LD_KBYTES;
-        const uint32_t scale[LD_PARTS] = {sc.x, sc.y, sc.z, sc.w};
+        const int b = number % TILES, turn = piece >> 1;
+        const uint32_t tile = kb + b * LD_KBYTES + row * 128;
         if (!here && piece == 0) sh->flag[b][row] = 2 * number;
 #pragma unroll
         for (int m = 0; m < LD_PARTS; ++m) {
-          if (m >= nblk) break;
+          if (m >= parts) break;
           if (number >= TILES) ld_wait(&sh->kfree[b][m], (number / TILES - 1) & 1, abort);
-          uint32_t s = piece & 2 ? scale[m] >> 16 : scale[m] & 0xFFFFu;
-          if (4 * m + piece < 2 * nl) {
+          if (8 * m + piece < 2 * nl) {
+            const uint32_t two = piece & 4 ? (m ? sc.w : sc.y) : (m ? sc.z : sc.x);
+            uint32_t s = piece & 2 ? two >> 16 : two & 0xFFFFu;
             if ((s & 0x7C00u) == 0x7C00u) {       // a non-finite scale: the row reads as NaN, see the softmax
               s = 0;
               sh->flag[b][row] = 2 * number + 1;
             }
             const __half2 s2 = __half2half2(__ushort_as_half((unsigned short)s)), c2 = __hmul2(s2, __float2half2_rn(-24.f));
-            const uint32_t w[4] = {piece & 2 ? lat[m].z : lat[m].x, piece & 2 ? lat[m].w : lat[m].y, piece & 2 ? lat[m].x : lat[m].z,
-                                   piece & 2 ? lat[m].y : lat[m].w};
-            const uint32_t base = tile + (2 * m + (piece >> 1)) * LD_UNIT + row * 128;
+            uint32_t w0 = lat[m].x, w1 = lat[m].y, w2 = lat[m].z, w3 = lat[m].w, t;
+            if (turn & 1) { t = w0; w0 = w1; w1 = t; t = w2; w2 = w3; w3 = t; }
+            if (turn & 2) { t = w0; w0 = w2; w2 = t; t = w1; w1 = w3; w3 = t; }
+            const uint32_t w[4] = {w0, w1, w2, w3};
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              // nibble u = n + 8 in the top mantissa bits of 16 + u; (16 + u) s - 24 s = n s, exact in fp16
-              const uint32_t h[4] = {(w[q] << 6 & 0x03C003C0u) | 0x4C004C00u, (w[q] << 2 & 0x03C003C0u) | 0x4C004C00u,
-                                     (w[q] >> 2 & 0x03C003C0u) | 0x4C004C00u, (w[q] >> 6 & 0x03C003C0u) | 0x4C004C00u};
-              uint4 v;
-              __half2 x;
-              x = __hfma2(*(const __half2*)&h[0], s2, c2); v.x = *(uint32_t*)&x;
-              x = __hfma2(*(const __half2*)&h[1], s2, c2); v.y = *(uint32_t*)&x;
-              x = __hfma2(*(const __half2*)&h[2], s2, c2); v.z = *(uint32_t*)&x;
-              x = __hfma2(*(const __half2*)&h[3], s2, c2); v.w = *(uint32_t*)&x;
-              const int c = (piece & 1) * 4 + (q ^ (piece & 2));
-              sts128_v(base + ((c ^ (row & 7)) << 4), v);
-            }
+            for (int q = 0; q < 4; ++q)
+              sts128_v(tile + (4 * m + turn) * LD_UNIT + ((((piece & 1) * 4 + (q ^ turn)) ^ (row & 7)) << 4),
+                       make_uint4(ln_pair<0>(w[q], s2, c2), ln_pair<1>(w[q], s2, c2), ln_pair<2>(w[q], s2, c2), ln_pair<3>(w[q], s2, c2)));
           }
-          if (m == nblk - 1 && R) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int r = warp * 8 + (lane >> 3) + 4 * k;
-              sts128_v(tile + nl * LD_UNIT + r * 128 + ((chunk ^ (r & 7)) << 4), rope[k]);
-            }
-          }
+          if (m == parts - 1 && R) sts128_v(tile + nl * LD_UNIT + ((piece ^ (row & 7)) << 4), rope);
           fence_async_smem();
           tc_fence_before();
           __syncwarp();
@@ -364,7 +335,7 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
       auto softmax = [&](int i, const LdPos& p, bool opens, int seg) {
         const int b = i % TILES;
         ld_wait(&sh->sfull[b], (i / TILES) & 1, abort);
-        ld_wait(&sh->kfull[b][nblk - 1], (i / TILES) & 1, abort);        // long done: orders the other warps' flags before their reads
+        ld_wait(&sh->kfull[b][parts - 1], (i / TILES) & 1, abort);        // long done: orders the other warps' flags before their reads
         tc_fence_after();
         float z[CPH];
         {
@@ -409,7 +380,7 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
             if ((lane & 15) == 0) sh->red[quarter][col0 + c] = m;
           }
           // O is rescaled below: every product into it so far has to be done (P V of the tile before)
-          if (!opens) ld_wait(&sh->kfree[(i - 1) % TILES][nblk - 1], ((i - 1) / TILES) & 1, abort);
+          if (!opens) ld_wait(&sh->kfree[(i - 1) % TILES][parts - 1], ((i - 1) / TILES) & 1, abort);
           tc_fence_after();
           ld_sync_group(grp);
 #pragma unroll
@@ -449,17 +420,11 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
         }
         // rows of 2 NQ bytes, 16-byte chunks swizzled as the descriptor says
         const uint32_t prow = kb + b * LD_KBYTES + nl * LD_UNIT + kr * (2 * NQ), at = col0 * 2;
-        if (NQ == 64) {
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-            sts128_v(prow + ((((at >> 4) + k) ^ (kr & 7)) << 4), make_uint4(ph[4 * k % (CPH / 2)], ph[(4 * k + 1) % (CPH / 2)],
-                                                                            ph[(4 * k + 2) % (CPH / 2)], ph[(4 * k + 3) % (CPH / 2)]));
-        } else if (NQ == 32) {
-          sts128_v(prow + (((at >> 4) ^ ((kr >> 1) & 3)) << 4), make_uint4(ph[0], ph[1], ph[2 % (CPH / 2)], ph[3 % (CPH / 2)]));
-        } else {
-          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(prow + (((at >> 4) ^ ((kr >> 2) & 1)) << 4) + (at & 15)), "r"(ph[0]), "r"(ph[1])
+        if (NQ == 64)
+          sts128_v(prow + (((at >> 4) ^ (kr & 7)) << 4), make_uint4(ph[0], ph[1], ph[2 % (CPH / 2)], ph[3 % (CPH / 2)]));
+        else
+          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(prow + (((at >> 4) ^ ((kr >> 1) & 3)) << 4) + (at & 15)), "r"(ph[0]), "r"(ph[1])
                        : "memory");
-        }
         fence_async_smem();
         tc_fence_before();
         __syncwarp();
@@ -516,7 +481,7 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
         }
         softmax(is, ps, is == 0 || ps.tile == 0, seg);
         if (is + 1 == count || ps.tile + 1 == ps.tiles) {
-          ld_wait(&sh->kfree[is % TILES][nblk - 1], (is / TILES) & 1, abort);
+          ld_wait(&sh->kfree[is % TILES][parts - 1], (is / TILES) & 1, abort);
           tc_fence_after();
           finish(ps);
           tc_fence_before();
