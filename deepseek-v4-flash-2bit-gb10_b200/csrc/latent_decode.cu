@@ -24,6 +24,7 @@
 // path is kept busy: a tile is handed over in parts of 128 latent values, S starts on the first part, and
 // a part is filled again as soon as P V has used it. Up to 32 query rows there is room for two tiles, and the softmax of a
 // tile runs under the products of the next. In the steady state no barrier spans the block.
+#include <algorithm>
 #include "latent_decode.cuh"
 
 namespace vq2 {
@@ -524,7 +525,8 @@ static LdLayout ld_layout(int B, int nq, int nrb, int L, int R, int grid) {
   w.total = at + 256;
   return w;
 }
-constexpr int LD_MAX_GRID = 148;        // workspace is sized without a device; a B200 has 148 SMs
+// Blocks that share the tiles: two an SM for the narrow kernel. The workspace is sized without a device; a B200 has 148 SMs.
+static int ld_blocks(int nq, int sms) { return std::min(sms, 148) * (nq == 16 ? 2 : 1); }
 
 // Three launches: query rows, the main kernel (NQ rows a block; NARROW: the one for 16), the join; the later two by programmatic
 // dependent launch.
@@ -573,7 +575,7 @@ extern "C" size_t vq2_latent_decode_workspace_size(int B, int T, int heads, int 
       (long long)B * ((long long)T * heads + 64) >= 1LL << 27)
     return 0;
   const int nq = ld_nq(T, heads);
-  return ld_layout(B, nq, (int)(((long long)T * heads + nq - 1) / nq), latent_dim, rope_dim, LD_MAX_GRID).total;
+  return ld_layout(B, nq, (int)(((long long)T * heads + nq - 1) / nq), latent_dim, rope_dim, ld_blocks(nq, 148)).total;
 }
 
 extern "C" int vq2_latent_decode(const vq2_latent_decode_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -595,7 +597,7 @@ extern "C" int vq2_latent_decode(const vq2_latent_decode_args* a, void* ws, size
   if (sms <= 0) return VQ2_ERR_CUDA;
   g.rb = latent_row_bytes(a->latent_dim, a->rope_dim);
   g.nrb = (a->T * a->heads + nq - 1) / nq;
-  g.grid = min(sms, LD_MAX_GRID);
+  g.grid = ld_blocks(nq, sms);
   // j / page_size for 0 <= j < 2^31: a shift, or with s = ceil(log2 page_size) the high half of j * ceil(2^(31+s) / page_size)
   int s = 0;
   while ((1LL << s) < a->page_size) ++s;
