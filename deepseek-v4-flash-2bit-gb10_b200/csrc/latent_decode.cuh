@@ -132,9 +132,9 @@ struct LdRows {
 
 
 // Query rows, one warp a row: latent part rotated, all scaled into fp16's range by a power of two. Written as swizzled units of
-// NQ rows x 64 values, or (ROWS) row by row.
+// NQ rows x 64 values, or (OPERANDS, 16 rows) as the left operands of m16n8k16 products.
 constexpr int LQ_WARPS = 4;
-template <int DT, int NQ, bool ROWS>
+template <int DT, int NQ, bool OPERANDS>
 __global__ void __launch_bounds__(LQ_WARPS * 32) latent_query_kernel(LdArgs g) {
   pdl_launch_dependents();
   const vq2_latent_decode_args& a = g.a;
@@ -157,14 +157,21 @@ __global__ void __launch_bounds__(LQ_WARPS * 32) latent_query_kernel(LdArgs g) {
     for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[k][i]));
   }
   const float2 f = f16_range_scale(fminf(warp_max(m), 3.0e38f));
-  uint8_t* dst = ROWS ? g.q + (size_t)at * units * 128 : g.q + (size_t)item * units * (NQ * 128) + r * 128;
+  uint8_t* dst = g.q + (size_t)item * units * (NQ * 128);
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
     const int u = k < 2 ? lane + 32 * k : lane, unit = k < 2 ? u >> 3 : nl, c = u & 7;
-    if (k < 2 ? u * 8 < L : R && u < 8)
-      *(uint4*)(dst + (ROWS ? unit * 128 + c * 16 : unit * (NQ * 128) + ((c ^ (r & 7)) << 4))) =
-          make_uint4(pack2<VQ2_DT_F16>(v[k][0] * f.x, v[k][1] * f.x), pack2<VQ2_DT_F16>(v[k][2] * f.x, v[k][3] * f.x),
-                     pack2<VQ2_DT_F16>(v[k][4] * f.x, v[k][5] * f.x), pack2<VQ2_DT_F16>(v[k][6] * f.x, v[k][7] * f.x));
+    if (!(k < 2 ? u * 8 < L : R && u < 8)) continue;
+    const uint32_t w[4] = {pack2<VQ2_DT_F16>(v[k][0] * f.x, v[k][1] * f.x), pack2<VQ2_DT_F16>(v[k][2] * f.x, v[k][3] * f.x),
+                           pack2<VQ2_DT_F16>(v[k][4] * f.x, v[k][5] * f.x), pack2<VQ2_DT_F16>(v[k][6] * f.x, v[k][7] * f.x)};
+    if (OPERANDS) {
+      // piece 2 unit + c / 4, lane 4 (r mod 8) + c mod 4; values 0-1 and 2-3 are registers r / 8 and r / 8 + 2 of its first product
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        ((uint32_t*)dst)[(((2 * unit + (c >> 2)) * 2 + (j >> 1)) * 32 + (r & 7) * 4 + (c & 3)) * 4 + (r >> 3) + 2 * (j & 1)] = w[j];
+    } else {
+      *(uint4*)(dst + (size_t)unit * (NQ * 128) + r * 128 + ((c ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
   // a row that pads the block sees nothing
   if (lane == 0)

@@ -19,13 +19,11 @@ namespace vq2 {
 
 constexpr int LN_ROWS = 16, LN_WARPS = 8, LN_THREADS = LN_WARPS * 32;
 constexpr int LN_STAGES = 3, LN_STAGE = LD_TILE * 400;
-constexpr int LN_QPITCH = 9 * 128 + 64;                        // bytes of a query row: neighbouring rows on the other half of the banks
 constexpr float LN_BIAS = 5.f, LN_RAISE = 10.f;                // P = 2^(z - m + BIAS)
-constexpr int LN_PPITCH = 144;                                 // bytes of a row of P: 64 fp16 values, rows on different banks
 
 struct LnShared {
-  alignas(16) uint8_t q[LN_ROWS * LN_QPITCH];
-  alignas(16) uint8_t p[2][LN_ROWS * LN_PPITCH];
+  uint4 q[18][2][32];                  // query rows as operands: piece of 32 values, product, lane
+  uint4 p[2][LD_TILE / 16][32];        // probabilities as operands: 16 cached rows, lane
   float4 half[LN_WARPS][32];           // sums over half of the values, on their way to the other warp of the pair
   uint64_t rfull[LN_STAGES];
   uint32_t there[LN_STAGES][2];        // rows of a tile that were found
@@ -37,14 +35,17 @@ struct LnShared {
 constexpr size_t LN_SMEM = (size_t)LN_STAGES * LN_STAGE + sizeof(LnShared) + 128;
 static_assert(2 * (LN_SMEM + 1024) <= 228 * 1024, "two blocks on an SM");
 
-__device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+// The left operand's four registers are neighbours as they come from shared memory (moved there they cost as much as the
+// product).
+__device__ __forceinline__ void mma16816(float* c, const uint4& a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 // Nibbles J of both halves of w, as n s in fp16: nibble u = n + 8 in the top mantissa bits of 16 + u; (16 + u) s - 24 s, exact.
 template <int J>
 __device__ __forceinline__ uint32_t ln_pair(uint32_t w, __half2 s2, __half2 c2) {
-  const uint32_t h = ((J < 2 ? w << (6 - 4 * J) : w >> (4 * J - 6)) & 0x03C003C0u) | 0x4C004C00u;
+  uint32_t h;                            // (and, or) in one instruction: given two constants the compiler makes it two
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(h) : "r"(J < 2 ? w << (6 - 4 * J) : w >> (4 * J - 6)), "r"(0x03C003C0u), "r"(0x4C004C00u));
   const __half2 x = __hfma2(*(const __half2*)&h, s2, c2);
   return *(const uint32_t*)&x;
 }
@@ -60,18 +61,18 @@ __device__ __forceinline__ void ln_sync_pair(int k) { asm volatile("barrier.cta.
 
 // Pieces FROM .. TO - 1 (32 values each) of the latent part of S for 16 cached rows: acc[u] for rows 8 u .. 8 u + 7 of them.
 template <int FROM, int TO>
-__device__ __forceinline__ void ln_scores(float (*acc)[2][4], const uint8_t* q, const uint8_t* row0, const uint8_t* row1, const uint32_t* sc0,
-                                          const uint32_t* sc1, int t) {
+__device__ __forceinline__ void ln_scores(float (*acc)[2][4], const uint4 (*q)[2][32], const uint8_t* row0, const uint8_t* row1,
+                                          const uint32_t* sc0, const uint32_t* sc1, int lane) {
 #pragma unroll
   for (int n = FROM; n < TO; ++n) {
-    const uint4 qa = *(const uint4*)(q + n * 64), qb = *(const uint4*)(q + 8 * LN_QPITCH + n * 64);
+    const uint4 qa = q[n][0][lane], qb = q[n][1][lane];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const uint32_t s = __byte_perm((u ? sc1 : sc0)[n >> 2], 0, (n >> 1) & 1 ? 0x3232 : 0x1010);
       const __half2 s2 = *(const __half2*)&s, c2 = __hmul2(s2, __float2half2_rn(-24.f));
-      const uint32_t w = *(const uint32_t*)((u ? row1 : row0) + (4 * n + t) * 4);
-      mma16816(acc[u][0], qa.x, qb.x, qa.y, qb.y, ln_pair<0>(w, s2, c2), ln_pair<1>(w, s2, c2));
-      mma16816(acc[u][1], qa.z, qb.z, qa.w, qb.w, ln_pair<2>(w, s2, c2), ln_pair<3>(w, s2, c2));
+      const uint32_t w = *(const uint32_t*)((u ? row1 : row0) + (4 * n + (lane & 3)) * 4);
+      mma16816(acc[u][0], qa, ln_pair<0>(w, s2, c2), ln_pair<1>(w, s2, c2));
+      mma16816(acc[u][1], qb, ln_pair<2>(w, s2, c2), ln_pair<3>(w, s2, c2));
     }
   }
 }
@@ -139,10 +140,7 @@ __global__ void __launch_bounds__(LN_THREADS, 2) latent_decode_narrow_kernel(LdA
       if (i == 0 || p.tile == 0) {                // a new query block: its rows to shared memory (the one before is done with)
         if (i == 0) pdl_wait();
         const uint4* src = (const uint4*)(g.q + (size_t)item * LN_ROWS * units * 128);
-        for (int u = tid; u < LN_ROWS * units * 8; u += LN_THREADS) {
-          const int row = u / (units * 8);
-          *(uint4*)(sh->q + row * LN_QPITCH + (u - row * units * 8) * 16) = src[u];
-        }
+        for (int u = tid; u < LN_ROWS * units * 8; u += LN_THREADS) ((uint4*)sh->q)[u] = src[u];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const float2 m = g.meta[item * LN_ROWS + gr + 8 * k];
@@ -164,23 +162,22 @@ __global__ void __launch_bounds__(LN_THREADS, 2) latent_decode_narrow_kernel(LdA
         uint8_t* row1 = row0 + 8 * PITCH;
         const uint4 x0 = *(const uint4*)(row0 + tail), x1 = *(const uint4*)(row1 + tail);
         const uint32_t sc0[4] = {x0.x, x0.y, x0.z, x0.w}, sc1[4] = {x1.x, x1.y, x1.z, x1.w};
-        const uint8_t* q = sh->q + gr * LN_QPITCH + t * 16;
         float acc[2][2][4] = {};
         if (half == 0) {
-          ln_scores<0, NL + 1>(acc, q, row0, row1, sc0, sc1, t);
+          ln_scores<0, NL + 1>(acc, sh->q, row0, row1, sc0, sc1, lane);
         } else {
-          ln_scores<NL + 1, 2 * NL>(acc, q, row0, row1, sc0, sc1, t);
+          ln_scores<NL + 1, 2 * NL>(acc, sh->q, row0, row1, sc0, sc1, lane);
           if (R) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              const uint4 qa = *(const uint4*)(q + (2 * NL + k) * 64), qb = *(const uint4*)(q + 8 * LN_QPITCH + (2 * NL + k) * 64);
+              const uint4 qa = sh->q[2 * NL + k][0][lane], qb = sh->q[2 * NL + k][1][lane];
               const int d = k * 32 + 8 * t;
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
                 uint4 w = make_uint4(0, 0, 0, 0);
                 if (d < R) w = *(const uint4*)((u ? row1 : row0) + L / 2 + 2 * d);
-                mma16816(acc[u][0], qa.x, qb.x, qa.y, qb.y, w.x, w.y);
-                mma16816(acc[u][1], qa.z, qb.z, qa.w, qb.w, w.z, w.w);
+                mma16816(acc[u][0], qa, w.x, w.y);
+                mma16816(acc[u][1], qb, w.z, w.w);
               }
             }
           }
@@ -223,14 +220,13 @@ __global__ void __launch_bounds__(LN_THREADS, 2) latent_decode_narrow_kernel(LdA
         if (!((there >> (k & 1)) & 1) || j > p.len - a.T + tok[k >> 1]) z[k] = -INFINITY;
         raise |= z[k] > ref[k >> 1] + LN_RAISE;
       }
-      uint8_t* pb = sh->p[i & 1];
+      uint4 (*pb)[32] = sh->p[i & 1];
       float pr[4];
       auto probabilities = [&]() {
 #pragma unroll
         for (int k = 0; k < 4; ++k) pr[k] = ex2(z[k] - ((ref[k >> 1] == -INFINITY ? 0.f : ref[k >> 1]) - LN_BIAS));
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          *(uint32_t*)(pb + (gr + 8 * k) * LN_PPITCH + (mine + 2 * t) * 2) = pack2<VQ2_DT_F16>(pr[2 * k], pr[2 * k + 1]);
+        // registers 0, 1 (rows gr, gr + 8) of the operand of 16 cached rows for the first 8 of them, 2, 3 for the others
+        *((uint2*)&pb[quad][lane] + half) = make_uint2(pack2<VQ2_DT_F16>(pr[0], pr[1]), pack2<VQ2_DT_F16>(pr[2], pr[3]));
       };
       probabilities();
       if (ln_any(raise)) {
@@ -275,9 +271,7 @@ __global__ void __launch_bounds__(LN_THREADS, 2) latent_decode_narrow_kernel(LdA
         const uint8_t* srow = tile + 2 * t * PITCH + tail + 2 * warp;
 #pragma unroll
         for (int ks = 0; ks < LD_TILE / 16; ++ks) {
-          const uint8_t* pa = pb + gr * LN_PPITCH + (16 * ks + 2 * t) * 2;
-          const uint32_t a0 = *(const uint32_t*)pa, a1 = *(const uint32_t*)(pa + 8 * LN_PPITCH), a2 = *(const uint32_t*)(pa + 16),
-                         a3 = *(const uint32_t*)(pa + 8 * LN_PPITCH + 16);
+          const uint4 pa = pb[ks][lane];
           uint32_t w[4], s[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -291,14 +285,14 @@ __global__ void __launch_bounds__(LN_THREADS, 2) latent_decode_narrow_kernel(LdA
           // halves of two rows' words side by side: values 2 j in the low ones, 2 j + 1 in the high ones
           const uint32_t al = __byte_perm(w[0], w[1], 0x5410), ah = __byte_perm(w[0], w[1], 0x7632);
           const uint32_t bl = __byte_perm(w[2], w[3], 0x5410), bh = __byte_perm(w[2], w[3], 0x7632);
-          mma16816(o[0], a0, a1, a2, a3, ln_pair<0>(al, sa2, ca2), ln_pair<0>(bl, sb2, cb2));
-          mma16816(o[1], a0, a1, a2, a3, ln_pair<0>(ah, sa2, ca2), ln_pair<0>(bh, sb2, cb2));
-          mma16816(o[2], a0, a1, a2, a3, ln_pair<1>(al, sa2, ca2), ln_pair<1>(bl, sb2, cb2));
-          mma16816(o[3], a0, a1, a2, a3, ln_pair<1>(ah, sa2, ca2), ln_pair<1>(bh, sb2, cb2));
-          mma16816(o[4], a0, a1, a2, a3, ln_pair<2>(al, sa2, ca2), ln_pair<2>(bl, sb2, cb2));
-          mma16816(o[5], a0, a1, a2, a3, ln_pair<2>(ah, sa2, ca2), ln_pair<2>(bh, sb2, cb2));
-          mma16816(o[6], a0, a1, a2, a3, ln_pair<3>(al, sa2, ca2), ln_pair<3>(bl, sb2, cb2));
-          mma16816(o[7], a0, a1, a2, a3, ln_pair<3>(ah, sa2, ca2), ln_pair<3>(bh, sb2, cb2));
+          mma16816(o[0], pa, ln_pair<0>(al, sa2, ca2), ln_pair<0>(bl, sb2, cb2));
+          mma16816(o[1], pa, ln_pair<0>(ah, sa2, ca2), ln_pair<0>(bh, sb2, cb2));
+          mma16816(o[2], pa, ln_pair<1>(al, sa2, ca2), ln_pair<1>(bl, sb2, cb2));
+          mma16816(o[3], pa, ln_pair<1>(ah, sa2, ca2), ln_pair<1>(bh, sb2, cb2));
+          mma16816(o[4], pa, ln_pair<2>(al, sa2, ca2), ln_pair<2>(bl, sb2, cb2));
+          mma16816(o[5], pa, ln_pair<2>(ah, sa2, ca2), ln_pair<2>(bh, sb2, cb2));
+          mma16816(o[6], pa, ln_pair<3>(al, sa2, ca2), ln_pair<3>(bl, sb2, cb2));
+          mma16816(o[7], pa, ln_pair<3>(ah, sa2, ca2), ln_pair<3>(bh, sb2, cb2));
         }
       }
       if (i + 1 == count || p.tile + 1 == p.tiles) {
