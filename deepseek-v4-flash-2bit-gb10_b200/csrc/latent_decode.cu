@@ -500,9 +500,13 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
   if (warp == LD_WARPS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS));
 }
 
-static int ld_nq(int T, int heads) {
+// Query rows a block, by the rows of a sequence. Up to 16 the narrow kernel; up to 32, or more, the wide one with that many
+// (64 sequences, 320,206 cached rows: 16 query rows 84 us narrow, 151 us with 64 wide; 32 rows 122 us with 32 wide, 141 us as two
+// narrow blocks, 151 us with 64 wide; 48 rows 158 us with 64 wide, 201 us narrow). Where every tile of every 16 rows has a block of
+// its own at once, time is latency, and the narrow kernel has less of it (64 rows, 64 cached: 11 us, 18 us wide).
+static int ld_nq(int B, int T, int heads, long long most) {
   const long long rows = (long long)T * heads;
-  return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  return rows <= 16 || (double)B * ((most + LD_TILE - 1) / LD_TILE) * ((rows + 15) / 16) <= 2 * 148 ? 16 : rows <= 32 ? 32 : 64;
 }
 
 struct LdLayout {
@@ -561,9 +565,10 @@ static int ld_launch(const LdArgs& g, cudaStream_t st) {
   cfg.dynamicSmemBytes = smem;
   if (cudaLaunchKernelEx(&cfg, kernel, g) != cudaSuccess) return VQ2_ERR_CUDA;
   cfg.gridDim = dim3((unsigned)(items * (g.a.latent_dim / 64) * (NQ / 8)));
-  cfg.blockDim = dim3(LJ_WARPS * 32);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, latent_join_kernel<DT, NQ>, g) == cudaSuccess ? VQ2_OK : VQ2_ERR_CUDA;
+  const bool many = g.grid > 8 * items;          // parts a query block: at most about grid / items
+  cfg.blockDim = dim3(many ? 512 : 128);
+  return cudaLaunchKernelEx(&cfg, many ? latent_join_kernel<DT, NQ, 16> : latent_join_kernel<DT, NQ, 4>, g) == cudaSuccess ? VQ2_OK : VQ2_ERR_CUDA;
 }
 
 }  // namespace vq2
@@ -574,8 +579,11 @@ extern "C" size_t vq2_latent_decode_workspace_size(int B, int T, int heads, int 
   if (B <= 0 || T <= 0 || heads <= 0 || !latent_dims_ok(latent_dim, rope_dim) || (long long)T * heads > 1 << 20 ||
       (long long)B * ((long long)T * heads + 64) >= 1LL << 27)
     return 0;
-  const int nq = ld_nq(T, heads);
-  return ld_layout(B, nq, (int)(((long long)T * heads + nq - 1) / nq), latent_dim, rope_dim, ld_blocks(nq, 148)).total;
+  // the larger of what the two kernels that may be taken need
+  size_t most = 0;
+  for (const int nq : {16, ld_nq(B, T, heads, 1LL << 40)})
+    most = std::max(most, ld_layout(B, nq, (int)(((long long)T * heads + nq - 1) / nq), latent_dim, rope_dim, ld_blocks(nq, 148)).total);
+  return most;
 }
 
 extern "C" int vq2_latent_decode(const vq2_latent_decode_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -593,7 +601,7 @@ extern "C" int vq2_latent_decode(const vq2_latent_decode_args* a, void* ws, size
     return VQ2_ERR_WORKSPACE;
   LdArgs g = {};
   g.a = *a;
-  const int nq = ld_nq(a->T, a->heads), sms = device_sm_count();
+  const int nq = ld_nq(a->B, a->T, a->heads, (long long)a->max_pages * a->page_size), sms = device_sm_count();
   if (sms <= 0) return VQ2_ERR_CUDA;
   g.rb = latent_row_bytes(a->latent_dim, a->rope_dim);
   g.nrb = (a->T * a->heads + nq - 1) / nq;

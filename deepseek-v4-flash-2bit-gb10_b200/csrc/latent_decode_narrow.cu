@@ -135,9 +135,80 @@ __global__ void __launch_bounds__(LN_THREADS, 2) latent_decode_narrow_kernel(LdA
     if (warp == 0 && LN_STAGES - 1 < count) rows.find(g, pl);
     float o[8][4], l[2], ref[2], fac[2];
     int tok[2];
-    for (int i = 0; i < count; ++i) {
-      const int st = i % LN_STAGES, item = p.b * g.nrb + p.rb;
-      if (i == 0 || p.tile == 0) {                // a new query block: its rows to shared memory (the one before is done with)
+    // ---------------- O: values 64 warp .. 64 warp + 63 of all rows of tile i
+    auto values = [&](int i) {
+      const uint8_t* tile = ln_smem + i % LN_STAGES * LN_STAGE;
+      const uint4 (*pb)[32] = sh->p[i & 1];
+      if (NL == LN_WARPS || warp < NL) {
+        const uint8_t* col = tile + 2 * t * PITCH + (warp * 8 + gr) * 4;
+        const uint8_t* srow = tile + 2 * t * PITCH + tail + 2 * warp;
+#pragma unroll
+        for (int ks = 0; ks < LD_TILE / 16; ++ks) {
+          const uint4 pa = pb[ks][lane];
+          uint32_t w[4], s[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int r = (16 * ks + (k & 1) + 8 * (k >> 1)) * PITCH;
+            w[k] = *(const uint32_t*)(col + r);
+            s[k] = *(const uint16_t*)(srow + r);
+          }
+          const uint32_t sa = s[0] | s[1] << 16, sb = s[2] | s[3] << 16;
+          const __half2 sa2 = *(const __half2*)&sa, sb2 = *(const __half2*)&sb;
+          const __half2 ca2 = __hmul2(sa2, __float2half2_rn(-24.f)), cb2 = __hmul2(sb2, __float2half2_rn(-24.f));
+          // halves of two rows' words side by side: values 2 j in the low ones, 2 j + 1 in the high ones
+          const uint32_t al = __byte_perm(w[0], w[1], 0x5410), ah = __byte_perm(w[0], w[1], 0x7632);
+          const uint32_t bl = __byte_perm(w[2], w[3], 0x5410), bh = __byte_perm(w[2], w[3], 0x7632);
+          mma16816(o[0], pa, ln_pair<0>(al, sa2, ca2), ln_pair<0>(bl, sb2, cb2));
+          mma16816(o[1], pa, ln_pair<0>(ah, sa2, ca2), ln_pair<0>(bh, sb2, cb2));
+          mma16816(o[2], pa, ln_pair<1>(al, sa2, ca2), ln_pair<1>(bl, sb2, cb2));
+          mma16816(o[3], pa, ln_pair<1>(ah, sa2, ca2), ln_pair<1>(bh, sb2, cb2));
+          mma16816(o[4], pa, ln_pair<2>(al, sa2, ca2), ln_pair<2>(bl, sb2, cb2));
+          mma16816(o[5], pa, ln_pair<2>(ah, sa2, ca2), ln_pair<2>(bh, sb2, cb2));
+          mma16816(o[6], pa, ln_pair<3>(al, sa2, ca2), ln_pair<3>(bl, sb2, cb2));
+          mma16816(o[7], pa, ln_pair<3>(ah, sa2, ca2), ln_pair<3>(bh, sb2, cb2));
+        }
+      }
+    };
+    auto finish = [&](int item) {
+      // ---------------- this block's part of the query block
+      const size_t slot = (size_t)item + blockIdx.x;
+      if (warp < NL) {
+        float* dst = g.part + (slot * L + (warp * 8 + 2 * t) * 8) * LN_ROWS + gr;
+#pragma unroll
+        for (int v = 0; v < 8; ++v)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) dst[((k & 1) * 8 + v) * LN_ROWS + 8 * (k >> 1)] = o[v][k];
+      }
+      ln_sync();                     // the maxima's place is free
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float s = l[k] + __shfl_xor_sync(0xffffffffu, l[k], 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        if (t == 0) sh->red[warp][gr + 8 * k] = s;
+      }
+      ln_sync();
+      if (warp == 0 && t == 0)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float s = 0.f;
+#pragma unroll
+          for (int w = 0; w < LN_WARPS; ++w) s += sh->red[w][gr + 8 * k];
+          g.ml[slot * LN_ROWS + gr + 8 * k] = make_float2(ref[k], s);
+        }
+      ln_sync();
+    };
+    // The products of O run a tile behind, beside those of S of the next: two independent chains in one run of instructions.
+    int item = 0;
+    for (int i = 0;; ++i) {
+      const int st = i % LN_STAGES;
+      const bool fresh = i == 0 || i == count || p.tile == 0;
+      if (i > 0 && fresh) {
+        values(i - 1);
+        finish(item);
+      }
+      if (i == count) break;
+      if (fresh) {                                // a new query block: its rows to shared memory (the one before is done with)
+        item = p.b * g.nrb + p.rb;
         if (i == 0) pdl_wait();
         const uint4* src = (const uint4*)(g.q + (size_t)item * LN_ROWS * units * 128);
         for (int u = tid; u < LN_ROWS * units * 8; u += LN_THREADS) ((uint4*)sh->q)[u] = src[u];
@@ -163,9 +234,8 @@ __global__ void __launch_bounds__(LN_THREADS, 2) latent_decode_narrow_kernel(LdA
         const uint4 x0 = *(const uint4*)(row0 + tail), x1 = *(const uint4*)(row1 + tail);
         const uint32_t sc0[4] = {x0.x, x0.y, x0.z, x0.w}, sc1[4] = {x1.x, x1.y, x1.z, x1.w};
         float acc[2][2][4] = {};
-        if (half == 0) {
-          ln_scores<0, NL + 1>(acc, sh->q, row0, row1, sc0, sc1, lane);
-        } else {
+        auto low = [&]() { ln_scores<0, NL + 1>(acc, sh->q, row0, row1, sc0, sc1, lane); };
+        auto high = [&]() {
           ln_scores<NL + 1, 2 * NL>(acc, sh->q, row0, row1, sc0, sc1, lane);
           if (R) {
 #pragma unroll
@@ -181,6 +251,16 @@ __global__ void __launch_bounds__(LN_THREADS, 2) latent_decode_narrow_kernel(LdA
               }
             }
           }
+        };
+        if (fresh) {
+          if (half == 0) low();
+          else high();
+        } else if (half == 0) {
+          low();
+          values(i - 1);
+        } else {
+          high();
+          values(i - 1);
         }
         const int away = half ^ 1;                // the rows that the other warp of the pair keeps
         float give[4], keep[4];
@@ -265,64 +345,6 @@ __global__ void __launch_bounds__(LN_THREADS, 2) latent_decode_narrow_kernel(LdA
       }
       l[0] += pr[0] + pr[1];
       l[1] += pr[2] + pr[3];
-      // ---------------- O: values 64 warp .. 64 warp + 63 of all the tile's rows
-      if (warp < NL) {
-        const uint8_t* col = tile + 2 * t * PITCH + (warp * 8 + gr) * 4;
-        const uint8_t* srow = tile + 2 * t * PITCH + tail + 2 * warp;
-#pragma unroll
-        for (int ks = 0; ks < LD_TILE / 16; ++ks) {
-          const uint4 pa = pb[ks][lane];
-          uint32_t w[4], s[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int r = (16 * ks + (k & 1) + 8 * (k >> 1)) * PITCH;
-            w[k] = *(const uint32_t*)(col + r);
-            s[k] = *(const uint16_t*)(srow + r);
-          }
-          const uint32_t sa = s[0] | s[1] << 16, sb = s[2] | s[3] << 16;
-          const __half2 sa2 = *(const __half2*)&sa, sb2 = *(const __half2*)&sb;
-          const __half2 ca2 = __hmul2(sa2, __float2half2_rn(-24.f)), cb2 = __hmul2(sb2, __float2half2_rn(-24.f));
-          // halves of two rows' words side by side: values 2 j in the low ones, 2 j + 1 in the high ones
-          const uint32_t al = __byte_perm(w[0], w[1], 0x5410), ah = __byte_perm(w[0], w[1], 0x7632);
-          const uint32_t bl = __byte_perm(w[2], w[3], 0x5410), bh = __byte_perm(w[2], w[3], 0x7632);
-          mma16816(o[0], pa, ln_pair<0>(al, sa2, ca2), ln_pair<0>(bl, sb2, cb2));
-          mma16816(o[1], pa, ln_pair<0>(ah, sa2, ca2), ln_pair<0>(bh, sb2, cb2));
-          mma16816(o[2], pa, ln_pair<1>(al, sa2, ca2), ln_pair<1>(bl, sb2, cb2));
-          mma16816(o[3], pa, ln_pair<1>(ah, sa2, ca2), ln_pair<1>(bh, sb2, cb2));
-          mma16816(o[4], pa, ln_pair<2>(al, sa2, ca2), ln_pair<2>(bl, sb2, cb2));
-          mma16816(o[5], pa, ln_pair<2>(ah, sa2, ca2), ln_pair<2>(bh, sb2, cb2));
-          mma16816(o[6], pa, ln_pair<3>(al, sa2, ca2), ln_pair<3>(bl, sb2, cb2));
-          mma16816(o[7], pa, ln_pair<3>(ah, sa2, ca2), ln_pair<3>(bh, sb2, cb2));
-        }
-      }
-      if (i + 1 == count || p.tile + 1 == p.tiles) {
-        // ---------------- this block's part of the query block
-        const size_t slot = (size_t)item + blockIdx.x;
-        if (warp < NL) {
-          float* dst = g.part + (slot * L + (warp * 8 + 2 * t) * 8) * LN_ROWS + gr;
-#pragma unroll
-          for (int v = 0; v < 8; ++v)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) dst[((k & 1) * 8 + v) * LN_ROWS + 8 * (k >> 1)] = o[v][k];
-        }
-        ln_sync();                     // the maxima's place is free
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float s = l[k] + __shfl_xor_sync(0xffffffffu, l[k], 1);
-          s += __shfl_xor_sync(0xffffffffu, s, 2);
-          if (t == 0) sh->red[warp][gr + 8 * k] = s;
-        }
-        ln_sync();
-        if (warp == 0 && t == 0)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float s = 0.f;
-#pragma unroll
-            for (int w = 0; w < LN_WARPS; ++w) s += sh->red[w][gr + 8 * k];
-            g.ml[slot * LN_ROWS + gr + 8 * k] = make_float2(ref[k], s);
-          }
-        ln_sync();
-      }
       p.next(g);
     }
   }
