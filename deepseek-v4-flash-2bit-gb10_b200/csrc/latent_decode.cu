@@ -502,11 +502,12 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
 
 // Query rows a block, by the rows of a sequence. Up to 16 the narrow kernel; up to 32, or more, the wide one with that many
 // (64 sequences, 320,206 cached rows: 16 query rows 84 us narrow, 151 us with 64 wide; 32 rows 122 us with 32 wide, 141 us as two
-// narrow blocks, 151 us with 64 wide; 48 rows 158 us with 64 wide, 201 us narrow). Where every tile of every 16 rows has a block of
-// its own at once, time is latency, and the narrow kernel has less of it (64 rows, 64 cached: 11 us, 18 us wide).
+// narrow blocks, 151 us with 64 wide; 48 rows 158 us with 64 wide, 201 us narrow). Where the narrow kernel's blocks have at most 5
+// tiles each, time is mostly latency, and it has less of it (64 rows of 8 sequences: 2048 cached rows each 31 us, 36 us wide;
+// 4096 each 43 and 42 us; 64 rows of one sequence, 64 cached: 11 and 18 us).
 static int ld_nq(int B, int T, int heads, long long most) {
   const long long rows = (long long)T * heads;
-  return rows <= 16 || (double)B * ((most + LD_TILE - 1) / LD_TILE) * ((rows + 15) / 16) <= 2 * 148 ? 16 : rows <= 32 ? 32 : 64;
+  return rows <= 16 || (double)B * ((most + LD_TILE - 1) / LD_TILE) * ((rows + 15) / 16) <= 5 * 2 * 148 ? 16 : rows <= 32 ? 32 : 64;
 }
 
 struct LdLayout {

@@ -126,7 +126,7 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
   const int per = a.heads * a.B;
   const int qb = nqb - 1 - (int)(blockIdx.x / per), h = (int)(blockIdx.x % per) % a.heads, b = (int)(blockIdx.x % per) / a.heads;
   // offsets are clamped to the tensors, so wrong ones give wrong rows and no access out of range
-  const int q0 = min(max(a.cu_q[b], 0), a.total_q), nq = min(min(max(a.cu_q[b + 1], q0), a.total_q) - q0, a.max_q);
+  const int q0 = min(max(a.cu_q[b], 0), a.total_q), nq = min(max(a.cu_q[b + 1], q0), a.total_q) - q0;
   const int k0 = min(max(a.cu_k[b], 0), a.total_k), nk = min(max(a.cu_k[b + 1], k0), a.total_k) - k0;
   const int row0 = qb * 2 * LP_TILE;
   if (row0 >= nq) return;
@@ -217,7 +217,9 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
       // ---------------- products: one thread issues them all
       constexpr uint32_t fmt = DT == VQ2_DT_BF16 ? (1u << 7) | (1u << 10) : 0u;
       constexpr uint32_t id_s = (1u << 4) | fmt | ((LP_TILE >> 3) << 17) | ((LP_TILE >> 4) << 24);
-      const uint32_t id_o = (1u << 4) | fmt | (1u << 16) | ((uint32_t)((a.v_dim + 15) / 16 * 2) << 17) | ((LP_TILE >> 4) << 24);
+      // whole units of values: columns past v_dim are zeros in V (a descriptor known at compile time is what lets a product be
+      // issued in 15 cycles)
+      constexpr uint32_t id_o = (1u << 4) | fmt | (1u << 16) | ((uint32_t)(VU * 64 >> 3) << 17) | ((LP_TILE >> 4) << 24);
       constexpr uint32_t U = LP_UNIT >> 4;
       const uint32_t qlo = (qbase >> 4) | 1u << 16, klo = (kring >> 4) | 1u << 16, vlo = (vring >> 4) | U << 16;
       const int lastt = ntile - 1;                  // it has the most steps

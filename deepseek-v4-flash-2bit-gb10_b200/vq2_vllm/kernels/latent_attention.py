@@ -69,11 +69,11 @@ def latent_attention_decode(q: torch.Tensor, cache: LatentCache, block_table: to
     return out
 
 
-def _heads(x: torch.Tensor, what: str, rows=None, heads=None):
-    """x [rows, heads, D], last dimension contiguous and the others in multiples of 16 bytes (copied if not)."""
-    if x.dim() != 3 or (rows is not None and x.shape[0] != rows) or (heads is not None and x.shape[1] != heads):
-        raise ValueError(f"vq2 latent attention: {what} must be [tokens, heads, dim]")
-    if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or min(x.stride()) < 1 or x.data_ptr() % 16:
+def _rows(x: torch.Tensor):
+    """x [tokens, .., dim] as the kernels can read it, last dimension contiguous and the others in multiples of 16
+    bytes (copied if not)."""
+    st = x.stride()
+    if st[-1] != 1 or min(st) < 1 or any(n % 8 for n in st[:-1]) or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     return x
 
@@ -94,7 +94,10 @@ def latent_attention_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_rope: torc
     if q.dim() != 3 or k_nope.dim() != 3 or v.dim() != 3:
         raise ValueError("vq2 latent attention: q, k_nope and v must be [tokens, heads, dim]")
     Tq, heads, dq = q.shape
-    Tk, dn, dv = k_nope.shape[0], k_nope.shape[2], v.shape[2]
+    Tk, _, dn = k_nope.shape
+    dv = v.shape[2]
+    if v.shape[:2] != k_nope.shape[:2] or k_nope.shape[1] != heads:
+        raise ValueError("vq2 latent attention: k_nope and v must be [key tokens, heads, dim] with q's heads")
     R = dq - dn
     if not (0 < dn <= MAX_HEAD_DIM and 0 < dv <= MAX_HEAD_DIM and 0 <= R <= MAX_ROPE) or dn % 8 or dv % 8 or R % 8:
         raise ValueError(f"vq2 latent attention: nope {dn} and v {dv} must be multiples of 8 up to {MAX_HEAD_DIM}, rope {R} one up "
@@ -114,9 +117,9 @@ def latent_attention_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_rope: torc
     if not out.numel() or not B:
         return out
     with _lib.on_device(dev):
-        q, k_nope, v = _heads(q, "q"), _heads(k_nope, "k_nope", Tk, heads), _heads(v, "v", Tk, heads)
+        q, k_nope, v = _rows(q), _rows(k_nope), _rows(v)
         if R:
-            k_rope = _heads(k_rope[:, None, :], "k_rope")
+            k_rope = _rows(k_rope)
         a = _lib.Vq2LatentPrefillArgs(B, heads, dn, R, dv, max_q, _DT[q.dtype], Tq, Tk, scale, q.stride(0), q.stride(1),
                                       k_nope.stride(0), k_nope.stride(1), v.stride(0), v.stride(1), k_rope.stride(0) if R else 0,
                                       q.data_ptr(), k_nope.data_ptr(), k_rope.data_ptr() if R else None, v.data_ptr(),

@@ -103,8 +103,8 @@ def latent_cache_read(cache: LatentCache, slots: torch.Tensor, dtype: torch.dtyp
     dev = cache.data.get_device()
     _lib.require_cuda(slots, device=dev)
     N = slots.shape[0]
-    c = torch.empty((N, cache.latent_dim), dtype=dtype, device=slots.device)
-    k_rope = torch.empty((N, cache.rope_dim), dtype=dtype, device=slots.device)
+    c = torch.empty(N, cache.latent_dim, dtype=dtype, device=slots.device)
+    k_rope = torch.empty(N, cache.rope_dim, dtype=dtype, device=slots.device)
     if N:
         with _lib.on_device(dev):
             rc = _lib.lib().vq2_latent_cache_read(cache.args, slots.data_ptr(), _lib.ID[slots.dtype], N, c.data_ptr(),
