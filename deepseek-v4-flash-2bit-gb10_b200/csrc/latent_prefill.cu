@@ -145,6 +145,11 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
   const uint32_t qbase = smem_u32(smem), kring = qbase + 6 * LP_UNIT, vring = kring + LP_KUNITS * LP_UNIT;
   LpShared* sh = (LpShared*)(smem + (6 + LP_KUNITS + LP_VUNITS) * LP_UNIT);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  if (threadIdx.x == 32) {
+    // the first copy through a tensor map would wait for the map itself
+    asm volatile("prefetch.tensormap [%0];\n prefetch.tensormap [%1];\n prefetch.tensormap [%2];\n prefetch.tensormap [%3];"
+                 ::"l"(&tq), "l"(&tk), "l"(&tr), "l"(&tv) : "memory");
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < LP_KMAX; ++s) { mbar_init(&sh->kfull[s], 1); mbar_init(&sh->kempty[s], 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(&sh->vfull[s], 1); mbar_init(&sh->vempty[s], 1); }
@@ -172,7 +177,7 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
   volatile int* abort = &sh->abort;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0 && nsteps > 0 && elect_one()) {
       // ---------------- loader
       for (int t = 0; t < ntile; ++t) {
@@ -291,7 +296,7 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
     }
   } else {
     // ---------------- softmax: thread = query row
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int t = (warp - 4) >> 2, r = (warp & 3) * 32 + lane, i = row0 + t * LP_TILE + r;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * 128;
