@@ -193,7 +193,8 @@ __global__ void __launch_bounds__(WARPS * 32) latent_join_kernel(LdArgs g) {
   const int r0 = blockIdx.x % (NQ / 8) * 8, d0 = blockIdx.x / (NQ / 8) % (L / 64) * 64, item = blockIdx.x / (NQ / 8) / (L / 64);
   const int b = item / g.nrb, rb = item % g.nrb;
   if (rb * NQ + r0 >= rows) return;
-  const int total = g.start[a.B], s0 = g.start[b], s1 = g.start[b + 1];
+  // (reads through L2: this kernel may have started while the main one was still writing)
+  const int total = __ldcg(g.start + a.B), s0 = __ldcg(g.start + b), s1 = __ldcg(g.start + b + 1);
   const int quota = max(1, (total + g.grid - 1) / g.grid), tiles = (s1 - s0) / g.nrb;
   const int begin = s0 + rb * tiles, c0 = begin / quota, c1 = tiles ? (begin + tiles - 1) / quota : c0 - 1;
   float m[8], l[8], v[2][8];
@@ -210,12 +211,12 @@ __global__ void __launch_bounds__(WARPS * 32) latent_join_kernel(LdArgs g) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const float4* p = (const float4*)(g.part + (at * L + d0 + lane + 32 * k) * NQ + r0);
-      const float4 y = __ldg(p), z = __ldg(p + 1);
+      const float4 y = __ldcg(p), z = __ldcg(p + 1);
       x[k][0] = y.x; x[k][1] = y.y; x[k][2] = y.z; x[k][3] = y.w;
       x[k][4] = z.x; x[k][5] = z.y; x[k][6] = z.z; x[k][7] = z.w;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ml[i] = __ldg(g.ml + at * NQ + r0 + i);
+    for (int i = 0; i < 8; ++i) ml[i] = __ldcg(g.ml + at * NQ + r0 + i);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       // a part that saw nothing has maximum -inf and, unless it met a NaN, denominator 0: it changes nothing, a NaN all

@@ -211,10 +211,10 @@ __global__ void __launch_bounds__(LN_THREADS, 2) latent_decode_narrow_kernel(LdA
         item = p.b * g.nrb + p.rb;
         if (i == 0) pdl_wait();
         const uint4* src = (const uint4*)(g.q + (size_t)item * LN_ROWS * units * 128);
-        for (int u = tid; u < LN_ROWS * units * 8; u += LN_THREADS) ((uint4*)sh->q)[u] = src[u];
+        for (int u = tid; u < LN_ROWS * units * 8; u += LN_THREADS) ((uint4*)sh->q)[u] = __ldcg(src + u);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float2 m = g.meta[item * LN_ROWS + gr + 8 * k];
+          const float2 m = __ldcg(g.meta + item * LN_ROWS + gr + 8 * k);
           fac[k] = m.x;
           tok[k] = __float_as_int(m.y);
           l[k] = 0.f;
