@@ -187,11 +187,13 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0 && nsteps > 0 && elect_one()) {
       // ---------------- loader
-      for (int t = 0; t < ntile; ++t) {
+      auto queries = [&](int t) {
         mbar_arrive_expect_tx(&sh->qfull[t], KU * LP_UNIT);
+#pragma unroll
         for (int s = 0; s < KU; ++s)
           tma_load_3d(qbase + (t * 3 + s) * LP_UNIT, &tq, s < kn ? s * 64 : a.nope_dim, h, q0 + row0 + t * LP_TILE, &sh->qfull[t]);
-      }
+      };
+      queries(0);
       // keys of step j go out before the values of step j - 1: the scores of a step are computed first
       Ring<KS> rk;
       Ring<VS> rv;
@@ -207,6 +209,7 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
                         &sh->kfull[rk.stage]);
           rk.next();
           ++nkeys;
+          if (j == 0 && ntile > 1) queries(1);       // after the first keys: tile 0 starts on them
         }
         if (j > 0) {
           if (!(ok = mbar_wait(&sh->vempty[rv.stage], rv.parity ^ 1))) break;
@@ -382,14 +385,32 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
       const float l = l2.x + l2.y;
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
       const long long at = ((long long)(q0 + i) * a.heads + h) * a.v_dim;
-#pragma unroll 1
-      for (int c = 0; c < a.v_dim; c += 8) {
-        float o[8];
-        if (n > 0) tmem_ld8(to + c, o);
+      const bool sectors = a.v_dim % 16 == 0 && ((uintptr_t)a.out & 31) == 0;      // a thread's run as whole 32-byte sectors
+#pragma unroll
+      for (int u = 0; u < VU; ++u) {
+        float o[64];
+        if (n > 0) {
+          tmem_ld64(to + u * 64, o);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int k = 0; k < 64; ++k) asm volatile("" : "+f"(o[k]));
+        }
         if (i < nq) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) o[k] = n > 0 && l != 0.f ? o[k] * inv : 0.f;
-          store8<DT>(a.out, at + c, o);
+          for (int k = 0; k < 64; ++k) o[k] = n > 0 && l != 0.f ? o[k] * inv : 0.f;
+#pragma unroll
+          for (int c = 0; c < 64; c += 16) {
+            if (u * 64 + c >= a.v_dim) break;
+            if (sectors) {
+              uint32_t w[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) w[k] = pack2<DT>(o[c + 2 * k], o[c + 2 * k + 1]);
+              store_sector((uint16_t*)a.out + at + u * 64 + c, w);
+            } else {
+              store8<DT>(a.out, at + u * 64 + c, o + c);
+              if (u * 64 + c + 8 < a.v_dim) store8<DT>(a.out, at + u * 64 + c + 8, o + c + 8);
+            }
+          }
         }
       }
     }
