@@ -201,6 +201,8 @@ __device__ __forceinline__ void store_sector(void* p, const uint32_t* v) {
 // The inverse. A thread expands half a group (16 bytes of nibbles) and rotates it with its neighbour's half: one shuffle a value
 // (with a group over 8 lanes it is three, half the instructions), and few enough registers for 1280 threads an SM to cover the
 // two dependent reads. All rows' groups come first, then all rows' rotary parts, so that a warp has one kind of work.
+// Bound by memory latency: 65,536 rows of 512 + 64 values 32 us in calls back to back (49 with 8 lanes a group, 37 with a thread a
+// group), 27 us with other work between, 3.8 TB/s.
 template <int DT>
 __global__ void __launch_bounds__(LC_THREADS, 5) latent_read_kernel(const uint8_t* __restrict__ cache, const void* __restrict__ slots,
                                                                     int slot_dtype, uint32_t n, int L, int R, long long capacity,

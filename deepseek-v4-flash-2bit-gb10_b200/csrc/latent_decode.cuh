@@ -29,6 +29,7 @@ __device__ __forceinline__ void ld_wait(uint64_t* bar, uint32_t parity, volatile
       return;
     }
 }
+
 // Position of a tile: sequence, block of query rows, tile; the order is sequence, block, tile.
 struct LdPos {
   int b, rb, tile, len, tiles;

@@ -18,7 +18,7 @@
 // keys, so that O's products start under the second half's exponentials.
 // What bounds it: the products of a step (two tiles, 128 keys) take 2560 cycles, the step about 3400: 1700 for a
 // tile's softmax (1024 of them its exponentials) and the hand-overs before and after it, under which only the other tile's
-// products run. 8192 tokens, 32 heads, 128 + 64 and 128 values: 0.61 ms, 1120 TFLOP/s, at the power limit; the library's plain
+// products run. 8192 tokens, 32 heads, 128 + 64 and 128 values: 0.605 ms, 1135 TFLOP/s, at the power limit; the library's plain
 // bf16 product of 8192^3 sustains 1395 there.
 // A key that a row does not see has probability 0; a NaN or an infinity in its value reaches the row all the same (0 times
 // NaN) if both are in one step of 128 keys of one sequence, but never another sequence's rows.

@@ -40,7 +40,8 @@ def latent_attention_decode(q: torch.Tensor, cache: LatentCache, block_table: to
         out = sum_j softmax_j(scale * (q_c . c_j + q_r . r_j)) c_j,   j <= kv_len - T + t
 
     A sequence of length 0 (or a row that sees nothing) gives zeros; rows of the cache past kv_len are never
-    used, whatever they hold. Nothing waits for the host: safe to capture in a CUDA graph."""
+    used, whatever they hold. ``scale`` is positive. Three launches; nothing waits for the host: safe to capture in
+    a CUDA graph."""
     L, R = cache.latent_dim, cache.rope_dim
     if not scale > 0:
         raise ValueError("vq2 latent attention: scale must be positive")
@@ -85,7 +86,8 @@ def latent_attention_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_rope: torc
     contiguous last dimension are taken as they are) -> [Tq, heads, dv]. Sequence b has query rows
     cu_q[b] .. cu_q[b+1]-1 and key rows cu_k[b] .. cu_k[b+1]-1 (int32 [B+1] on the GPU): its keys are a prefix
     followed by the chunk's own, and query i sees keys up to i + keys - queries. ``max_q`` is the most query
-    rows a sequence has. A row that sees no key gives zeros. Dimensions are multiples of 8, nope and dv at
+    rows a sequence has; rows of ``q`` outside cu_q, or past max_q in their sequence, are left unset. A row that sees no
+    key gives zeros. ``scale`` is positive. Dimensions are multiples of 8, nope and dv at
     most 128, rope at most 64."""
     if q.dtype not in _DT:
         raise ValueError("vq2 latent attention: q must be bf16 or fp16")

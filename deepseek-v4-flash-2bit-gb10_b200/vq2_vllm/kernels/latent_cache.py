@@ -93,8 +93,8 @@ def latent_cache_write(cache: LatentCache, c: torch.Tensor, k_rope: torch.Tensor
 
 def latent_cache_read(cache: LatentCache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
     """The values that cache rows ``slots`` [N] stand for -> (c [N, latent_dim], k_rope [N, rope_dim]) of
-    ``dtype`` (bf16 / fp16 / fp32): what the expanded form projects up for a cached prefix. A negative slot
-    gives zeros."""
+    ``dtype`` (bf16 / fp16 / fp32): what the expanded form projects up for a cached prefix. A negative slot, or
+    one beyond the cache (reported by ``vq2_device_status``), gives zeros. N < 2^27."""
     dt = _lib.DT.get(dtype)
     if dt is None:
         raise ValueError("vq2 latent cache: dtype must be bf16, fp16 or fp32")

@@ -272,7 +272,7 @@ size_t vq2_latent_row_bytes(int latent_dim, int rope_dim);   /* 0 for unsupporte
 int vq2_latent_cache_write(const vq2_latent_cache* cache, const void* c, const void* k_rope, int dtype, long long c_stride,
                            long long rope_stride, const void* slots, int slot_dtype, int n, void* stream);
 /* What slots[i] stand for: c [n][L] (32-byte aligned) and k_rope [n][R] of VQ2_DT_* (zeros for a slot that write
-   skips). */
+   skips); n < 2^27. */
 int vq2_latent_cache_read(const vq2_latent_cache* cache, const void* slots, int slot_dtype, int n, void* c, void* k_rope,
                           int dtype, void* stream);
 
@@ -286,7 +286,7 @@ typedef struct vq2_latent_decode_args {
   int page_size, max_pages;      /* block_table is [B][max_pages] */
   int dtype;                     /* VQ2_DT_BF16 or VQ2_DT_F16, of q and out */
   long long pages;
-  float scale;
+  float scale;                   /* > 0 */
   const void* q;                 /* [B][T][heads][latent_dim + rope_dim] */
   const void* cache;
   const int32_t* block_table;
@@ -306,7 +306,7 @@ typedef struct vq2_latent_prefill_args {
   int B, heads, nope_dim, rope_dim, v_dim;   /* nope_dim, v_dim <= 128, rope_dim <= 64, multiples of 8 */
   int max_q, dtype;                          /* VQ2_DT_BF16 or VQ2_DT_F16 */
   int total_q, total_k;                      /* rows of q and of k_nope / k_rope / v */
-  float scale;
+  float scale;                               /* > 0 */
   long long q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, r_stride_t;
   const void* q;                             /* [total_q][heads][nope_dim + rope_dim] */
   const void* k_nope;                        /* [total_k][heads][nope_dim] */
