@@ -16,12 +16,15 @@
 // A row's maximum is refreshed only when it rose by more than 2^8 in the exponent: P then stays below
 // 256 (exact enough in 16 bits: the rounding is relative) and O is rarely rescaled. P goes over in halves of 64
 // keys, so that O's products start under the second half's exponentials.
+// Where there are fewer blocks of queries than SMs, a block's keys are split into parts, one CTA each, and a second kernel joins
+// them (below: lp_split).
 // What bounds it: the products of a step (two tiles, 128 keys) take 2560 cycles, the step about 3400: 1700 for a
 // tile's softmax (1024 of them its exponentials) and the hand-overs before and after it, under which only the other tile's
 // products run. 8192 tokens, 32 heads, 128 + 64 and 128 values: 0.605 ms, 1135 TFLOP/s, at the power limit; the library's plain
 // bf16 product of 8192^3 sustains 1395 there.
 // A key that a row does not see has probability 0; a NaN or an infinity in its value reaches the row all the same (0 times
 // NaN) if both are in one step of 128 keys of one sequence, but never another sequence's rows.
+#include <algorithm>
 #include <type_traits>
 #include "vq2_common.cuh"
 
@@ -123,25 +126,54 @@ struct Ring {
   }
 };
 
+// A block of queries: blocks are numbered (query block, sequence, head), the last query block of every head and sequence first,
+// as it has most keys. Offsets are clamped to the tensors, so wrong ones give wrong rows and no access out of range.
+struct LpBlock {
+  int h, b, q0, nq, k0, nk, row0, past, ntile, n0, n1, nsteps;
+  __device__ __forceinline__ bool at(const vq2_latent_prefill_args& a, int nqb, int block) {
+    const int per = a.heads * a.B;
+    h = block % per % a.heads;
+    b = block % per / a.heads;
+    q0 = min(max(a.cu_q[b], 0), a.total_q);
+    nq = min(max(a.cu_q[b + 1], q0), a.total_q) - q0;
+    k0 = min(max(a.cu_k[b], 0), a.total_k);
+    nk = min(max(a.cu_k[b + 1], k0), a.total_k) - k0;
+    row0 = (nqb - 1 - block / per) * 2 * LP_TILE;
+    if (row0 >= nq) return false;
+    past = nk - nq;                               // key i + past is the newest that query i sees
+    ntile = nq - row0 > LP_TILE ? 2 : 1;
+    // key steps of each tile, by its last row
+    n0 = (max(0, min(nk, min(nq, row0 + LP_TILE) + past)) + LP_TILE - 1) / LP_TILE;
+    n1 = ntile > 1 ? (max(0, min(nk, min(nq, row0 + 2 * LP_TILE) + past)) + LP_TILE - 1) / LP_TILE : 0;
+    nsteps = max(n0, n1);
+    return true;
+  }
+};
+
+// The key steps of a block in parts of `steps` steps (more where that would be over `most` parts), one CTA each. Of a block with
+// several parts each leaves its unnormalised rows and their maxima (in log2 units) and sums; slot = block * most + part, 256 rows.
+struct LpParts {
+  int most, steps;
+  float* o;
+  float2* ml;
+  __device__ __forceinline__ int length(int nsteps) const { return max(steps, (nsteps + most - 1) / most); }
+};
+
 // KU, VU: units of 64 values in a key row (positionless part, then rotary part) and in a value row.
 template <int DT, int KU, int VU>
 __global__ void __launch_bounds__(LP_THREADS, 1)
-latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, LpParts parts, const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                       const __grid_constant__ CUtensorMap tr, const __grid_constant__ CUtensorMap tv) {
   extern __shared__ __align__(1024) uint8_t lp_smem_raw[];
-  // block -> (sequence, head, query block): the last query block of every head and sequence first, as it has most keys
-  const int per = a.heads * a.B;
-  const int qb = nqb - 1 - (int)(blockIdx.x / per), h = (int)(blockIdx.x % per) % a.heads, b = (int)(blockIdx.x % per) / a.heads;
-  // offsets are clamped to the tensors, so wrong ones give wrong rows and no access out of range
-  const int q0 = min(max(a.cu_q[b], 0), a.total_q), nq = min(max(a.cu_q[b + 1], q0), a.total_q) - q0;
-  const int k0 = min(max(a.cu_k[b], 0), a.total_k), nk = min(max(a.cu_k[b + 1], k0), a.total_k) - k0;
-  const int row0 = qb * 2 * LP_TILE;
-  if (row0 >= nq) return;
-  const int past = nk - nq;                       // key i + past is the newest that query i sees
-  const int ntile = nq - row0 > LP_TILE ? 2 : 1;
-  // key steps of each tile, by its last row
-  const int n0 = (max(0, min(nk, min(nq, row0 + LP_TILE) + past)) + LP_TILE - 1) / LP_TILE;
-  const int n1 = ntile > 1 ? (max(0, min(nk, min(nq, row0 + 2 * LP_TILE) + past)) + LP_TILE - 1) / LP_TILE : 0;
+  LpBlock w;
+  if (!w.at(a, nqb, blockIdx.x)) return;
+  const int per_part = parts.length(w.nsteps), first = blockIdx.y * per_part;      // this CTA's first key step
+  if (first && first >= w.nsteps) return;
+  const bool whole = w.nsteps <= per_part;
+  // from here on keys and steps count from the part's first
+  const int h = w.h, q0 = w.q0, nq = w.nq, row0 = w.row0, ntile = w.ntile;
+  const int k0 = w.k0 + first * LP_TILE, nk = w.nk - first * LP_TILE, past = w.past - first * LP_TILE;
+  const int n0 = min(max(w.n0 - first, 0), per_part), n1 = min(max(w.n1 - first, 0), per_part);
   const int nsteps = max(n0, n1);
   const bool tail = nsteps * LP_TILE > nk;        // the last step's values end inside their units
   auto n_of = [&](int t) { return t ? n1 : n0; };
@@ -386,6 +418,8 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
       const long long at = ((long long)(q0 + i) * a.heads + h) * a.v_dim;
       const bool sectors = a.v_dim % 16 == 0 && ((uintptr_t)a.out & 31) == 0;      // a thread's run as whole 32-byte sectors
+      const size_t slot = ((size_t)blockIdx.x * parts.most + blockIdx.y) * (2 * LP_TILE) + t * LP_TILE + r;
+      if (!whole && i < nq) parts.ml[slot] = make_float2(m * sl, l);
 #pragma unroll
       for (int u = 0; u < VU; ++u) {
         float o[64];
@@ -395,7 +429,12 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
 #pragma unroll
           for (int k = 0; k < 64; ++k) asm volatile("" : "+f"(o[k]));
         }
-        if (i < nq) {
+        if (i < nq && !whole) {
+#pragma unroll
+          for (int k = 0; k < 64; ++k) o[k] = n > 0 ? o[k] : 0.f;
+#pragma unroll
+          for (int c = 0; c < 64; c += 8) store_sector(parts.o + slot * (VU * 64) + u * 64 + c, (const uint32_t*)(o + c));
+        } else if (i < nq) {
 #pragma unroll
           for (int k = 0; k < 64; ++k) o[k] = n > 0 && l != 0.f ? o[k] * inv : 0.f;
 #pragma unroll
@@ -421,6 +460,76 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, const __grid_constant_
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
+// Adds up the parts of the blocks that have several, in order, and divides. 16 threads a row, 8 values each.
+constexpr int LPJ_ROWS = 16;
+template <int DT, int VU>
+__global__ void __launch_bounds__(LPJ_ROWS * 16) latent_prefill_join_kernel(vq2_latent_prefill_args a, int nqb, LpParts parts) {
+  pdl_wait();
+  constexpr int per = 2 * LP_TILE / LPJ_ROWS;
+  const int block = blockIdx.x / per, r = blockIdx.x % per * LPJ_ROWS + threadIdx.x / 16, d = threadIdx.x % 16 * 8;
+  LpBlock w;
+  if (!w.at(a, nqb, block) || w.row0 + r >= w.nq || d >= a.v_dim) return;
+  const int len = parts.length(w.nsteps);
+  if (w.nsteps <= len) return;
+  const int count = (w.nsteps + len - 1) / len;
+  float n = -INFINITY, l = 0.f, v[8] = {};
+#pragma unroll 4
+  for (int s = 0; s < count; ++s) {
+    // (reads through L2: this kernel may have started while the main one was still writing)
+    const size_t slot = ((size_t)block * parts.most + s) * (2 * LP_TILE) + r;
+    const float2 ml = __ldcg(parts.ml + slot);
+    const float4* p = (const float4*)(parts.o + slot * (VU * 64) + d);
+    const float4 x = __ldcg(p), y = __ldcg(p + 1);
+    if (ml.y == 0.f) continue;                    // the row saw no key of this part
+    const float mx = fmaxf(n, ml.x), f = n == mx ? 1.f : ex2(n - mx), e = ml.x == mx ? 1.f : ex2(ml.x - mx);
+    n = mx;
+    l = l * f + ml.y * e;
+    const float z[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = v[k] * f + z[k] * e;
+  }
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = l != 0.f ? v[k] * inv : 0.f;
+  store8<DT>(a.out, ((long long)(w.q0 + w.row0 + r) * a.heads + w.h) * a.v_dim + d, v);
+}
+
+// How the keys are split: not at all where there is a block of queries for every SM; else in the parts that the sizes (sequences taken
+// as alike) say are soonest done. A part takes LP_FIXED steps beside its keys, the join LP_JOIN; a schedule ends no later than full
+// rounds of parts over the SMs, nor than an even share of all steps and one part more. Whole and split, us on the device, 128 + 64 and
+// 128 values: 256 queries after 512, 8 heads 18 and 15; after 4,000, 32 heads 74 and 36; 1,024 after 15,000, 20 heads 241 and 195;
+// 1,024 alone, 16 heads 21 and 20; 8,192 alone, 1 head 111 and 34, 4 heads 115 and 97. Where the rule leaves them whole: 512 alone, 8
+// heads 14.1; 2,048 alone, 16 heads 35. At most 3 parts an SM: the workspace stays under 60 MB.
+constexpr int LP_FIXED = 3, LP_JOIN = 3;          // in key steps (1.8 us)
+static LpParts lp_split(const vq2_latent_prefill_args& a, int nqb, int sms) {
+  LpParts s = {1, 1 << 30, nullptr, nullptr};
+  const long long per = (long long)a.heads * a.B, blocks = nqb * per;
+  if (blocks >= sms) return s;
+  const int keys = a.total_k / a.B, prefix = std::max(0, (a.total_k - a.total_q) / a.B);
+  auto steps_of = [&](int qb) { return (int)((std::min<long long>(keys, prefix + (qb + 1LL) * 2 * LP_TILE) + LP_TILE - 1) / LP_TILE); };
+  const int longest = steps_of(nqb - 1);
+  long long best = longest + LP_FIXED;
+  for (int most = 2; most <= longest && most * blocks <= 3 * sms; ++most) {
+    const int len = (longest + most - 1) / most;
+    long long all = 0, work = 0;
+    for (int qb = 0; qb < nqb; ++qb) {
+      all += std::max(1, (steps_of(qb) + len - 1) / len) * per;
+      work += steps_of(qb) * per;
+    }
+    const long long rounds = (all + sms - 1) / sms * (len + LP_FIXED), even = (work + all * LP_FIXED) / sms + len + LP_FIXED;
+    const long long cost = std::min(rounds, even) + LP_JOIN;
+    if (cost < best) {
+      best = cost;
+      s.most = most;
+      s.steps = len;
+    }
+  }
+  return s;
+}
+static size_t lp_part_rows(const vq2_latent_prefill_args& a, int nqb, const LpParts& s) {
+  return s.most > 1 ? (size_t)nqb * a.heads * a.B * s.most * 2 * LP_TILE : 0;
+}
+
 // Tensor map of [rows][heads][dim] 16-bit values with element strides: boxes of 64 values x 1 head x 128 rows.
 static int lp_encode(CUtensorMap* m, const void* base, int dim, int heads, int rows, long long stride_h, long long stride_t) {
   if (const int rc = tensor_map_ready()) return rc;
@@ -438,6 +547,20 @@ static int lp_encode(CUtensorMap* m, const void* base, int dim, int heads, int r
 
 using namespace vq2;
 
+static int lp_nqb(int max_q) { return (int)((max_q + 2LL * LP_TILE - 1) / (2 * LP_TILE)); }
+
+extern "C" size_t vq2_latent_prefill_workspace_size(int B, int heads, int v_dim, int max_q, int total_q, int total_k) {
+  if (B <= 0 || heads <= 0 || v_dim <= 0 || v_dim > LP_MAX_D || max_q <= 0 || total_q < 0 || total_k < 0) return 0;
+  vq2_latent_prefill_args a = {};
+  a.B = B;
+  a.heads = heads;
+  a.total_q = total_q;
+  a.total_k = total_k;
+  const int nqb = lp_nqb(max_q);
+  const size_t rows = lp_part_rows(a, nqb, lp_split(a, nqb, 148));
+  return rows ? rows * ((v_dim + 63) / 64 * 64 * 4 + 8) + 256 : 0;
+}
+
 extern "C" int vq2_latent_prefill(const vq2_latent_prefill_args* a, void* stream) {
   if (!a) return VQ2_ERR_NULL;
   if (a->B <= 0 || a->heads <= 0 || a->max_q < 0 || a->total_q < 0 || a->total_k < 0 || a->nope_dim <= 0 || a->nope_dim > LP_MAX_D ||
@@ -451,7 +574,7 @@ extern "C" int vq2_latent_prefill(const vq2_latent_prefill_args* a, void* stream
   if (!a->q || !a->cu_q || !a->cu_k || !a->out) return VQ2_ERR_NULL;
   if (a->total_k && (!a->k_nope || !a->v || (a->rope_dim && !a->k_rope))) return VQ2_ERR_NULL;
   if (((uintptr_t)a->q | (uintptr_t)a->k_nope | (uintptr_t)a->v | (uintptr_t)a->k_rope | (uintptr_t)a->out) & 15) return VQ2_ERR_ALIGN;
-  const int nqb = (a->max_q + 2 * LP_TILE - 1) / (2 * LP_TILE);
+  const int nqb = lp_nqb(a->max_q);
   const long long blocks = (long long)nqb * a->heads * a->B;
   if (blocks > 0x7FFFFFFFLL) return VQ2_ERR_SHAPE;
   CUtensorMap tq, tk, tr, tv;
@@ -464,10 +587,33 @@ extern "C" int vq2_latent_prefill(const vq2_latent_prefill_args* a, void* stream
   if (!rc && any && a->rope_dim) rc = lp_encode(&tr, a->k_rope, a->rope_dim, 1, a->total_k, 0, a->r_stride_t);
   if (rc) return rc;
   const int ku = (a->nope_dim + 63) / 64 + (a->rope_dim ? 1 : 0), vu = (a->v_dim + 63) / 64;
+  LpParts parts = lp_split(*a, nqb, 148);
+  const size_t rows = lp_part_rows(*a, nqb, parts), need = rows * (vu * 64 * 4 + 8) + 256;
+  if (rows && a->workspace && a->ws_bytes >= need) {
+    parts.o = (float*)(((uintptr_t)a->workspace + 255) & ~(uintptr_t)255);
+    parts.ml = (float2*)(parts.o + rows * vu * 64);
+  } else {
+    parts = {1, 1 << 30, nullptr, nullptr};
+  }
+  auto join = [&] {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.stream = (cudaStream_t)stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cfg.gridDim = dim3((unsigned)(blocks * (2 * LP_TILE / LPJ_ROWS)));
+    cfg.blockDim = dim3(LPJ_ROWS * 16);
+    auto kernel = a->dtype == VQ2_DT_BF16 ? (vu == 1 ? latent_prefill_join_kernel<VQ2_DT_BF16, 1> : latent_prefill_join_kernel<VQ2_DT_BF16, 2>)
+                                          : (vu == 1 ? latent_prefill_join_kernel<VQ2_DT_F16, 1> : latent_prefill_join_kernel<VQ2_DT_F16, 2>);
+    return cudaLaunchKernelEx(&cfg, kernel, *a, nqb, parts) == cudaSuccess ? VQ2_OK : VQ2_ERR_CUDA;
+  };
   auto launch = [&](auto kernel, bool* raised) {
     if (!smem_limit_once(kernel, LP_SMEM, raised)) return VQ2_ERR_CUDA;
-    kernel<<<(unsigned)blocks, LP_THREADS, LP_SMEM, (cudaStream_t)stream>>>(*a, nqb, tq, tk, tr, tv);
-    return cudaGetLastError() == cudaSuccess ? VQ2_OK : VQ2_ERR_CUDA;
+    kernel<<<dim3((unsigned)blocks, parts.most), LP_THREADS, LP_SMEM, (cudaStream_t)stream>>>(*a, nqb, parts, tq, tk, tr, tv);
+    if (cudaGetLastError() != cudaSuccess) return VQ2_ERR_CUDA;
+    return parts.most > 1 ? join() : VQ2_OK;
   };
   auto pick = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;

@@ -55,7 +55,8 @@ class Vq2LatentPrefillArgs(ctypes.Structure):
                 + [("scale", ctypes.c_float)]
                 + [(n, ctypes.c_longlong) for n in ("q_stride_t", "q_stride_h", "k_stride_t", "k_stride_h", "v_stride_t",
                                                     "v_stride_h", "r_stride_t")]
-                + [(n, ctypes.c_void_p) for n in ("q", "k_nope", "k_rope", "v", "cu_q", "cu_k", "out")])
+                + [(n, ctypes.c_void_p) for n in ("q", "k_nope", "k_rope", "v", "cu_q", "cu_k", "out", "workspace")]
+                + [("ws_bytes", ctypes.c_size_t)])
 
 
 _SIGS = {
@@ -123,6 +124,7 @@ _SIGS = {
     "vq2_latent_decode_workspace_size": (ctypes.c_size_t, [ctypes.c_int] * 5),
     "vq2_latent_decode": (ctypes.c_int, [ctypes.POINTER(Vq2LatentDecodeArgs), ctypes.c_void_p, ctypes.c_size_t,
                                          ctypes.c_void_p]),
+    "vq2_latent_prefill_workspace_size": (ctypes.c_size_t, [ctypes.c_int] * 6),
     "vq2_latent_prefill": (ctypes.c_int, [ctypes.POINTER(Vq2LatentPrefillArgs), ctypes.c_void_p]),
     "vq2_device_status": (ctypes.c_int, [ctypes.c_int]),
     "vq2_strerror": (ctypes.c_char_p, [ctypes.c_int]),

@@ -27,6 +27,11 @@ def _i32(t: torch.Tensor, dim: int, what: str):
 
 
 @functools.lru_cache(maxsize=1024)
+def _prefill_workspace_size(B: int, heads: int, dv: int, max_q: int, Tq: int, Tk: int) -> int:
+    return _lib.lib().vq2_latent_prefill_workspace_size(B, heads, dv, max_q, Tq, Tk)
+
+
+@functools.lru_cache(maxsize=1024)
 def _workspace_size(B: int, T: int, heads: int, L: int, R: int) -> int:
     return _lib.lib().vq2_latent_decode_workspace_size(B, T, heads, L, R)
 
@@ -122,10 +127,12 @@ def latent_attention_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_rope: torc
         q, k_nope, v = _rows(q), _rows(k_nope), _rows(v)
         if R:
             k_rope = _rows(k_rope)
+        stream, nb = _lib.raw_stream(dev), _prefill_workspace_size(B, heads, dv, max_q, Tq, Tk)
+        ws = _lib.workspace(nb, q.device, stream).data_ptr() if nb else None
         a = _lib.Vq2LatentPrefillArgs(B, heads, dn, R, dv, max_q, _DT[q.dtype], Tq, Tk, scale, q.stride(0), q.stride(1),
                                       k_nope.stride(0), k_nope.stride(1), v.stride(0), v.stride(1), k_rope.stride(0) if R else 0,
                                       q.data_ptr(), k_nope.data_ptr(), k_rope.data_ptr() if R else None, v.data_ptr(),
-                                      cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr())
-        rc = _lib.lib().vq2_latent_prefill(a, _lib.raw_stream(dev))
+                                      cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(), ws, nb)
+        rc = _lib.lib().vq2_latent_prefill(a, stream)
     _lib.check(rc, "vq2_latent_prefill")
     return out

@@ -301,7 +301,8 @@ int vq2_latent_decode(const vq2_latent_decode_args* a, void* workspace, size_t w
    the chunk's own): query i sees keys j <= i + keys - queries, so the last query sees all; a row that
    sees nothing gives zeros. Key of head h: [k_nope[:, h], k_rope], the rotary part shared by the heads.
    Strides in elements (multiples of 8; the last dimension is contiguous); max_q >= every
-   sequence's query rows. */
+   sequence's query rows. With a workspace of the size below, calls with few blocks of queries split their
+   keys over the SMs; without one (or where that size is 0) they do not. */
 typedef struct vq2_latent_prefill_args {
   int B, heads, nope_dim, rope_dim, v_dim;   /* nope_dim, v_dim <= 128, rope_dim <= 64, multiples of 8 */
   int max_q, dtype;                          /* VQ2_DT_BF16 or VQ2_DT_F16 */
@@ -315,7 +316,10 @@ typedef struct vq2_latent_prefill_args {
   const int32_t* cu_q;                       /* [B + 1] */
   const int32_t* cu_k;                       /* [B + 1] */
   void* out;                                 /* [total_q][heads][v_dim] */
+  void* workspace;                           /* may be null */
+  size_t ws_bytes;
 } vq2_latent_prefill_args;
+size_t vq2_latent_prefill_workspace_size(int B, int heads, int v_dim, int max_q, int total_q, int total_k);
 int vq2_latent_prefill(const vq2_latent_prefill_args* a, void* stream);
 
 /* Error word written by bounded device waits and device-side range checks (0 = none);

@@ -404,3 +404,62 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="no CPU path"):
         latent_attention_prefill(p, k, r, v, cu.cpu(), cu, 4, 1.0)
     assert latent_attention_prefill(p[:0], k, r, v, cu * 0, cu, 0, 1.0).shape == (0, 2, 128)
+
+
+# ------------------------------------------------------------------------------------ keys split over blocks
+# The parts' sums are held and joined in fp32: a value takes at most 64 parts' factors and sums, 3 roundings of 2^-24 each, and its
+# denominator the same, under 2^-16 of A in all: half of it beside the 1e-5 that the bound has for sums already. P is
+# rounded relative to itself, whatever maximum it is held against, so its term does not change.
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("qlens,prefix,heads,dn,R,dv", [
+    ([1], [5000], 1, 128, 64, 128),
+    ([64], [4000], 3, 128, 64, 128),
+    ([129], [3001], 2, 96, 32, 96),
+    ([300], [2900], 4, 64, 0, 64),
+    ([2000], [0], 1, 128, 64, 128),                     # blocks from one part to many
+    ([1, 0, 200], [3000, 700, 9], 2, 128, 64, 72),      # one sequence far longer than the others
+    ([5, 7], [6000, 0], 1, 64, 16, 128),
+])
+def test_prefill_with_split_keys(dtype, qlens, prefix, heads, dn, R, dv):
+    from vq2_vllm import _lib
+    klens = [n + p for n, p in zip(qlens, prefix)]
+    assert _lib.lib().vq2_latent_prefill_workspace_size(len(qlens), heads, dv, max(qlens), sum(qlens), sum(klens)) > 0
+    _prefill_case(qlens, prefix, heads, dn, R, dv, dtype, seed=sum(klens) + heads)
+
+
+@pytest.mark.parametrize("q_scale", [1e-3, 10.0, 100.0])
+def test_split_keys_over_flat_and_peaked_rows(q_scale):
+    _prefill_case([140], [4000], 2, 128, 64, 128, "bf16", 81, q_scale=q_scale)
+
+
+def test_split_keys_rows_that_see_nothing():
+    """Rows before the first key give zeros, also where their block has keys in several parts."""
+    out = _prefill_case([2400], [-100], 1, 128, 64, 128, "bf16", 82)[-1]
+    assert not out[:100].any()
+
+
+def test_split_keys_keep_nan_where_it_is_seen():
+    """A NaN value reaches the rows that see it and, from another step, no other; a graph gives the same bits."""
+    from vq2_vllm.kernels.latent_attention import latent_attention_prefill
+    q, kn, kr, v, cu_q, cu_k, scale, out = _prefill_case([600], [2000], 2, 128, 64, 128, "bf16", 83)
+    v = v.clone()
+    v[2432] = math.nan                                  # the first key of a step; rows from 432 on see it
+    got = latent_attention_prefill(q, kn, kr, v, cu_q, cu_k, 600, scale)
+    assert torch.equal(got[:256], out[:256]) and got[432:].isnan().all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = latent_attention_prefill(q, kn, kr, v, cu_q, cu_k, 600, scale)
+    graph.replay()
+    assert torch.equal(again.nan_to_num(7.0), got.nan_to_num(7.0))
+
+
+def test_prefill_without_workspace_agrees():
+    """The C call without a workspace does not split and agrees to the roundings of the output and of P."""
+    from vq2_vllm import _lib
+    q, kn, kr, v, cu_q, cu_k, scale, out = _prefill_case([200], [3000], 2, 128, 64, 128, "f16", 84)
+    whole = torch.empty_like(out)
+    a = _lib.Vq2LatentPrefillArgs(1, 2, 128, 64, 128, 200, 1, len(q), len(v), scale, q.stride(0), q.stride(1), kn.stride(0), kn.stride(1),
+                                  v.stride(0), v.stride(1), kr.stride(0), q.data_ptr(), kn.data_ptr(), kr.data_ptr(), v.data_ptr(),
+                                  cu_q.data_ptr(), cu_k.data_ptr(), whole.data_ptr())
+    assert _lib.lib().vq2_latent_prefill(a, torch.cuda.current_stream().cuda_stream) == 0
+    assert (whole.double() - out.double()).norm() <= 4 * 2.0 ** -11 * out.double().norm()
