@@ -190,10 +190,19 @@ def require_cuda(*ts, device: int = -1):
 
 
 _WS = {}
+_WS_CAPTURED = {}          # buffers that a graph may write to, by id
+
+
+def held(buf: torch.Tensor) -> torch.Tensor:
+    """A cached workspace that is about to be used: kept for good where the stream is being captured, since the graph has its
+    address and a later, larger call must not free it."""
+    if torch.cuda.is_current_stream_capturing():
+        _WS_CAPTURED[id(buf)] = buf
+    return buf
 
 
 def workspace(nbytes: int, device, stream=None) -> torch.Tensor:
-    """Cached per-(device, stream) byte workspace, grown on demand (graph-safe once sized)."""
+    """Cached per-(device, stream) byte workspace, grown on demand (what a graph was captured with stays, see ``held``)."""
     if stream is None:
         stream = torch.cuda.current_stream(device).cuda_stream
     key = (device.index if isinstance(device, torch.device) else device, stream)
@@ -201,7 +210,7 @@ def workspace(nbytes: int, device, stream=None) -> torch.Tensor:
     if buf is None or buf.numel() < nbytes:
         buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
         _WS[key] = buf
-    return buf
+    return held(buf)
 
 
 _TLS = threading.local()

@@ -34,6 +34,7 @@ def router_topk(x: torch.Tensor, w_r: torch.Tensor, k: int):
     if ws is None or ws.numel() < need:
         ws = torch.empty(max(need, 1 << 20), dtype=torch.uint8, device=x.device)
         _WS[key] = ws
+    _lib.held(ws)
     _lib.check(L.vq2_router_topk(x.data_ptr(), _lib.DT[x.dtype], w_r.data_ptr(), N, H, E, k, ids.data_ptr(),
                                  wts.data_ptr(), ws.data_ptr(), ws.numel(), stream), "vq2_router_topk")
     return ids, wts

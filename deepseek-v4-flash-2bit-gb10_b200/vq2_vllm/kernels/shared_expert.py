@@ -42,6 +42,7 @@ def shared_expert_fused(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, ou
         if ws is None or ws.numel() < need:
             ws = torch.empty(max(need, 1 << 16), dtype=torch.uint8, device=x.device)
             _WS[key] = ws
+        _lib.held(ws)
         _lib.check(L.vq2_shared_expert(x.data_ptr(), _lib.DT[x.dtype], w13.data_ptr(), w2.data_ptr(), N, H, Is,
                                        out.data_ptr(), int(acc), ws.data_ptr(), ws.numel(), stream),
                    "vq2_shared_expert")

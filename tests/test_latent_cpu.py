@@ -102,3 +102,24 @@ def test_c_entries_reject_bad_arguments_without_a_gpu():
     assert prefill(nope_dim=136) == 2 and prefill(v_dim=4) == 2 and prefill(rope_dim=72) == 2 and prefill(B=0) == 2 and prefill(max_q=-1) == 2
     assert prefill(k_stride_h=127) == 2 and prefill(r_stride_t=4) == 2
     assert prefill(v=fake + 8) == 3 and prefill(dtype=2) == 4 and prefill(max_q=0) == 0
+
+
+def test_a_captured_workspace_outlives_a_larger_one(monkeypatch):
+    """A graph keeps the address of the workspace it was captured with: a later, larger call on the stream takes a new buffer
+    and leaves that one alone. A buffer that no graph has is let go."""
+    import weakref
+
+    import torch
+    from vq2_vllm import _lib
+    monkeypatch.setattr(_lib, "_WS", {})
+    capturing = True
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    dev, stream = torch.device("cpu"), -12345
+    first = weakref.ref(_lib.workspace(1 << 20, dev, stream))
+    again = weakref.ref(_lib.workspace(1 << 19, dev, stream))
+    assert again() is first()
+    capturing = False
+    second = weakref.ref(_lib.workspace(1 << 21, dev, stream))
+    assert first() is not None and second() is not first()
+    _lib.workspace(1 << 22, dev, stream)
+    assert second() is None and first() is not None

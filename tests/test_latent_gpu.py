@@ -463,3 +463,29 @@ def test_prefill_without_workspace_agrees():
                                   cu_q.data_ptr(), cu_k.data_ptr(), whole.data_ptr())
     assert _lib.lib().vq2_latent_prefill(a, torch.cuda.current_stream().cuda_stream) == 0
     assert (whole.double() - out.double()).norm() <= 4 * 2.0 ** -11 * out.double().norm()
+
+
+def test_graphs_of_growing_sizes_keep_their_workspaces():
+    """Graphs captured for growing batches replay right after the stream's workspace has grown past the first one's."""
+    from vq2_vllm.kernels.latent_attention import latent_attention_decode
+    from vq2_vllm.kernels.latent_cache import LatentCache, latent_cache_write
+    g = _gen(91)
+    cache = LatentCache.alloc(40, 64, 512, 64)
+    latent_cache_write(cache, torch.randn(2560, 512, generator=g, device="cuda").bfloat16(),
+                       torch.randn(2560, 64, generator=g, device="cuda").bfloat16(), torch.arange(2560, device="cuda"))
+    made = []
+    for B in (1, 8, 96):
+        q = torch.randn(B, 1, 64, 576, generator=g, device="cuda").bfloat16()
+        table = torch.stack([torch.randperm(40, generator=g, device="cuda") for _ in range(B)]).int()
+        n = torch.randint(1, 2561, (B,), generator=g, device="cuda").int()
+        want = latent_attention_decode(q, cache, table, n, 0.05)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = latent_attention_decode(q, cache, table, n, 0.05)
+        made.append((graph, out, want, q, table, n))
+    others = [torch.full((1 << 20,), 7.0, device="cuda") for _ in range(64)]       # takes any memory let go
+    for graph, out, want, *_ in made:
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)
+    assert all((t == 7.0).all() for t in others)
