@@ -10,7 +10,7 @@
 //   O^T [L x NQ]        += V^T P^T     the same tile read along the other direction (MN-major): the
 //                                      latent is key and value, expanded from 4 bits once for both
 // A row is held as n s in fp16, which is exact (|n| <= 7, s has 8 significant bits), q in fp16 with a
-// power-of-two scale a row, P in fp16 with its largest values between 2^5 and 2^15, so that values down to
+// power-of-two scale a row (fp16 queries in two such terms, both into the same S: see the query kernel), P in fp16 with its largest values between 2^5 and 2^15, so that values down to
 // 2^-29 of the largest still count; sums are fp32 in tensor memory.
 //
 // Work: the (sequence, block of NQ query rows, tile of 64 cached rows) triples in order, split evenly over one
@@ -42,8 +42,10 @@ constexpr float LD_BIAS = 5.f, LD_RAISE = 10.f;    // P = 2^(z - m + BIAS); m is
 constexpr int LD_PARTS = 2;             // of a tile: four units each, the last with the rotary unit
 constexpr int LD_RAW = LD_TILE * 400;   // a tile's raw rows (at most 400 bytes each)
 // Tiles and raw tiles that fit beside Q (NQ x 1152 bytes) in 227 KB.
-template <int NQ> constexpr int LD_TILES = NQ == 64 ? 1 : 2;
-template <int NQ> constexpr int LD_RAWS = NQ == 64 ? 3 : 1;
+// (TWO: fp16 query rows in two terms, 32 of them.)
+template <int NQ, bool TWO> constexpr int LD_TILES = NQ == 64 || TWO ? 1 : 2;
+template <int NQ, bool TWO> constexpr int LD_RAWS = NQ == 64 || TWO ? 3 : 1;
+template <int NQ, bool TWO> constexpr int LD_QBYTES = LD_UNITS * NQ * 128 * (TWO ? 2 : 1);
 
 template <int NQ>
 struct LdShared {
@@ -61,9 +63,11 @@ struct LdShared {
   float lsum[4][NQ];
   int scan[LD_WARPS];
 };
-template <int NQ>
-constexpr size_t ld_smem() { return (size_t)LD_TILES<NQ> * LD_KBYTES + (size_t)LD_RAWS<NQ> * LD_RAW + (size_t)LD_UNITS * NQ * 128 + sizeof(LdShared<NQ>) + 1024; }
-static_assert(ld_smem<64>() <= 227 * 1024 && ld_smem<32>() <= 227 * 1024, "latent decode shared memory");
+template <int NQ, bool TWO>
+constexpr size_t ld_smem() {
+  return (size_t)LD_TILES<NQ, TWO> * LD_KBYTES + (size_t)LD_RAWS<NQ, TWO> * LD_RAW + LD_QBYTES<NQ, TWO> + sizeof(LdShared<NQ>) + 1024;
+}
+static_assert(ld_smem<64, false>() <= 227 * 1024 && ld_smem<32, false>() <= 227 * 1024 && ld_smem<32, true>() <= 227 * 1024, "latent decode shared memory");
 
 __device__ __forceinline__ void ld_sync_workers() { asm volatile("barrier.cta.sync 1, 512;" ::: "memory"); }
 __device__ __forceinline__ void ld_sync_group(int g) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(2 + g) : "memory"); }
@@ -117,18 +121,18 @@ __device__ __forceinline__ void ld_value_block(uint32_t d, uint32_t v, uint32_t 
   if constexpr (KS + 1 < LD_TILE / 16) ld_value_block<NQ, M, KS + 1>(d, v, p, acc);
 }
 
-template <int NQ>
+template <int NQ, bool TWO>
 __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) {
-  constexpr int TILES = LD_TILES<NQ>, RAWS = LD_RAWS<NQ>;
+  constexpr int TILES = LD_TILES<NQ, TWO>, RAWS = LD_RAWS<NQ, TWO>;
   constexpr int CPT = NQ / 4, CPH = NQ / 8;     // columns of S^T (query rows) a column group has, a softmax thread takes
   constexpr uint32_t COLS = NQ == 64 ? 512 : 256;    // tensor memory: O^T 4 x NQ columns, S^T 2 x NQ
   extern __shared__ __align__(1024) uint8_t ld_smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)ld_smem_raw + 1023) & ~(uintptr_t)1023);
-  const uint32_t kb = smem_u32(smem), qb = kb + TILES * LD_KBYTES, raw = qb + LD_UNITS * NQ * 128;
-  LdShared<NQ>* sh = (LdShared<NQ>*)(smem + TILES * LD_KBYTES + LD_UNITS * NQ * 128 + RAWS * LD_RAW);
+  const uint32_t kb = smem_u32(smem), qb = kb + TILES * LD_KBYTES, raw = qb + LD_QBYTES<NQ, TWO>;
+  LdShared<NQ>* sh = (LdShared<NQ>*)(smem + TILES * LD_KBYTES + LD_QBYTES<NQ, TWO> + RAWS * LD_RAW);
   const vq2_latent_decode_args& a = g.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  const int L = a.latent_dim, R = a.rope_dim, nl = L / 64, nblk = (nl + 1) / 2, parts = (nl + 3) / 4;
+  const int L = a.latent_dim, R = a.rope_dim, nl = L / 64, nblk = (nl + 1) / 2, parts = (nl + 3) / 4, units = nl + (R ? 1 : 0);
   volatile int* abort = &sh->abort;
   pdl_launch_dependents();
 
@@ -194,6 +198,13 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
         if (nl > 1) ld_score_unit<NQ, 1>(d, k, q, 1);
         if (nl > 2) ld_score_unit<NQ, 2>(d, k, q, 1);
         if (nl > 3) ld_score_unit<NQ, 3>(d, k, q, 1);
+        const uint32_t q2 = q + units * (NQ * 8);         // the second term follows the first
+        if constexpr (TWO) {
+          ld_score_unit<NQ, 0>(d, k, q2, 1);
+          if (nl > 1) ld_score_unit<NQ, 1>(d, k, q2, 1);
+          if (nl > 2) ld_score_unit<NQ, 2>(d, k, q2, 1);
+          if (nl > 3) ld_score_unit<NQ, 3>(d, k, q2, 1);
+        }
         if (nl > 4) {
           ld_wait(&sh->kfull[b][1], (i / TILES) & 1, abort);
           tc_fence_after();
@@ -201,6 +212,12 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
           if (nl > 5) ld_score_unit<NQ, 5>(d, k, q, 1);
           if (nl > 6) ld_score_unit<NQ, 6>(d, k, q, 1);
           if (nl > 7) ld_score_unit<NQ, 7>(d, k, q, 1);
+          if constexpr (TWO) {
+            ld_score_unit<NQ, 4>(d, k, q2, 1);
+            if (nl > 5) ld_score_unit<NQ, 5>(d, k, q2, 1);
+            if (nl > 6) ld_score_unit<NQ, 6>(d, k, q2, 1);
+            if (nl > 7) ld_score_unit<NQ, 7>(d, k, q2, 1);
+          }
         }
         if (R) ld_score_any<NQ>(nl, d, k, q);
         umma_commit(&sh->sfull[b]);
@@ -238,7 +255,7 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
         const int st = i % RAWS;
         if (i == 0 || p.tile == 0) {
           // a query block's rows, once the products with the block before are done
-          const int bytes = (nl + (R ? 1 : 0)) * NQ * 128, item = p.b * g.nrb + p.rb;
+          const int bytes = units * NQ * 128 * (TWO ? 2 : 1), item = p.b * g.nrb + p.rb;
           if (++seg == 0) pdl_wait();
           else ld_wait(&sh->qfree, (seg - 1) & 1, abort);
           if (lane == 0) {
@@ -507,10 +524,11 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
 // (64 sequences, 320,206 cached rows: 16 query rows 84 us narrow, 151 us with 64 wide; 32 rows 122 us with 32 wide, 141 us as two
 // narrow blocks, 151 us with 64 wide; 48 rows 158 us with 64 wide, 201 us narrow). Where the narrow kernel's blocks have at most 5
 // tiles each, time is mostly latency, and it has less of it (64 rows of 8 sequences: 2048 cached rows each 31 us, 36 us wide;
-// 4096 each 43 and 42 us; 64 rows of one sequence, 64 cached: 11 and 18 us).
-static int ld_nq(int B, int T, int heads, long long most) {
+// 4096 each 43 and 42 us; 64 rows of one sequence, 64 cached: 11 and 18 us). fp16 queries in two terms take the room of 64 rows with
+// 32 (4 sequences of 65,536 rows, 64 heads: 166 us, bf16 113; 64 sequences, 16 heads, narrow: 95 and 80).
+static int ld_nq(int B, int T, int heads, long long most, bool two) {
   const long long rows = (long long)T * heads;
-  return rows <= 16 || (double)B * ((most + LD_TILE - 1) / LD_TILE) * ((rows + 15) / 16) <= 5 * 2 * 148 ? 16 : rows <= 32 ? 32 : 64;
+  return rows <= 16 || (double)B * ((most + LD_TILE - 1) / LD_TILE) * ((rows + 15) / 16) <= 5 * 2 * 148 ? 16 : two || rows <= 32 ? 32 : 64;
 }
 
 struct LdLayout {
@@ -528,7 +546,7 @@ static LdLayout ld_layout(int B, int nq, int nrb, int L, int R, int grid) {
   w.start = take((size_t)(B + 1) * 4);
   w.ml = take(parts * nq * 8);
   w.meta = take(items * nq * 8);
-  w.q = take(items * (L / 64 + (R ? 1 : 0)) * nq * 128);
+  w.q = take(items * (L / 64 + (R ? 1 : 0)) * nq * 256);       // (a second term of fp16 rows included)
   w.part = take(parts * nq * L * 4);
   w.total = at + 256;
   return w;
@@ -540,17 +558,19 @@ static int ld_blocks(int nq, int sms) { return std::min(sms, 148) * (nq == 16 ? 
 // dependent launch.
 template <int DT, int NQ, bool NARROW>
 static int ld_launch(const LdArgs& g, cudaStream_t st) {
+  constexpr bool TWO = DT == VQ2_DT_F16;
   void (*kernel)(LdArgs);
   size_t smem;
   if constexpr (NARROW) {
-    static void (*const by_groups[8])(LdArgs) = {latent_decode_narrow_kernel<1>, latent_decode_narrow_kernel<2>, latent_decode_narrow_kernel<3>,
-                                                 latent_decode_narrow_kernel<4>, latent_decode_narrow_kernel<5>, latent_decode_narrow_kernel<6>,
-                                                 latent_decode_narrow_kernel<7>, latent_decode_narrow_kernel<8>};
+    static void (*const by_groups[8])(LdArgs) = {
+        latent_decode_narrow_kernel<1, TWO>, latent_decode_narrow_kernel<2, TWO>, latent_decode_narrow_kernel<3, TWO>,
+        latent_decode_narrow_kernel<4, TWO>, latent_decode_narrow_kernel<5, TWO>, latent_decode_narrow_kernel<6, TWO>,
+        latent_decode_narrow_kernel<7, TWO>, latent_decode_narrow_kernel<8, TWO>};
     kernel = by_groups[g.a.latent_dim / 64 - 1];
     smem = LN_SMEM;
   } else {
-    kernel = latent_decode_kernel<NQ>;
-    smem = ld_smem<NQ>();
+    kernel = latent_decode_kernel<NQ, TWO>;
+    smem = ld_smem<NQ, TWO>();
   }
   static bool raised[8][64];
   if (!smem_limit_once(kernel, smem, raised[NARROW ? g.a.latent_dim / 64 - 1 : 0])) return VQ2_ERR_CUDA;
@@ -583,9 +603,9 @@ extern "C" size_t vq2_latent_decode_workspace_size(int B, int T, int heads, int 
   if (B <= 0 || T <= 0 || heads <= 0 || !latent_dims_ok(latent_dim, rope_dim) || (long long)T * heads > 1 << 20 ||
       (long long)B * ((long long)T * heads + 64) >= 1LL << 27)
     return 0;
-  // the larger of what the two kernels that may be taken need
+  // the most that a kernel which may be taken needs
   size_t most = 0;
-  for (const int nq : {16, ld_nq(B, T, heads, 1LL << 40)})
+  for (const int nq : {16, ld_nq(B, T, heads, 1LL << 40, false), ld_nq(B, T, heads, 1LL << 40, true)})
     most = std::max(most, ld_layout(B, nq, (int)(((long long)T * heads + nq - 1) / nq), latent_dim, rope_dim, ld_blocks(nq, 148)).total);
   return most;
 }
@@ -605,7 +625,7 @@ extern "C" int vq2_latent_decode(const vq2_latent_decode_args* a, void* ws, size
     return VQ2_ERR_WORKSPACE;
   LdArgs g = {};
   g.a = *a;
-  const int nq = ld_nq(a->B, a->T, a->heads, (long long)a->max_pages * a->page_size), sms = device_sm_count();
+  const int nq = ld_nq(a->B, a->T, a->heads, (long long)a->max_pages * a->page_size, a->dtype == VQ2_DT_F16), sms = device_sm_count();
   if (sms <= 0) return VQ2_ERR_CUDA;
   g.rb = latent_row_bytes(a->latent_dim, a->rope_dim);
   g.nrb = (a->T * a->heads + nq - 1) / nq;
@@ -631,5 +651,5 @@ extern "C" int vq2_latent_decode(const vq2_latent_decode_args* a, void* ws, size
   const bool bf = a->dtype == VQ2_DT_BF16;
   if (nq == 16) return bf ? ld_launch<VQ2_DT_BF16, 16, true>(g, st) : ld_launch<VQ2_DT_F16, 16, true>(g, st);
   if (nq == 32) return bf ? ld_launch<VQ2_DT_BF16, 32, false>(g, st) : ld_launch<VQ2_DT_F16, 32, false>(g, st);
-  return bf ? ld_launch<VQ2_DT_BF16, 64, false>(g, st) : ld_launch<VQ2_DT_F16, 64, false>(g, st);
+  return ld_launch<VQ2_DT_BF16, 64, false>(g, st);
 }

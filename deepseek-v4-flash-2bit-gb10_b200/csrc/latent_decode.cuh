@@ -16,7 +16,7 @@ struct LdArgs {
   int* start;           // [B + 1] first position of each sequence
   float2* ml;           // [parts][NQ] maximum and denominator of a part
   float* part;          // [parts][L][NQ]; a block's part of query block n is number n + block
-  uint8_t* q;           // [query blocks][units][NQ][128 bytes] rotated query rows, fp16, swizzled
+  uint8_t* q;           // [query blocks][units][NQ][128 bytes] rotated query rows, fp16, swizzled (for fp16 then their remainders)
   float2* meta;         // [query blocks][NQ] factor of a row's logits, and its token (as int bits)
 };
 
@@ -133,7 +133,10 @@ struct LdRows {
 
 
 // Query rows, one warp a row: latent part rotated, all scaled into fp16's range by a power of two. Written as swizzled units of
-// NQ rows x 64 values, or (OPERANDS, 16 rows) as the left operands of m16n8k16 products.
+// NQ rows x 64 values, or (OPERANDS, 16 rows) as the left operands of m16n8k16 products. Rounding a rotated fp16 row to fp16 would cost
+// as much as rounding the output (2e-4 of it each), so its remainders follow as a second term: in fp16, or (OPERANDS) in their upper
+// 8 bits, whose 3 significant ones leave 2^-14 of the row. A bf16 output rounds 8 times coarser and needs none, nor does the rotary part
+// (only scaled).
 constexpr int LQ_WARPS = 4;
 template <int DT, int NQ, bool OPERANDS>
 __global__ void __launch_bounds__(LQ_WARPS * 32) latent_query_kernel(LdArgs g) {
@@ -158,20 +161,36 @@ __global__ void __launch_bounds__(LQ_WARPS * 32) latent_query_kernel(LdArgs g) {
     for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[k][i]));
   }
   const float2 f = f16_range_scale(fminf(warp_max(m), 3.0e38f));
-  uint8_t* dst = g.q + (size_t)item * units * (NQ * 128);
+  constexpr bool TWO = DT == VQ2_DT_F16;
+  const size_t bytes = (size_t)units * (NQ * 128);
+  uint8_t* dst = g.q + item * bytes * (TWO ? 2 : 1);
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
     const int u = k < 2 ? lane + 32 * k : lane, unit = k < 2 ? u >> 3 : nl, c = u & 7;
     if (!(k < 2 ? u * 8 < L : R && u < 8)) continue;
     const uint32_t w[4] = {pack2<VQ2_DT_F16>(v[k][0] * f.x, v[k][1] * f.x), pack2<VQ2_DT_F16>(v[k][2] * f.x, v[k][3] * f.x),
                            pack2<VQ2_DT_F16>(v[k][4] * f.x, v[k][5] * f.x), pack2<VQ2_DT_F16>(v[k][6] * f.x, v[k][7] * f.x)};
+    uint32_t rest[4] = {};
+    if (TWO && k < 2)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 h = __half22float2(*(const __half2*)&w[j]);
+        rest[j] = pack2<VQ2_DT_F16>(v[k][2 * j] * f.x - h.x, v[k][2 * j + 1] * f.x - h.y);
+      }
     if (OPERANDS) {
       // piece 2 unit + c / 4, lane 4 (r mod 8) + c mod 4; values 0-1 and 2-3 are registers r / 8 and r / 8 + 2 of its first product
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         ((uint32_t*)dst)[(((2 * unit + (c >> 2)) * 2 + (j >> 1)) * 32 + (r & 7) * 4 + (c & 3)) * 4 + (r >> 3) + 2 * (j & 1)] = w[j];
+      if (TWO && k < 2)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)      // rounded to the upper 8 bits of each half
+          ((uint16_t*)(dst + bytes))[(((2 * unit + (c >> 2)) * 2 + (j >> 1)) * 32 + (r & 7) * 4 + (c & 3)) * 4 + (r >> 3) + 2 * (j & 1)] =
+              (uint16_t)__byte_perm(rest[j] + 0x00800080u, 0, 0x0031);
     } else {
-      *(uint4*)(dst + (size_t)unit * (NQ * 128) + r * 128 + ((c ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      const size_t to = (size_t)unit * (NQ * 128) + r * 128 + ((c ^ (r & 7)) << 4);
+      *(uint4*)(dst + to) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (TWO && k < 2) *(uint4*)(dst + bytes + to) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
     }
   }
   // a row that pads the block sees nothing

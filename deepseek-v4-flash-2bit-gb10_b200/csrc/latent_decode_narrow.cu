@@ -25,6 +25,7 @@ constexpr float LN_BIAS = 5.f, LN_RAISE = 10.f;                // P = 2^(z - m +
 
 struct LnShared {
   uint4 q[18][2][32];                  // query rows as operands: piece of 32 values, product, lane
+  uint2 rest[16][2][32];               // of fp16 rows: what q rounded away, in 8 bits a value
   uint4 p[2][LD_TILE / 16][32];        // probabilities as operands: 16 cached rows, lane
   float4 half[LN_WARPS][32];           // sums over half of the values, on their way to the other warp of the pair
   uint64_t rfull[LN_STAGES];
@@ -61,10 +62,16 @@ __device__ __forceinline__ void ln_sync() { asm volatile("barrier.cta.sync 1, 25
 
 __device__ __forceinline__ void ln_sync_pair(int k) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(2 + k) : "memory"); }
 
+// Eight 8-bit values (the upper bytes of halves) as an operand.
+__device__ __forceinline__ uint4 ln_rest(const uint2& x) {
+  return make_uint4(__byte_perm(x.x, 0, 0x1404), __byte_perm(x.x, 0, 0x3424), __byte_perm(x.y, 0, 0x1404), __byte_perm(x.y, 0, 0x3424));
+}
+
 // Pieces FROM .. TO - 1 (32 values each) of the latent part of S for 16 cached rows: acc[u] for rows 8 u .. 8 u + 7 of them.
-template <int FROM, int TO>
-__device__ __forceinline__ void ln_scores(float (*acc)[2][4], const uint4 (*q)[2][32], const uint8_t* row0, const uint8_t* row1,
-                                          const uint32_t* sc0, const uint32_t* sc1, int lane) {
+// TWO: with the query rows' second term.
+template <int FROM, int TO, bool TWO>
+__device__ __forceinline__ void ln_scores(float (*acc)[2][4], const uint4 (*q)[2][32], const uint2 (*rest)[2][32], const uint8_t* row0,
+                                          const uint8_t* row1, const uint32_t* sc0, const uint32_t* sc1, int lane) {
 #pragma unroll
   for (int n = FROM; n < TO; ++n) {
     const uint4 qa = q[n][0][lane], qb = q[n][1][lane];
@@ -73,14 +80,19 @@ __device__ __forceinline__ void ln_scores(float (*acc)[2][4], const uint4 (*q)[2
       const uint32_t s = __byte_perm((u ? sc1 : sc0)[n >> 2], 0, (n >> 1) & 1 ? 0x3232 : 0x1010);
       const __half2 s2 = *(const __half2*)&s, c2 = __hmul2(s2, __float2half2_rn(-24.f));
       const uint32_t w = *(const uint32_t*)((u ? row1 : row0) + (4 * n + (lane & 3)) * 4);
-      mma16816(acc[u][0], qa, ln_pair<0>(w, s2, c2), ln_pair<1>(w, s2, c2));
-      mma16816(acc[u][1], qb, ln_pair<2>(w, s2, c2), ln_pair<3>(w, s2, c2));
+      const uint32_t k0 = ln_pair<0>(w, s2, c2), k1 = ln_pair<1>(w, s2, c2), k2 = ln_pair<2>(w, s2, c2), k3 = ln_pair<3>(w, s2, c2);
+      mma16816(acc[u][0], qa, k0, k1);
+      mma16816(acc[u][1], qb, k2, k3);
+      if (TWO) {
+        mma16816(acc[u][0], ln_rest(rest[n][0][lane]), k0, k1);
+        mma16816(acc[u][1], ln_rest(rest[n][1][lane]), k2, k3);
+      }
     }
   }
 }
 
 // NL: groups of 64 latent values, known at compile time so that a tile's work is three straight runs of instructions.
-template <int NL>
+template <int NL, bool TWO>
 __global__ void __launch_bounds__(LN_THREADS, 2) latent_decode_narrow_kernel(LdArgs g) {
   extern __shared__ __align__(128) uint8_t ln_smem[];
   LnShared* sh = (LnShared*)(ln_smem + LN_STAGES * LN_STAGE);
@@ -212,8 +224,10 @@ __global__ void __launch_bounds__(LN_THREADS, 2) latent_decode_narrow_kernel(LdA
       if (fresh) {                                // a new query block: its rows to shared memory (the one before is done with)
         item = p.b * g.nrb + p.rb;
         if (i == 0) pdl_wait();
-        const uint4* src = (const uint4*)(g.q + (size_t)item * LN_ROWS * units * 128);
+        const uint4* src = (const uint4*)(g.q + (size_t)item * LN_ROWS * units * 128 * (TWO ? 2 : 1));
         for (int u = tid; u < LN_ROWS * units * 8; u += LN_THREADS) ((uint4*)sh->q)[u] = __ldcg(src + u);
+        if (TWO)
+          for (int u = tid; u < NL * 64; u += LN_THREADS) ((uint4*)sh->rest)[u] = __ldcg(src + LN_ROWS * units * 8 + u);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const float2 m = __ldcg(g.meta + item * LN_ROWS + gr + 8 * k);
@@ -236,9 +250,9 @@ __global__ void __launch_bounds__(LN_THREADS, 2) latent_decode_narrow_kernel(LdA
         const uint4 x0 = *(const uint4*)(row0 + tail), x1 = *(const uint4*)(row1 + tail);
         const uint32_t sc0[4] = {x0.x, x0.y, x0.z, x0.w}, sc1[4] = {x1.x, x1.y, x1.z, x1.w};
         float acc[2][2][4] = {};
-        auto low = [&]() { ln_scores<0, NL + 1>(acc, sh->q, row0, row1, sc0, sc1, lane); };
+        auto low = [&]() { ln_scores<0, NL + 1, TWO>(acc, sh->q, sh->rest, row0, row1, sc0, sc1, lane); };
         auto high = [&]() {
-          ln_scores<NL + 1, 2 * NL>(acc, sh->q, row0, row1, sc0, sc1, lane);
+          ln_scores<NL + 1, 2 * NL, TWO>(acc, sh->q, sh->rest, row0, row1, sc0, sc1, lane);
           if (R) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {

@@ -489,3 +489,23 @@ def test_graphs_of_growing_sizes_keep_their_workspaces():
         graph.replay()
         assert torch.equal(out, want)
     assert all((t == 7.0).all() for t in others)
+
+
+# ------------------------------------------------------------------------------------ fp16 queries
+# In the 2-norm the fp16 form may err by the rounding of its output (that of ref.half(), measured on the same values) and by that of the
+# probabilities, whose relative errors have the same distribution and average over the keys: together at most sqrt(2) of
+# the first. The query's remainder beyond its second term (2^-14 of it at most) and the fp32 sums stay under the rest up to 1.5; a
+# query rounded to fp16 alone gives 1.6 to 2.6.
+@pytest.mark.parametrize("lens,T,heads,L,R,page", [
+    ([236], 1, 3, 128, 64, 64),                     # 16 query rows a block
+    ([4000, 1700], 1, 16, 512, 64, 64),
+    ([90, 0, 33], 2, 5, 448, 0, 1),
+    ([40000, 20000], 1, 24, 512, 64, 64),           # 32 query rows a block
+    ([30000, 10000], 2, 64, 320, 32, 16),
+    ([60000, 3], 1, 64, 64, 64, 128),
+])
+def test_fp16_decode_errs_like_its_output(lens, T, heads, L, R, page):
+    from oracle import latent_ref as O
+    q, cache, table, kv_len, scale, out = _decode_case(lens, T, heads, L, R, page, "f16", seed=sum(lens) + L)
+    ref, _ = O.decode(q, cache.data, table, kv_len, scale, L, R)
+    assert (out.double() - ref).norm() <= 1.5 * (ref.half().double() - ref).norm()
