@@ -26,7 +26,7 @@
 // tile runs under the products of the next. In the steady state no barrier spans the block.
 // What bounds it: with 64 query rows there is room for one tile, so its expansion, S, softmax and P V follow one another: 5,300
 // cycles a tile, where the products take 2,040 (36 of S at 34 cycles, 16 of P V at 51, measured alone) and the matrix units
-// need 1,088 of those. 4 sequences of 65,536 rows, 64 query rows: 115 us a call, DRAM 14 % and tensor pipe 30 % busy.
+// need 1,088 of those. 4 sequences of 65,536 rows, 64 query rows: 115 us a call, DRAM 13 % and tensor pipe 30 % busy.
 #include <algorithm>
 #include "latent_decode.cuh"
 

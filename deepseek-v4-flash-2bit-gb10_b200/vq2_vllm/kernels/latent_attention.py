@@ -45,7 +45,8 @@ def latent_attention_decode(q: torch.Tensor, cache: LatentCache, block_table: to
         out = sum_j softmax_j(scale * (q_c . c_j + q_r . r_j)) c_j,   j <= kv_len - T + t
 
     A sequence of length 0 (or a row that sees nothing) gives zeros; rows of the cache past kv_len are never
-    used, whatever they hold. ``scale`` is positive. Three launches; nothing waits for the host: safe to capture in
+    used, whatever they hold. ``scale`` is positive. fp16 queries are held in two terms, which costs up to half as much
+    time again as bf16. Three launches; nothing waits for the host: safe to capture in
     a CUDA graph."""
     L, R = cache.latent_dim, cache.rope_dim
     if not scale > 0:
