@@ -322,11 +322,12 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
       auto expand = [&](int number) {
         const int b = number % TILES, turn = piece >> 1;
         const uint32_t tile = kb + b * LD_KBYTES + row * 128;
-        if (!here && piece == 0) sh->flag[b][row] = 2 * number;
 #pragma unroll
         for (int m = 0; m < LD_PARTS; ++m) {
           if (m >= parts) break;
           if (number >= TILES) ld_wait(&sh->kfree[b][m], (number / TILES - 1) & 1, abort);
+          // (after the wait: until P V of the buffer's tile before has begun, a slower column group may still read its flags)
+          if (m == 0 && !here && piece == 0) sh->flag[b][row] = 2 * number;
           if (8 * m + piece < 2 * nl) {
             const uint32_t two = piece & 4 ? (m ? sc.w : sc.y) : (m ? sc.z : sc.x);
             uint32_t s = piece & 2 ? two >> 16 : two & 0xFFFFu;
