@@ -38,6 +38,7 @@ constexpr int LP_UNIT = LP_TILE * 128;         // bytes of a unit: 128 rows of 6
 constexpr int LP_KUNITS = 6, LP_VUNITS = 2, LP_KMAX = 3;
 constexpr int LP_THREADS = 384;
 constexpr float LP_RAISE = 8.f;    // log2 by which a row's maximum may grow before O is rescaled
+constexpr float LP_FAR = 65536.f;  // log2 units from 0 beyond which scores are taken relative to the maximum before they are scaled
 
 struct LpShared {
   uint64_t kfull[LP_KMAX], kempty[LP_KMAX], vfull[2], vempty[2];
@@ -347,7 +348,7 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, LpParts parts, const _
     const int n = n_of(t);
     float m = -INFINITY;                                      // the maximum that P and O are relative to
     float2 l2 = make_float2(0.f, 0.f);
-    bool ok = true;
+    bool ok = true, far = false;
     for (int j = 0; j < n; ++j) {
       if (!__all_sync(0xffffffffu, mbar_wait(&sh->sfull[t], j & 1))) { ok = false; break; }
       tc_fence_after();
@@ -370,6 +371,7 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, LpParts parts, const _
       if (__any_sync(0xffffffffu, raise) ) {
         const float mn = raise ? mx : m, f = raise ? ex2((m - mn) * sl) : 1.f;
         m = mn;
+        far = __any_sync(0xffffffffu, m != -INFINITY && fabsf(m) * sl > LP_FAR);
         l2.x *= f;
         l2.y *= f;
         if (j > 0) {              // every product into O issued before this step's scores is done
@@ -385,7 +387,14 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, LpParts parts, const _
           }
         }
       }
-      const float mb = m == -INFINITY ? 0.f : -m * sl;
+      // scale (s - m) as one fused multiply-add costs nothing, but -m scale is rounded first: 2^-9 at LP_FAR, whole
+      // powers of 2 beyond 2^24, where P would leave its type's range. There the difference, exact near m, comes first.
+      if (far) {
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int c = 0; c < 128; ++c) s[c] -= base;
+      }
+      const float mb = far || m == -INFINITY ? 0.f : -m * sl;
       const float2 s2 = make_float2(sl, sl), b2 = make_float2(mb, mb);
       float2 sum = make_float2(0.f, 0.f), sumb = sum;
 #pragma unroll
