@@ -387,35 +387,56 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, LpParts parts, const _
           }
         }
       }
-      // scale (s - m) as one fused multiply-add costs nothing, but -m scale is rounded first: 2^-9 at LP_FAR, whole
-      // powers of 2 beyond 2^24, where P would leave its type's range. There the difference, exact near m, comes first.
-      if (far) {
-        const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-        for (int c = 0; c < 128; ++c) s[c] -= base;
-      }
-      const float mb = far || m == -INFINITY ? 0.f : -m * sl;
-      const float2 s2 = make_float2(sl, sl), b2 = make_float2(mb, mb);
       float2 sum = make_float2(0.f, 0.f), sumb = sum;
+      if (__builtin_expect(far, 0)) {
+        // scale (s - m) as one fused multiply-add rounds -m scale first: by 2^-9 at LP_FAR, by whole powers of 2 beyond 2^24, where P would
+        // leave its type's range. Here the difference, exact near m, comes first. (From tensor memory again, 16 scores at a
+        // time, so that the other path keeps its registers; P's columns lie below the scores still to be read.)
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 16) {
+          float x[16];
+          uint32_t p[8];
+          tmem_ld16(ts + c, x);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t p[32];
+          for (int k = 0; k < 16; ++k) {
+            x[k] = c + k < lim ? ex2((x[k] - base) * sl) : 0.f;
+            sum.x += x[k];
+          }
 #pragma unroll
-        for (int c = 0; c < 64; c += 2) {
-          float2 x = ffma2(make_float2(s[half * 64 + c], s[half * 64 + c + 1]), s2, b2);
-          x.x = ex2(x.x);
-          x.y = ex2(x.y);
-          if (c & 2) sumb = fadd2(sumb, x);
-          else sum = fadd2(sum, x);
-          p[c >> 1] = pack2<DT>(x.x, x.y);
+          for (int k = 0; k < 8; ++k) p[k] = pack2<DT>(x[2 * k], x[2 * k + 1]);
+          tmem_st8(ts + (c >> 1), p);
+          tmem_st_wait();
+          keep_live8(p);
+          if ((c & 63) == 48) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->pfull[t][c >> 6]);
+          }
         }
-        tmem_st32(ts + half * 32, p);
-        tmem_st_wait();
-        keep_live16(p);
-        keep_live16(p + 16);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->pfull[t][half]);
+      } else {
+        const float mb = m == -INFINITY ? 0.f : -m * sl;
+        const float2 s2 = make_float2(sl, sl), b2 = make_float2(mb, mb);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t p[32];
+#pragma unroll
+          for (int c = 0; c < 64; c += 2) {
+            float2 x = ffma2(make_float2(s[half * 64 + c], s[half * 64 + c + 1]), s2, b2);
+            x.x = ex2(x.x);
+            x.y = ex2(x.y);
+            if (c & 2) sumb = fadd2(sumb, x);
+            else sum = fadd2(sum, x);
+            p[c >> 1] = pack2<DT>(x.x, x.y);
+          }
+          tmem_st32(ts + half * 32, p);
+          tmem_st_wait();
+          keep_live16(p);
+          keep_live16(p + 16);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->pfull[t][half]);
+        }
       }
       l2 = fadd2(l2, fadd2(sum, sumb));
     }
