@@ -13,9 +13,11 @@
 //                lies, rows = keys, so no transpose); the two tiles alternate, so one tile's products
 //                run under the other tile's softmax
 //   warps 4-11   softmax, one thread a query row (4 warps a tile): the row's 128 scores in registers
-// A row's maximum is refreshed only when it rose by more than 2^8 in the exponent: P then stays below
-// 256 (exact enough in 16 bits: the rounding is relative) and O is rarely rescaled. P goes over in halves of 64
-// keys, so that O's products start under the second half's exponentials.
+// A row's maximum is refreshed only when it rose by more than 2^8 in the exponent, so that O is rarely rescaled: P is at most 2^8
+// times what it is at the maximum. In bf16, with the range of fp32, that is 1 and every P rounds by 2^-9 of itself. In fp16 it is 2^7,
+// so that P ends at 2^15, a key of 2^-21 of the largest still rounds by 2^-12 of itself and one of 2^-32 is the last to count (held
+// at 1, keys 2^-14 below a dominant one lost bits and those 2^-25 below it were gone, all of the output where that key's value is 0).
+// P goes over in halves of 64 keys, so that O's products start under the second half's exponentials.
 // Where there are fewer blocks of queries than SMs, a block's keys are split into parts, one CTA each, and a second kernel joins
 // them (below: lp_split).
 // What bounds it: the products of a step (two tiles, 128 keys) take 2560 cycles, the step about 3400: 1700 for a
@@ -38,6 +40,7 @@ constexpr int LP_UNIT = LP_TILE * 128;         // bytes of a unit: 128 rows of 6
 constexpr int LP_KUNITS = 6, LP_VUNITS = 2, LP_KMAX = 3;
 constexpr int LP_THREADS = 384;
 constexpr float LP_RAISE = 8.f;    // log2 by which a row's maximum may grow before O is rescaled
+constexpr float LP_BIAS_F16 = 7.f; // log2 of P at its row's maximum, in fp16
 constexpr float LP_FAR = 65536.f;  // log2 units from 0 beyond which scores are taken relative to the maximum before they are scaled
 
 struct LpShared {
@@ -387,6 +390,7 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, LpParts parts, const _
           }
         }
       }
+      constexpr float bias = DT == VQ2_DT_F16 ? LP_BIAS_F16 : 0.f;      // denominators carry the factor too, and so do all parts of a row
       float2 sum = make_float2(0.f, 0.f), sumb = sum;
       if (__builtin_expect(far, 0)) {
         // scale (s - m) as one fused multiply-add rounds -m scale first: by 2^-9 at LP_FAR, by whole powers of 2 beyond 2^24, where P would
@@ -400,7 +404,7 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, LpParts parts, const _
           tmem_ld16(ts + c, x);
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            x[k] = c + k < lim ? ex2((x[k] - base) * sl) : 0.f;
+            x[k] = c + k < lim ? ex2(fmaf(x[k] - base, sl, bias)) : 0.f;
             sum.x += x[k];
           }
 #pragma unroll
@@ -415,7 +419,7 @@ latent_prefill_kernel(vq2_latent_prefill_args a, int nqb, LpParts parts, const _
           }
         }
       } else {
-        const float mb = m == -INFINITY ? 0.f : -m * sl;
+        const float mb = (m == -INFINITY ? 0.f : -m * sl) + bias;
         const float2 s2 = make_float2(sl, sl), b2 = make_float2(mb, mb);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {

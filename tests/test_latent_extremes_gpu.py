@@ -38,3 +38,63 @@ def test_prefill_over_logits_of_any_size(dtype, e, f, n, past):
         out = latent_attention_prefill(q, k, None, v, cu_q, cu_k, n, 1.0)
         ref, absolute = O.prefill(q, k, None, v, cu_q, cu_k, 1.0)
         _check(out, ref, absolute, u, u, 2.0 ** -18, 64)
+
+
+# ------------------------------------------------------------------------------- one key with nearly all the weight
+# Probabilities in fp16 are held with their row's maximum at 2^7 or above (at most 2^15): above 2^-21 of it they round by 2^-11 of themselves,
+# below by up to 2^-32 of it. The 2-norm counts both as independent (the values are), the first twice for good measure, and half a step
+# of the output's smallest values.
+@pytest.mark.parametrize("n,past", [(200, 0), (1000, 0), (64, 4000)])
+@pytest.mark.parametrize("gap", [8, 10, 12, 14, 16, 18, 20])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_prefill_beside_a_key_without_a_value(dtype, gap, n, past):
+    """The first key is `gap` above the others' logits (e^gap times a weight) and its value is zero: the output is
+    what the others leave."""
+    from vq2_vllm.kernels.latent_attention import latent_attention_prefill
+    dt, u = DT[dtype]
+    g = _gen(gap)
+    S, scale, heads, d = n + past, 0.125, 2, 64
+    q = torch.randn(n, heads, d, generator=g, device="cuda") * 0.3
+    k = torch.randn(S, heads, d, generator=g, device="cuda")
+    v = torch.randn(S, heads, d, generator=g, device="cuda").to(dt)
+    q[..., 0], k[..., 0], k[0], v[0] = 8.0, 0.0, 0.0, 0.0
+    k[0, :, 0] = gap
+    q, k = q.to(dt), k.to(dt)
+    out = latent_attention_prefill(q, k, None, v, _cu(0, n), _cu(0, S), n, scale).double()
+    z = torch.einsum("ihd,jhd->hij", q.double(), k.double()) * scale
+    hidden = torch.arange(S, device="cuda")[None] > torch.arange(n, device="cuda")[:, None] + past
+    p = torch.softmax(z.masked_fill(hidden, -math.inf), -1)
+    sums = lambda w, x: torch.einsum("hij,jhd->ihd", w, x)  # noqa: E731
+    v = v.double()
+    ref, absolute, square = sums(p, v), sums(p, v.abs()), sums(p * p, v * v).sqrt()
+    seen = sums((~hidden).double().expand_as(p), v * v).sqrt()
+    dz = d * 2.0 ** -23 * scale * 0.3 * 8 * 2 * 8 * 2                 # of the keys but the first: norms under 0.6 * 8 and 2 * 8
+    tiny = 2.0 ** -32 if dtype == "f16" else 0.0
+    bound = u * ref.norm() + 2 * u * square.norm() + (2 * dz / math.sqrt(d) + 1e-5) * absolute.norm() + tiny * seen.norm()
+    bound += 2.0 ** -25 * math.sqrt(out.numel()) if dtype == "f16" else 0.0
+    assert torch.isfinite(out).all()
+    assert (out - ref).norm() <= bound, ((out - ref).norm() / bound).item()
+
+
+@pytest.mark.parametrize("q_scale", [1e-3, 10.0, 100.0])
+@pytest.mark.parametrize("qlens,prefix", [([333], [77]), ([140], [4000])])
+def test_fp16_prefill_over_flat_and_peaked_rows(q_scale, qlens, prefix):
+    from test_latent_gpu import _prefill_case
+    _prefill_case(qlens, prefix, 3, 128, 64, 128, "f16", 71, q_scale=q_scale)
+
+
+@pytest.mark.parametrize("n,past", [(1000, 0), (64, 4000)])
+def test_fp16_prefill_rising_logits(n, past):
+    from oracle import latent_ref as O
+    from vq2_vllm.kernels.latent_attention import latent_attention_prefill
+    heads, S, g = 2, n + past, _gen(74)
+    q = torch.randn(n, heads, 144, generator=g, device="cuda").half()
+    kv = torch.randn(S, heads, 256, generator=g, device="cuda").half()
+    kr = torch.zeros(S, 16, device="cuda")
+    kr[:, 0] = torch.arange(S, device="cuda") / 4
+    kr = kr.half()
+    for sign in (1.0, -1.0):
+        q[..., 128] = sign * 8.0
+        out = latent_attention_prefill(q, kv[..., :128], kr, kv[..., 128:], _cu(0, n), _cu(0, S), n, 0.25)
+        ref, absolute = O.prefill(q, kv[..., :128], kr, kv[..., 128:], _cu(0, n), _cu(0, S), 0.25)
+        _check(out, ref, absolute, 2.0 ** -11, 2.0 ** -11, 144 * 2.0 ** -23 * 0.25 * 30 * (S / 4 + 50), 144)
