@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
         }
         bool raise = opens;
 #pragma unroll
-        for (int c = 0; c < CPH; ++c) raise |= z[c] > ref[c] + LD_RAISE;
+        for (int c = 0; c < CPH; ++c) raise |= z[c] - ref[c] > LD_RAISE;     // (differences first, here and below: exact where a sum is not)
         if (ld_any_group(grp, raise)) {
           float f[CPH];
 #pragma unroll
@@ -434,8 +434,8 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
         uint32_t ph[CPH / 2];
 #pragma unroll
         for (int c = 0; c < CPH; c += 2) {
-          const float p0 = ex2(z[c] - ((ref[c] == -INFINITY ? 0.f : ref[c]) - LD_BIAS));
-          const float p1 = ex2(z[c + 1] - ((ref[c + 1] == -INFINITY ? 0.f : ref[c + 1]) - LD_BIAS));
+          const float p0 = ex2((z[c] - (ref[c] == -INFINITY ? 0.f : ref[c])) + LD_BIAS);
+          const float p1 = ex2((z[c + 1] - (ref[c + 1] == -INFINITY ? 0.f : ref[c + 1])) + LD_BIAS);
           l[c] += p0;
           l[c + 1] += p1;
           ph[c / 2] = pack2<VQ2_DT_F16>(p0, p1);

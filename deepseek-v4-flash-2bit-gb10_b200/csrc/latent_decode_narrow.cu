@@ -314,13 +314,13 @@ __global__ void __launch_bounds__(LN_THREADS, 2) latent_decode_narrow_kernel(LdA
       for (int k = 0; k < 4; ++k) {
         const int j = p.tile * LD_TILE + mine + 2 * t + (k & 1);
         if (!((there >> (k & 1)) & 1) || j > p.len - a.T + tok[k >> 1]) z[k] = -INFINITY;
-        raise |= z[k] > ref[k >> 1] + LN_RAISE;
+        raise |= z[k] - ref[k >> 1] > LN_RAISE;      // (differences first, here and below: exact where a sum with a large logit is not)
       }
       uint4 (*pb)[32] = sh->p[i & 1];
       float pr[4];
       auto probabilities = [&]() {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) pr[k] = ex2(z[k] - ((ref[k >> 1] == -INFINITY ? 0.f : ref[k >> 1]) - LN_BIAS));
+        for (int k = 0; k < 4; ++k) pr[k] = ex2((z[k] - (ref[k >> 1] == -INFINITY ? 0.f : ref[k >> 1])) + LN_BIAS);
         // registers 0, 1 (rows gr, gr + 8) of the operand of 16 cached rows for the first 8 of them, 2, 3 for the others
         *((uint2*)&pb[quad][lane] + half) = make_uint2(pack2<VQ2_DT_F16>(pr[0], pr[1]), pack2<VQ2_DT_F16>(pr[2], pr[3]));
       };

@@ -98,3 +98,45 @@ def test_fp16_prefill_rising_logits(n, past):
         out = latent_attention_prefill(q, kv[..., :128], kr, kv[..., 128:], _cu(0, n), _cu(0, S), n, 0.25)
         ref, absolute = O.prefill(q, kv[..., :128], kr, kv[..., 128:], _cu(0, n), _cu(0, S), 0.25)
         _check(out, ref, absolute, 2.0 ** -11, 2.0 ** -11, 144 * 2.0 ** -23 * 0.25 * 30 * (S / 4 + 50), 144)
+
+
+# ------------------------------------------------------------------------------- absorbed form
+def _unit_scale():
+    """A scale whose product with log2(e), both in 32 bits, rounds to 1."""
+    import numpy as np
+    log2e = np.float32(1.4426950408889634)
+    s = np.float32(1.0) / log2e
+    for s in (s, np.nextafter(s, np.float32(0)), np.nextafter(s, np.float32(1))):
+        if np.float32(s * log2e) == 1.0:
+            return float(s)
+    raise AssertionError("no such scale")
+
+
+@pytest.mark.parametrize("heads", [16, 24, 64])                        # narrow kernel, 32 and 64 query rows a block
+@pytest.mark.parametrize("dtype,e", [("bf16", 20), ("bf16", 24), ("bf16", 25), ("bf16", 26), ("bf16", 27), ("bf16", 29), ("f16", 20),
+                                     ("f16", 24), ("f16", 25)])
+def test_decode_over_logits_of_any_size(dtype, e, heads):
+    """Logits of 2^e, in log2 units, that grow over a block's tiles by less than what raises the running maximum and by
+    more, in multiples of what 32 bits resolve there (so that every sum of the two products behind a logit is exact)."""
+    from oracle import latent_ref as O
+    from vq2_vllm.kernels.latent_attention import latent_attention_decode
+    from vq2_vllm.kernels.latent_cache import LatentCache
+    dt, u = DT[dtype]
+    L, R, n, g = 64, 8, 64 * 296 * 4, _gen(e)                       # 4 tiles a block, 8 in the wide kernels
+    unit = max(4.0, 2.0 ** (e - 23))
+    for step in (0, 1, 2, 3, 4, -1):
+        c, kr = torch.randn(n, L, generator=g, device="cuda"), torch.zeros(n, R, device="cuda")
+        kr[:, 0] = 2.0 ** 10
+        kr[:, 1] = (7 + step * (torch.arange(n, device="cuda") // 64 % 4)) * unit / 4.0
+        cache = LatentCache.alloc(n, 1, L, R)
+        cache.data[:, 0] = O.pack_rows(c, kr)
+        table = torch.arange(n, dtype=torch.int32, device="cuda")[None]
+        q = torch.zeros(1, 1, heads, L + R, device="cuda")
+        q[..., L], q[..., L + 1] = 2.0 ** (e - 10), 4.0
+        q = q.to(dt)
+        kv_len = torch.tensor([n], dtype=torch.int32, device="cuda")
+        out = latent_attention_decode(q, cache, table, kv_len, _unit_scale())
+        k = torch.cat(O.unpack_rows(cache.data[:, 0], L, R), 1)
+        z = (q[0, 0].double() @ k.T) * math.log(2.0)
+        p = torch.softmax(z, -1)
+        _check(out, (p @ k[:, :L])[None, None], (p @ k[:, :L].abs())[None, None], u, 2.0 ** -11, 2.0 ** -18, L + R, True)
