@@ -611,14 +611,23 @@ extern "C" size_t vq2_latent_decode_workspace_size(int B, int T, int heads, int 
   return most;
 }
 
+static bool ld_sizes_ok(int B, int T, int heads, int max_pages, int page_size) {
+  if (B <= 0 || T <= 0 || heads <= 0 || page_size <= 0 || max_pages <= 0 || (long long)T * heads > 1 << 20 ||
+      (long long)B * ((long long)T * heads + 64) >= 1LL << 27)
+    return false;
+  // positions (tiles of all query blocks in order) are 32-bit numbers
+  return (double)B * (((double)max_pages * page_size + LD_TILE - 1) / LD_TILE) * ((double)T * heads / 16 + 1) < 2147483648.;
+}
+
+extern "C" int vq2_latent_decode_query_rows(int B, int T, int heads, int max_pages, int page_size, int dtype) {
+  if (!ld_sizes_ok(B, T, heads, max_pages, page_size) || (dtype != VQ2_DT_BF16 && dtype != VQ2_DT_F16)) return 0;
+  return ld_nq(B, T, heads, (long long)max_pages * page_size, dtype == VQ2_DT_F16);
+}
+
 extern "C" int vq2_latent_decode(const vq2_latent_decode_args* a, void* ws, size_t ws_bytes, void* stream) {
   if (!a || !a->q || !a->cache || !a->block_table || !a->kv_len || !a->out) return VQ2_ERR_NULL;
-  if (a->B <= 0 || a->T <= 0 || a->heads <= 0 || a->page_size <= 0 || a->max_pages <= 0 || a->pages <= 0 ||
-      !latent_dims_ok(a->latent_dim, a->rope_dim) || !(a->scale > 0.f) || (long long)a->T * a->heads > 1 << 20 ||
-      (long long)a->B * ((long long)a->T * a->heads + 64) >= 1LL << 27)
-    return VQ2_ERR_SHAPE;
-  // positions (tiles of all query blocks in order) are 32-bit numbers
-  if ((double)a->B * (((double)a->max_pages * a->page_size + LD_TILE - 1) / LD_TILE) * ((double)a->T * a->heads / 16 + 1) >= 2147483648.)
+  if (a->pages <= 0 || !latent_dims_ok(a->latent_dim, a->rope_dim) || !(a->scale > 0.f) ||
+      !ld_sizes_ok(a->B, a->T, a->heads, a->max_pages, a->page_size))
     return VQ2_ERR_SHAPE;
   if (a->dtype != VQ2_DT_BF16 && a->dtype != VQ2_DT_F16) return VQ2_ERR_DTYPE;
   if (((uintptr_t)a->q | (uintptr_t)a->cache | (uintptr_t)a->out) & 15) return VQ2_ERR_ALIGN;

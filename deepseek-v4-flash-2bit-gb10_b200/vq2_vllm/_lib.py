@@ -122,6 +122,7 @@ _SIGS = {
     "vq2_latent_cache_read": (ctypes.c_int, [ctypes.POINTER(Vq2LatentCache), ctypes.c_void_p, ctypes.c_int, ctypes.c_int,
                                              ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
     "vq2_latent_decode_workspace_size": (ctypes.c_size_t, [ctypes.c_int] * 5),
+    "vq2_latent_decode_query_rows": (ctypes.c_int, [ctypes.c_int] * 6),
     "vq2_latent_decode": (ctypes.c_int, [ctypes.POINTER(Vq2LatentDecodeArgs), ctypes.c_void_p, ctypes.c_size_t,
                                          ctypes.c_void_p]),
     "vq2_latent_prefill_workspace_size": (ctypes.c_size_t, [ctypes.c_int] * 6),

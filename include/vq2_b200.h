@@ -294,6 +294,9 @@ typedef struct vq2_latent_decode_args {
   void* out;                     /* [B][T][heads][latent_dim] */
 } vq2_latent_decode_args;
 size_t vq2_latent_decode_workspace_size(int B, int T, int heads, int latent_dim, int rope_dim);
+/* Query rows that a block of the kernel for such a call takes: 16 (few query rows, or few tiles of cached rows by the table's
+   width, whatever kv_len holds), 32 or 64; 0 for sizes that vq2_latent_decode refuses. */
+int vq2_latent_decode_query_rows(int B, int T, int heads, int max_pages, int page_size, int dtype);
 int vq2_latent_decode(const vq2_latent_decode_args* a, void* workspace, size_t ws_bytes, void* stream);
 
 /* Expanded form: causal attention of a ragged batch of prompt chunks over per-head keys and values.

@@ -123,3 +123,12 @@ def test_a_captured_workspace_outlives_a_larger_one(monkeypatch):
     assert first() is not None and second() is not first()
     _lib.workspace(1 << 22, dev, stream)
     assert second() is None and first() is not None
+
+
+def test_which_decode_kernel_a_call_takes():
+    """16 query rows a block for few rows or few tiles (counted by the table's width), else 32 or, in bf16, 64."""
+    from vq2_vllm import _lib
+    rows = _lib.lib().vq2_latent_decode_query_rows
+    assert rows(64, 1, 16, 128, 64, 0) == 16 and rows(1, 1, 64, 5, 64, 0) == 16 and rows(1, 1, 64, 370, 64, 0) == 16
+    assert rows(1, 1, 64, 371, 64, 0) == 64 and rows(1, 1, 64, 371, 64, 1) == 32 and rows(1, 1, 32, 1000, 64, 0) == 32
+    assert rows(0, 1, 16, 8, 64, 0) == 0 and rows(1, 1, 16, 8, 64, 2) == 0 and rows(1, 1, 16, 1 << 30, 1 << 10, 0) == 0

@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_latent_gpu import DT, _check, _gen
+from test_latent_gpu import DT, _cache_for, _check, _dz, _gen
 
 pytestmark = pytest.mark.gpu
 
@@ -93,3 +93,131 @@ def test_a_nan_row_is_not_forgotten_where_the_next_tiles_lack_it(T, heads):
         cache.data.copy_(data)
         assert torch.isfinite(latent_attention_decode(q, cache, wide, kv_len, 0.1)).all()
     assert _lib.lib().vq2_device_status(1) == 2          # the missing pages
+
+
+# ------------------------------------------------------------------------------- against the definition
+def _wide(q, table, page, nq):
+    """The table as wide as the kernel for `nq` query rows a block needs it, and a check that the call takes that one."""
+    from vq2_vllm import _lib
+    B, T, heads, _ = q.shape
+    lib, dt = _lib.lib(), {torch.bfloat16: 0, torch.float16: 1}[q.dtype]
+    rows = 64
+    while lib.vq2_latent_decode_query_rows(B, T, heads, -(-rows // page), page, dt) == 16 and rows < 1 << 22:
+        rows += 64
+    table = _widen(table, page, max(rows, table.shape[1] * page))
+    assert lib.vq2_latent_decode_query_rows(B, T, heads, table.shape[1], page, dt) == nq
+    return table
+
+
+def _case(lens, T, heads, L, R, page, dtype, seed, nq, q_scale=1.0, spread=1.0, scale=None):
+    from oracle import latent_ref as O
+    from vq2_vllm.kernels.latent_attention import latent_attention_decode
+    dt, u = DT[dtype]
+    cache, table, kv_len = _cache_for(lens, L, R, page, dt, seed, spread)
+    q = (torch.randn(len(lens), T, heads, L + R, generator=_gen(seed + 1), device="cuda") * q_scale).to(dt)
+    scale = (L // 4 + R) ** -0.5 if scale is None else scale
+    table = _wide(q, table, page, nq)
+    out = latent_attention_decode(q, cache, table, kv_len, scale)
+    assert out.dtype == dt and out.shape == (len(lens), T, heads, L)
+    ref, absolute = O.decode(q, cache.data, table, kv_len, scale, L, R)
+    _check(out, ref, absolute, u, 2.0 ** -11, _dz(q, cache, table, kv_len, scale, L, R), L + R, True)
+    return q, cache, table, kv_len, scale, out
+
+
+SIZES = [
+    # lens, T, heads, L, R, page
+    ([1], 1, 17, 64, 0, 1),
+    ([64], 1, 32, 512, 64, 64),                          # exactly one tile
+    ([65, 63, 0, 1], 2, 16, 512, 64, 64),                # one over, one under, empty, one row
+    ([2, 40, 3, 0, 200], 4, 5, 192, 8, 16),              # fewer rows than new tokens
+    ([5000, 17], 1, 24, 448, 64, 1),                     # single-row pages
+    ([1000, 900, 800], 3, 9, 320, 40, 7),
+    ([20000], 1, 32, 512, 0, 64),                        # some 2 tiles a block
+    ([70000, 3], 2, 16, 64, 16, 48),                     # 8 tiles a block, a block with both sequences
+    ([129, 700, 0, 0, 31, 2000] * 4, 1, 20, 128, 16, 16),
+]
+MORE = [
+    ([1], 1, 33, 64, 0, 1),
+    ([64], 1, 64, 512, 64, 64),
+    ([65, 63, 0, 1], 3, 64, 512, 64, 64),
+    ([2, 40, 3, 0, 200], 7, 5, 192, 8, 16),
+    ([5000, 17], 1, 65, 448, 64, 1),
+    ([1000, 900, 800], 2, 96, 320, 40, 7),
+    ([20000], 1, 64, 512, 0, 64),
+    ([70000, 3], 2, 32, 64, 16, 48),
+    ([129, 700, 0, 0, 31, 2000] * 4, 1, 40, 128, 16, 16),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("lens,T,heads,L,R,page", SIZES)
+def test_up_to_32_query_rows(dtype, lens, T, heads, L, R, page):
+    _case(lens, T, heads, L, R, page, dtype, sum(lens) + heads, 32)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("lens,T,heads,L,R,page", MORE)
+def test_more_than_32_query_rows(dtype, lens, T, heads, L, R, page):
+    _case(lens, T, heads, L, R, page, dtype, sum(lens) + heads, 64 if dtype == "bf16" else 32)
+
+
+@pytest.mark.parametrize("heads,nq", [(16, 32), (30, 64)])
+@pytest.mark.parametrize("q_scale,spread,scale", [(20.0, 1.0, 0.1), (1e-3, 1.0, None), (1.0, 50.0, 1e-3), (300.0, 1.0, 1e-3),
+                                                  (1.0, 0.02, 1.0)])
+def test_peaked_flat_large_and_small_values(heads, nq, q_scale, spread, scale):
+    _case([30777, 130], 2, heads, 512, 64, 64, "bf16", 21, nq, q_scale=q_scale, spread=spread, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads", [16, 30])
+@pytest.mark.parametrize("L", [64, 320])
+def test_rising_and_falling_logits(dtype, heads, L):
+    """Logits that rise from tile to tile, within a block's tiles too: O is rescaled each time."""
+    from oracle import latent_ref as O
+    from vq2_vllm.kernels.latent_attention import latent_attention_decode
+    dt, u = DT[dtype]
+    R, n, page, scale = 16, 64 * 148 * 5 + 9, 32, 0.5
+    cache, table, kv_len = _cache_for([n], L, R, page, dt, 31)
+    at = torch.arange(n, device="cuda")
+    kr = torch.zeros(n, R, device="cuda")
+    kr[:, 0] = (at % 1024).float() / 8
+    cache.data.view(-1, cache.data.shape[2])[table[0, at // page].long() * page + at % page] = \
+        O.pack_rows(torch.randn(n, L, generator=_gen(32), device="cuda"), kr)
+    for sign in (1.0, -1.0):
+        q = torch.randn(1, 2, heads, L + R, generator=_gen(33), device="cuda").to(dt)
+        q[..., L] = sign * 4.0
+        wide = _wide(q, table, page, 64 if dtype == "bf16" and heads == 30 else 32)
+        out = latent_attention_decode(q, cache, wide, kv_len, scale)
+        ref, absolute = O.decode(q, cache.data, wide, kv_len, scale, L, R)
+        _check(out, ref, absolute, u, 2.0 ** -11, _dz(q, cache, wide, kv_len, scale, L, R), L + R, True)
+
+
+@pytest.mark.parametrize("heads,nq", [(8, 32), (30, 64)])
+def test_nan_reaches_only_its_readers(heads, nq):
+    from vq2_vllm.kernels.latent_attention import latent_attention_decode
+    cache, table, kv_len = _cache_for([300, 250], 128, 16, 64, torch.bfloat16, 51)
+    q = torch.randn(2, 3, heads, 144, generator=_gen(52), device="cuda").bfloat16()
+    table = _wide(q, table, 64, nq)
+    before = latent_attention_decode(q, cache, table, kv_len, 0.1)
+    cache.data[table[1, 3], 249 - 192] = 255                     # the newest row of sequence 1: its last token sees it
+    out = latent_attention_decode(q, cache, table, kv_len, 0.1)
+    assert torch.equal(out[0], before[0]) and torch.equal(out[1, :2], before[1, :2])
+    assert out[1, 2].isnan().all() and torch.isfinite(before).all()
+
+
+@pytest.mark.parametrize("heads,nq", [(24, 32), (64, 64)])
+def test_repeats_bit_for_bit_on_another_stream_and_in_a_graph(heads, nq):
+    from vq2_vllm.kernels.latent_attention import latent_attention_decode
+    q, cache, table, kv_len, scale, out = _case([30000, 300, 0, 1], 1, heads, 512, 64, 64, "bf16", 61, nq)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        again = latent_attention_decode(q, cache, table, kv_len, scale)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(out, again)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = latent_attention_decode(q, cache, table, kv_len, scale)
+    kv_len.copy_(torch.tensor([4000, 0, 0, 1], dtype=torch.int32))        # lengths move between replays
+    g.replay()
+    assert torch.equal(got, latent_attention_decode(q, cache, table, kv_len, scale))
