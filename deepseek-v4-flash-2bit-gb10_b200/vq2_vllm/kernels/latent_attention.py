@@ -68,9 +68,9 @@ def latent_attention_decode(q: torch.Tensor, cache: LatentCache, block_table: to
             q = q.clone(memory_format=torch.contiguous_format)
         lib, stream = _lib.lib(), _lib.raw_stream(dev)
         ws = _lib.workspace(_workspace_size(B, T, heads, L, R), q.device, stream)
-        pages, page_size, _ = cache.data.shape
-        a = _lib.Vq2LatentDecodeArgs(B, T, heads, L, R, page_size, block_table.shape[1], _DT[q.dtype], pages, scale, q.data_ptr(),
-                                     cache.args.data, block_table.data_ptr(), kv_len.data_ptr(), out.data_ptr())
+        k = cache.args
+        a = _lib.Vq2LatentDecodeArgs(B, T, heads, L, R, k.page_size, block_table.shape[1], _DT[q.dtype], k.pages, scale, q.data_ptr(),
+                                     k.data, block_table.data_ptr(), kv_len.data_ptr(), out.data_ptr())
         rc = lib.vq2_latent_decode(a, ws.data_ptr(), ws.numel(), stream)
     _lib.check(rc, "vq2_latent_decode")
     return out

@@ -26,18 +26,32 @@ def latent_row_bytes(latent_dim: int, rope_dim: int) -> int:
 
 class LatentCache:
     """A paged latent cache: ``data`` u8 [pages, page_size, row_bytes], contiguous, on the GPU. Any
-    page size >= 1. A slot is ``page * page_size + place``. ``LatentCache.alloc`` makes one."""
+    page size >= 1. A slot is ``page * page_size + place``. ``LatentCache.alloc`` makes one. Another tensor may be assigned to
+    ``data`` (a grown pool); it is checked like the first, and calls use it from then on. The dimensions stay."""
 
-    __slots__ = ("data", "latent_dim", "rope_dim", "args")
+    __slots__ = ("_data", "_latent_dim", "_rope_dim", "args")
 
     def __init__(self, data: torch.Tensor, latent_dim: int, rope_dim: int):
-        rb = latent_row_bytes(latent_dim, rope_dim)
+        self._latent_dim, self._rope_dim = latent_dim, rope_dim
+        self.data = data
+
+    latent_dim = property(lambda self: self._latent_dim)
+    rope_dim = property(lambda self: self._rope_dim)
+
+    @property
+    def data(self) -> torch.Tensor:
+        return self._data
+
+    @data.setter
+    def data(self, data: torch.Tensor):
+        L, R = self._latent_dim, self._rope_dim
+        rb = latent_row_bytes(L, R)
         if data.dtype != torch.uint8 or data.dim() != 3 or data.shape[2] != rb or not data.is_contiguous():
             raise ValueError(f"vq2 latent cache: contiguous uint8 [pages, page_size, {rb}] expected")
         if data.shape[0] < 1 or data.shape[1] < 1:
             raise ValueError("vq2 latent cache: at least one page of at least one row expected")
-        self.data, self.latent_dim, self.rope_dim = data, latent_dim, rope_dim
-        self.args = _lib.Vq2LatentCache(data.data_ptr(), data.shape[0], data.shape[1], latent_dim, rope_dim)
+        # what the calls pass on: the pointer and the sizes of one and the same tensor
+        self._data, self.args = data, _lib.Vq2LatentCache(data.data_ptr(), data.shape[0], data.shape[1], L, R)
 
     @classmethod
     def alloc(cls, pages: int, page_size: int, latent_dim: int, rope_dim: int, device="cuda") -> "LatentCache":

@@ -132,3 +132,21 @@ def test_which_decode_kernel_a_call_takes():
     assert rows(64, 1, 16, 128, 64, 0) == 16 and rows(1, 1, 64, 5, 64, 0) == 16 and rows(1, 1, 64, 370, 64, 0) == 16
     assert rows(1, 1, 64, 371, 64, 0) == 64 and rows(1, 1, 64, 371, 64, 1) == 32 and rows(1, 1, 32, 1000, 64, 0) == 32
     assert rows(0, 1, 16, 8, 64, 0) == 0 and rows(1, 1, 16, 8, 64, 2) == 0 and rows(1, 1, 16, 1 << 30, 1 << 10, 0) == 0
+
+
+def test_calls_use_the_tensor_that_the_cache_has_now():
+    """A pool that is assigned anew is the one the calls point to; a tensor that does not fit is refused and changes nothing."""
+    from vq2_vllm.kernels.latent_cache import LatentCache
+    cache = LatentCache.alloc(2, 8, 128, 16, device="cpu")
+    grown = torch.zeros(5, 16, 112, dtype=torch.uint8)
+    cache.data = grown
+    assert cache.data is grown
+    assert (cache.args.data, cache.args.pages, cache.args.page_size) == (grown.data_ptr(), 5, 16)
+    for bad in (torch.zeros(5, 16, 96, dtype=torch.uint8), grown[:, ::2], grown[:0], grown.char()):
+        with pytest.raises(ValueError):
+            cache.data = bad
+    assert cache.data is grown and cache.args.data == grown.data_ptr()
+    for name in ("latent_dim", "rope_dim"):          # the kernels' sizes were checked against them
+        with pytest.raises(AttributeError):
+            setattr(cache, name, 64)
+    assert (cache.latent_dim, cache.rope_dim) == (128, 16)
