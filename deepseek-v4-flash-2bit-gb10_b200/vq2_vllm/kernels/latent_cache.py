@@ -66,12 +66,14 @@ def _slots(slots: torch.Tensor):
 
 
 def _rows(x: torch.Tensor):
-    """x [N, D] as rows the kernels can load 16 bytes at a time (a copy only where they cannot)."""
-    if x.data_ptr() % 16 or not x.is_contiguous():        # contiguous rows of a multiple of 8 values always serve
-        s0, s1 = x.stride()
-        if x.data_ptr() % 16 or s1 != 1 or s0 < x.shape[1] or s0 % 8:
-            x = x.clone(memory_format=torch.contiguous_format)
-    return x
+    """x [N, D] as rows the kernels can load 16 bytes at a time (a copy only where they cannot), and their stride."""
+    if x.is_contiguous():                  # (of a single row the tensor's own stride may be anything)
+        return x if x.data_ptr() % 16 == 0 else x.clone(), x.shape[1]
+    s0, s1 = x.stride()
+    if x.data_ptr() % 16 or s1 != 1 or s0 < x.shape[1] or s0 % 8:
+        x = x.clone(memory_format=torch.contiguous_format)
+        s0 = x.shape[1]
+    return x, s0
 
 
 def latent_cache_write(cache: LatentCache, c: torch.Tensor, k_rope: torch.Tensor | None, slots: torch.Tensor) -> None:
@@ -96,12 +98,12 @@ def latent_cache_write(cache: LatentCache, c: torch.Tensor, k_rope: torch.Tensor
     if not N:
         return
     with _lib.on_device(dev):
-        c = _rows(c)
+        c, c_stride = _rows(c)
+        rope_stride = 0
         if R:
-            k_rope = _rows(k_rope)
-        rc = _lib.lib().vq2_latent_cache_write(cache.args, c.data_ptr(), k_rope.data_ptr() if R else None, dt, c.stride(0),
-                                               k_rope.stride(0) if R else 0, slots.data_ptr(), _lib.ID[slots.dtype], N,
-                                               _lib.raw_stream(dev))
+            k_rope, rope_stride = _rows(k_rope)
+        rc = _lib.lib().vq2_latent_cache_write(cache.args, c.data_ptr(), k_rope.data_ptr() if R else None, dt, c_stride, rope_stride,
+                                               slots.data_ptr(), _lib.ID[slots.dtype], N, _lib.raw_stream(dev))
     _lib.check(rc, "vq2_latent_cache_write")
 
 

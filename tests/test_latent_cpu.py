@@ -150,3 +150,16 @@ def test_calls_use_the_tensor_that_the_cache_has_now():
         with pytest.raises(AttributeError):
             setattr(cache, name, 64)
     assert (cache.latent_dim, cache.rope_dim) == (128, 16)
+
+
+def test_strides_of_rows():
+    """What the write entry is given: rows on 16-byte boundaries, a stride of whole 16 bytes that is no less than the row. The stride
+    that a tensor of one row happens to have does not count."""
+    from vq2_vllm.kernels.latent_cache import _rows
+    x = torch.randn(6, 577)
+    one = torch.randn(600).as_strided((1, 512), (3, 1))
+    for rows in (x[:1, :512], x[2:3, 1:513], x[3:4, 4:516], x[:, :512], x[:, 1:513], x[::2, :64], torch.randn(512, 1).T, torch.randn(512, 4).T,
+                 one, torch.randn(6, 576)[:, :512], torch.randn(1, 512), torch.randn(512).expand(3, 512), torch.randn(4, 0)):
+        got, stride = _rows(rows)
+        assert torch.equal(got, rows) and got.data_ptr() % 16 == 0 and stride % 8 == 0 and stride >= rows.shape[1]
+        assert got.numel() == 0 or torch.equal(torch.as_strided(got, rows.shape, (stride, 1)), rows) or rows.shape[0] == 1
