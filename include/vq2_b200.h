@@ -267,8 +267,8 @@ typedef struct vq2_latent_cache {
 size_t vq2_latent_row_bytes(int latent_dim, int rope_dim);   /* 0 for unsupported dimensions */
 /* Quantise rows c[i * c_stride ..] and k_rope[i * rope_stride ..] (VQ2_DT_*, strides in elements,
    multiples of 8, 16-byte aligned bases) into slots[i] (VQ2_ID_*), i < n. A negative slot is skipped
-   (padding); one beyond the cache is skipped and vq2_device_status reports VQ2_ERR_SHAPE. Slots that
-   occur twice hold either row. */
+   (padding); one beyond the cache is skipped and vq2_device_status reports VQ2_ERR_SHAPE. The slots of one call differ: a row is
+   written by many threads, so one that occurs twice may end as a mixture of both rows. */
 int vq2_latent_cache_write(const vq2_latent_cache* cache, const void* c, const void* k_rope, int dtype, long long c_stride,
                            long long rope_stride, const void* slots, int slot_dtype, int n, void* stream);
 /* What slots[i] stand for: c [n][L] (32-byte aligned) and k_rope [n][R] of VQ2_DT_* (zeros for a slot that write
