@@ -5,7 +5,7 @@
 // kernel rotates the query and the result, never a cached row.
 //
 // Both products run on tcgen05 with the cached rows as the wide operand and NQ = 32 or 64 query
-// rows (heads x tokens of one sequence) as the narrow one (up to 16 rows have a kernel of their own):
+// rows (heads x tokens of one sequence) as the narrow one (up to 16 rows, and calls with few tiles, have a kernel of their own: ld_nq):
 //   S^T [64 cached x NQ] = K Q^T       K tile in shared memory, rows = cached rows (K-major)
 //   O^T [L x NQ]        += V^T P^T     the same tile read along the other direction (MN-major): the
 //                                      latent is key and value, expanded from 4 bits once for both
@@ -22,11 +22,12 @@
 // L1 have too few lines to be in flight beside 220 KB of shared memory); 16 worker warps expand a tile of 64 rows and do its softmax;
 // one thread issues the products. Both products are bound by reading the tile from shared memory, so that
 // path is kept busy: a tile is handed over in parts of 128 latent values, S starts on the first part, and
-// a part is filled again as soon as P V has used it. Up to 32 query rows there is room for two tiles, and the softmax of a
-// tile runs under the products of the next. In the steady state no barrier spans the block.
-// What bounds it: with 64 query rows there is room for one tile, so its expansion, S, softmax and P V follow one another: 5,300
+// a part is filled again as soon as P V has used it. With 32 query rows in one term (bf16) there is room for two tiles, and the softmax of
+// a tile runs under the products of the next. In the steady state no barrier spans the block.
+// What bounds it: with 64 query rows, or 32 in two terms (fp16), there is room for one tile, so its expansion, S, softmax and P V follow one another: 5,300
 // cycles a tile, where the products take 2,040 (36 of S at 34 cycles, 16 of P V at 51, measured alone) and the matrix units
-// need 1,088 of those. 4 sequences of 65,536 rows, 64 query rows: 115 us a call, DRAM 13 % and tensor pipe 30 % busy.
+// need 1,088 of those. 4 sequences of 65,536 rows, 64 query rows: 115 us a call, DRAM 13 % and tensor pipe 30 % busy;
+// 32 query rows 88 us.
 #include <algorithm>
 #include "latent_decode.cuh"
 
@@ -522,11 +523,12 @@ __global__ void __launch_bounds__(LD_THREADS, 1) latent_decode_kernel(LdArgs g) 
 }
 
 // Query rows a block, by the rows of a sequence. Up to 16 the narrow kernel; up to 32, or more, the wide one with that many
-// (64 sequences, 320,206 cached rows: 16 query rows 84 us narrow, 151 us with 64 wide; 32 rows 122 us with 32 wide, 141 us as two
-// narrow blocks, 151 us with 64 wide; 48 rows 158 us with 64 wide, 201 us narrow). Where the narrow kernel's blocks have at most 5
-// tiles each, time is mostly latency, and it has less of it (64 rows of 8 sequences: 2048 cached rows each 31 us, 36 us wide;
-// 4096 each 43 and 42 us; 64 rows of one sequence, 64 cached: 11 and 18 us). fp16 queries in two terms take the room of 64 rows with
-// 32 (4 sequences of 65,536 rows, 64 heads: 166 us, bf16 113; 64 sequences, 16 heads, narrow: 95 and 80).
+// (64 sequences, 320,206 cached rows: 16 query rows 81 us narrow, 116 with 32 wide, 144 with 64; 32 rows 120 us with 32 wide, 138 as two
+// narrow blocks, 148 with 64 wide; 48 rows 154 us with 64 wide, 195 narrow, 200 with 32). Where the narrow kernel's blocks have at most 5
+// tiles each, time is mostly latency, and it has less of it (in graphs, 64 rows of 8 sequences: 2048 cached rows each 32 us, 37 wide;
+// 4096 each 44 and 43 us; 64 rows of one sequence, 64 cached: 11 and 17 us). fp16 queries in two terms take the room of 64 rows with
+// 32 (4 sequences of 65,536 rows, 64 heads: 168 us, bf16 115; 64 sequences, 16 heads, narrow: 97 and 81). The rule goes by the table's
+// width, as the lengths are on the device: a table far wider than they are takes the wide kernel where the narrow one would be faster.
 static int ld_nq(int B, int T, int heads, long long most, bool two) {
   const long long rows = (long long)T * heads;
   return rows <= 16 || (double)B * ((most + LD_TILE - 1) / LD_TILE) * ((rows + 15) / 16) <= 5 * 2 * 148 ? 16 : two || rows <= 32 ? 32 : 64;

@@ -22,8 +22,8 @@
 // them (below: lp_split).
 // What bounds it: the products of a step (two tiles, 128 keys) take 2560 cycles, the step about 3400: 1700 for a
 // tile's softmax (1024 of them its exponentials) and the hand-overs before and after it, under which only the other tile's
-// products run. 8192 tokens, 32 heads, 128 + 64 and 128 values: 0.605 ms, 1135 TFLOP/s, at the power limit; the library's plain
-// bf16 product of 8192^3 sustains 1395 there.
+// products run. 8192 tokens, 32 heads, 128 + 64 and 128 values: 0.61 ms, 1125 TFLOP/s, at the power limit (fp16 draws more there:
+// 0.62 where bf16 takes 0.59); the library's plain bf16 product of 8192^3 sustains 1395.
 // A key that a row does not see has probability 0; a NaN or an infinity in its value reaches the row all the same (0 times
 // NaN) if both are in one step of 128 keys of one sequence, but never another sequence's rows.
 #include <algorithm>
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(LPJ_ROWS * 16) latent_prefill_join_kernel(vq2_
   float n = -INFINITY, l = 0.f, v[8] = {};
 #pragma unroll 4
   for (int s = 0; s < count; ++s) {
-    // (reads through L2: this kernel may have started while the main one was still writing)
+    // (the main kernel is done: it never signals early, so this launch is only prepared while it runs; each value is read once)
     const size_t slot = ((size_t)block * parts.most + s) * (2 * LP_TILE) + r;
     const float2 ml = __ldcg(parts.ml + slot);
     const float4* p = (const float4*)(parts.o + slot * (VU * 64) + d);

@@ -302,7 +302,8 @@ int vq2_latent_decode(const vq2_latent_decode_args* a, void* workspace, size_t w
 /* Expanded form: causal attention of a ragged batch of prompt chunks over per-head keys and values.
    Sequence b: query rows cu_q[b] .. cu_q[b+1]-1, key rows cu_k[b] .. cu_k[b+1]-1 (a prefix first, then
    the chunk's own): query i sees keys j <= i + keys - queries, so the last query sees all; a row that
-   sees nothing gives zeros. Key of head h: [k_nope[:, h], k_rope], the rotary part shared by the heads.
+   sees nothing gives zeros. A NaN or an infinity in a value may reach rows of its own sequence that do not see it but whose step of
+   128 keys it is in. Key of head h: [k_nope[:, h], k_rope], the rotary part shared by the heads.
    Strides in elements (multiples of 8; the last dimension is contiguous); max_q >= every
    sequence's query rows. With a workspace of the size below, calls with few blocks of queries split their
    keys over the SMs; without one (or where that size is 0) they do not. */
