@@ -108,7 +108,8 @@ class LatentLayer:
         latent_cache_write(cache, c, k_rope if self.R else None, slots)
         B = kv_len.shape[0]
         q_c = torch.einsum("thd,hdl->thl", q[..., : self.nope], self.w_uk)
-        o = latent_attention_decode(torch.cat((q_c, q[..., self.nope:]), -1).view(B, -1, self.heads, self.L + self.R), cache,
+        T = x.shape[0] // max(B, 1)
+        o = latent_attention_decode(torch.cat((q_c, q[..., self.nope:]), -1).view(B, T, self.heads, self.L + self.R), cache,
                                     block_table, kv_len, self.scale)
         return torch.einsum("thl,hld->thd", o.view(-1, self.heads, self.L), self.w_uv).reshape(-1, self.heads * self.dv)
 
@@ -117,6 +118,8 @@ class LatentLayer:
         """Router, routed experts and, where the layer has one, the shared expert -> fp32 [N, H]."""
         h = rms_norm(x, self.norm_ffn)
         N = h.shape[0]
+        if not N:                              # a step without tokens
+            return h.float()
         if N <= _ROUTER_MAX:
             ids, w = router_topk(h, self.w_r, self.topk)
         else:
